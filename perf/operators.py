@@ -114,7 +114,8 @@ def _int8_inputs(c, g):
     # activations: normal, with a few channels an order larger, as after a norm
     x = torch.randn(m, k, generator=g, device=DEV)
     x *= 1 + 12 * (torch.rand(k, generator=g, device=DEV) < 0.01)
-    codes = torch.empty(n, k, device=DEV, dtype=torch.int8)
+    # rows of codes start on 16-byte boundaries, as a weight is laid out once
+    codes = torch.zeros(n, -(-k // 16) * 16, device=DEV, dtype=torch.int8)[:, :k]
     for i in range(0, n, 16384):  # weights as codes: a normal row against its largest entry
         part = torch.randn(min(16384, n - i), k, generator=g, device=DEV) * (127 / 4.2)
         codes[i:i + 16384] = part.round().clamp(-127, 127).to(torch.int8)
