@@ -224,9 +224,10 @@ def prepare(case, seed):
 def _int8_plain(s):
     x = s["x"].float()
     top = x.abs().amax(-1, keepdim=True)
-    codes = torch.round(x * (127 / top))
+    n = torch.full_like(top, 127)  # a true division, which number / tensor is not
+    codes = torch.round(x * (n / top))
     y = codes @ s["w"].float().t()
-    y = y * (top / 127 * s["ws"])
+    y = y * (top / n * s["ws"])
     if s["bias"] is not None:
         y = y + s["bias"].float()
     return y.to(s["x"].dtype)
@@ -427,9 +428,10 @@ def exact(case, seed):
     # codes and scales are held in 32 and 8 bits by definition; all else in 64
     x = s["x"].double()
     top = x.abs().amax(-1, keepdim=True)
-    inv = (127.0 / top).float().double()
+    n = torch.full_like(top, 127)
+    inv = (n / top).float().double()
     codes = (x * inv).float().round().double()
-    scale = (top / 127.0).float().double()
+    scale = (top / n).float().double()
     w, ws = s["w"], s["ws"].double()
     y = torch.empty(c["m"], c["n"], device=DEV, dtype=torch.float64)
     for i in range(0, c["n"], 8192):
