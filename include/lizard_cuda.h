@@ -498,6 +498,103 @@ int lz_swa_decode(const void* q, const void* k, const void* v, int x_dtype,
                   const int* pos, const float* meta, int n_meta, void* y,
                   int B, int H, int Hkv, int window, int D, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* Drafted decoding: blocks of tokens, verification, 8-bit products         */
+/* ------------------------------------------------------------------------ */
+/* No counterpart in the reference, which has no cache and no decoding. */
+
+/* A block of T new tokens (0..64) through the GLA state, the state left at the
+ * accepted prefix: first the state advances in place by the first count[b]
+ * tokens (clamped to 0..T_prev; null = all) of the previous block, fk_prev
+ * [B*Hkv, T_prev, F], v_prev [B*Hkv, T_prev, D], log_gamma_prev, then y
+ * [B*H, T, D] (bf16, 8-byte aligned) is what T single steps from there would
+ * give for fq [B*H, T, F], fk, v, log_gamma ([B, T], or [B*H, T] with
+ * gate_per_head); the block itself is not folded in. T = 0 only advances the
+ * state (fq, fk, v, log_gamma, y may be null), T_prev = 0 only reads it.
+ * state [B*Hs, F, D] and zstate [B*Hs, F] fp32, Hs as in lz_gla_decode,
+ * F <= 256, D a multiple of 4 up to 256. */
+int lz_gla_decode_block(const void* fq, const void* fk, const void* v,
+                        const float* log_gamma, int gate_per_head,
+                        const void* fk_prev, const void* v_prev, const float* log_gamma_prev,
+                        const int* count, float* state, float* zstate, void* y,
+                        int B, int H, int Hkv, int Hs, int T, int T_prev, int F, int D,
+                        void* stream);
+
+/* A block of T new tokens (0..64) through the sliding-window ring: first the
+ * first count[b] tokens of the previous block (k_prev, v_prev, rotated with
+ * cos_prev / sin_prev) are written to ring slots (pos[b] + t) % window, then y
+ * [B*H, T, D] (bf16) attends the block's tokens, at positions pos[b] +
+ * count[b] and on, to the ring and to the block's earlier tokens, with the
+ * sink logits. pos[b] counts the tokens the rings hold before the call; the
+ * caller advances it by count[b]. q, k, v (k_prev, v_prev) are read in place:
+ * strides = {batch, head, token} in elements for q, k, v in turn (9 values;
+ * strides_prev 6), host memory, last dimension contiguous; cos, sin [T, D] per
+ * batch row, cs_sb elements apart (0: one table for all). Rings fp32
+ * [B*Hkv, window, D], D even up to 256, window up to 1024. */
+int lz_swa_decode_block(const void* q, const void* k, const void* v, int x_dtype,
+                        const long long* strides, const void* cos, const void* sin,
+                        int cs_dtype, long long cs_sb,
+                        const void* k_prev, const void* v_prev, const long long* strides_prev,
+                        const void* cos_prev, const void* sin_prev, long long cs_prev_sb,
+                        const int* count, float* k_ring, float* v_ring, const int* pos,
+                        const float* meta, int n_meta, void* y,
+                        int B, int H, int Hkv, int T, int T_prev, int window, int D,
+                        void* stream);
+
+/* Verification of K drafted tokens (0..64) per sequence. With p_i, q_i the
+ * softmax of row i of the target / draft logits over the temperature, token i
+ * is accepted while uniforms[b, i] * q_i(token) < p_i(token); the token after
+ * the accepted ones is argmax_j max(p_j - q_j, 0) / noise[b, j] at a refusal
+ * (of p_j / noise[b, j] where that residual is empty) and argmax_j p_j /
+ * noise[b, j] after the last draft, ties to the lowest index: with uniforms in
+ * [0, 1) and noise from Exp(1) the tokens follow p. A temperature below 1e-5
+ * is greedy: a drafted token has to be the target's argmax (lowest index), the
+ * next token is the argmax. Logits that are -inf or NaN are masked; a token
+ * outside 0..V-1 is refused; next is -1 when the row (or its noise) leaves
+ * nothing. out_tokens [B, K + 1]: accepted tokens, the next one, then -1;
+ * accepted [B]: how many drafted tokens stand.
+ * target [B, K + 1, V] and draft [B, K, V] in x_dtype, strides in elements
+ * (batch, row), last dimension contiguous; noise fp32 [B, V], noise_sb apart;
+ * tokens and out_tokens int64 (tokens_64) or int32; temperature fp32 [B], or
+ * null for temperature_all; lengths int32 [B] (drafted tokens of each
+ * sequence, clamped to 0..K), or null for K. B * (2 K + 1) <= 65535. */
+size_t lz_verify_drafts_workspace_bytes(int B, int K, int V);
+int lz_verify_drafts(const void* target, long long target_sb, long long target_sr,
+                     const void* draft, long long draft_sb, long long draft_sr, int x_dtype,
+                     const void* tokens, int tokens_64, const float* uniforms,
+                     const float* noise, long long noise_sb, const float* temperature,
+                     float temperature_all, const int* lengths, void* out_tokens, int* accepted,
+                     void* workspace, size_t workspace_bytes, int B, int K, int V, void* stream);
+
+/* Row-wise symmetric quantisation of x [M, K] (rows x_ld elements apart):
+ * scale[m] = max|x| / 127 and codes[m, k] = rint(x * (127 / max|x|)), fp32
+ * arithmetic, ties to even; rows of codes are codes_ld bytes apart (a multiple
+ * of 16, codes 16-byte aligned) and zero beyond K. A row whose largest value is
+ * below 4e-37 counts as zero (scale 0); one that holds an infinity or NaN gets
+ * the scale NaN and zero codes, so every product with it is NaN. */
+int lz_int8_quantize(const void* x, int x_dtype, long long x_ld, void* codes,
+                     long long codes_ld, float* scale, int M, int K, void* stream);
+
+/* y[m, n] = (sum_k a[m, k] b[n, k]) * (a_scale[m] * b_scale[n]) + bias[n] over
+ * signed 8-bit codes with an exact 32-bit sum (K <= 131071). Rows of a and b are
+ * a_ld / b_ld bytes apart; both should start on 16-byte boundaries (ld a
+ * multiple of 16), other layouts are repacked into the workspace first, which
+ * may be null when neither needs it. bias [N] (fp32 or bf16) may be null; y
+ * [M, N] contiguous fp32 or bf16. */
+size_t lz_int8_workspace_bytes(int M, int N, int K);
+int lz_int8_matmul(const void* a, long long a_ld, const float* a_scale,
+                   const void* b, long long b_ld, const float* b_scale,
+                   const void* bias, int bias_dtype, void* y, int y_dtype,
+                   void* workspace, size_t workspace_bytes, int M, int N, int K, void* stream);
+
+/* lz_int8_quantize of x and lz_int8_matmul with the weight codes w [N, K] in
+ * one call. Workspace: lz_int8_linear_workspace_bytes(M, K) when rows of w start
+ * on 16-byte boundaries, else lz_int8_workspace_bytes(M, N, K). */
+size_t lz_int8_linear_workspace_bytes(int M, int K);
+int lz_int8_linear(const void* x, int x_dtype, long long x_ld, const void* w, long long w_ld,
+                   const float* w_scale, const void* bias, int bias_dtype, void* y, int y_dtype,
+                   void* workspace, size_t workspace_bytes, int M, int N, int K, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

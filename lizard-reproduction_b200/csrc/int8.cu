@@ -1,0 +1,835 @@
+// Matrix product in 8-bit integers with one scale a token and one a channel:
+//   y[m, n] = (sum_k a[m, k] b[n, k]) * (sa[m] * sb[n]) + bias[n]
+// and the quantisation that feeds it, row by row:
+//   s = max_k |x_k| / 127,  code_k = rint(x_k * (127 / max))
+// (all in fp32; the product of x and the reciprocal is rounded once, then to the
+// nearest integer, ties to even). The integer sum is exact (K <= 131071 keeps it
+// inside 32 bits), so neither the order of the sum nor a split of K can change a
+// bit of y; what rounds is the conversion of the sum, the two products and the
+// bias, each once.
+//
+// Both products run on the 8-bit tensor cores (tcgen05 kind::i8, 32-bit integer
+// accumulators in TMEM, operands by TMA in 128-byte swizzled rows, K-major on
+// both sides, as activations and nn.Linear weights lie). Two kernels:
+//   narrow: few tokens. The weights stream once, so the kernel is bound by
+//     memory; weight rows take the 128 accumulator lanes (they are the long
+//     side) and 16 .. 128 tokens the columns. Where the tiles of N do not fill
+//     the machine, a cluster of 2 .. 8 CTAs splits K and adds its integer
+//     partials through distributed shared memory.
+//   wide: many tokens. Bound by the tensor cores. A pair of CTAs (cta_group::2)
+//     shares a 256 x 256 tile: each loads half of either operand, so a byte in
+//     shared memory feeds twice the math; two accumulators of 256 TMEM columns
+//     let the epilogue of a tile run under the next one's products.
+#include <algorithm>
+
+#include "common.cuh"
+#include "tc.cuh"
+
+namespace lz {
+namespace {
+
+constexpr int kMaxK = 131071;  // 128 * 128 * K < 2^31
+
+// ------------------------------------------------------------------ quantise
+constexpr int kQT = 256;   // threads a row
+constexpr int kQV = 4;     // 16-byte vectors a thread keeps
+
+template <typename T>
+struct Vec;
+template <>
+struct Vec<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ uint32_t top(const uint4& w) {  // largest |bits|
+    return max(max(w.x & 0x7fffffffu, w.y & 0x7fffffffu), max(w.z & 0x7fffffffu, w.w & 0x7fffffffu));
+  }
+  static __device__ __forceinline__ float value(const float* p) { return *p; }
+};
+template <>
+struct Vec<bf16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ uint32_t top(const uint4& w) {
+    constexpr uint32_t m = 0x7fff7fffu;
+    const uint32_t x = __vmaxu2(__vmaxu2(w.x & m, w.y & m), __vmaxu2(w.z & m, w.w & m));
+    return max(x & 0xffff0000u, x << 16);  // as fp32 bits
+  }
+  static __device__ __forceinline__ float value(const bf16* p) { return __bfloat162float(*p); }
+};
+
+// One code: the product rounded to fp32, then to an integer by adding 1.5 * 2^23.
+__device__ __forceinline__ uint32_t code_of(float x, float inv) {
+  return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.f));
+}
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+__device__ __forceinline__ void store_codes(int8_t* p, const uint4& w, float inv, float) {
+  *reinterpret_cast<uint32_t*>(p) =
+      pack4(code_of(__uint_as_float(w.x), inv), code_of(__uint_as_float(w.y), inv),
+            code_of(__uint_as_float(w.z), inv), code_of(__uint_as_float(w.w), inv));
+}
+__device__ __forceinline__ void store_codes(int8_t* p, const uint4& w, float inv, bf16) {
+  *reinterpret_cast<uint2*>(p) =
+      make_uint2(pack4(code_of(bf16_lo(w.x), inv), code_of(bf16_hi(w.x), inv),
+                       code_of(bf16_lo(w.y), inv), code_of(bf16_hi(w.y), inv)),
+                 pack4(code_of(bf16_lo(w.z), inv), code_of(bf16_hi(w.z), inv),
+                       code_of(bf16_lo(w.w), inv), code_of(bf16_hi(w.w), inv)));
+}
+
+// One CTA a row: the row is read once into registers (the part beyond kQT * kQV
+// vectors, and rows that do not start on 16 bytes, twice). The largest |x| is
+// taken on the bits, where infinities and NaN are larger than every number: such
+// a row gets the scale NaN, and so NaN outputs.
+template <typename T>
+__global__ void __launch_bounds__(kQT)
+i8_quantize_kernel(const T* __restrict__ x, long long ldx, int8_t* __restrict__ codes,
+                   long long ldc, float* __restrict__ scale, int K) {
+  using V = Vec<T>;
+  __shared__ uint32_t sTop[kQT / 32];
+  const int tid = threadIdx.x;
+  const T* row = x + (size_t)blockIdx.x * ldx;
+  int8_t* out = codes + (size_t)blockIdx.x * ldc;
+  const bool vec = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
+  const int nv = vec ? K / V::N : 0;
+  const uint4* rv = reinterpret_cast<const uint4*>(row);
+  uint4 keep[kQV];
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < kQV; ++i) {
+    const int at = tid + i * kQT;
+    keep[i] = at < nv ? rv[at] : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < kQV; ++i) top = max(top, V::top(keep[i]));
+  for (int at = tid + kQV * kQT; at < nv; at += kQT) top = max(top, V::top(rv[at]));
+  for (int k = nv * V::N + tid; k < K; k += kQT)
+    top = max(top, __float_as_uint(V::value(row + k)) & 0x7fffffffu);
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((tid & 31) == 0) sTop[tid >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kQT / 32; ++w) top = max(top, sTop[w]);
+  const float t = __uint_as_float(top);
+  // below 4e-37 the reciprocal leaves the fp32 range: the row counts as zero
+  const bool live = t >= 4e-37f && t < INFINITY;
+  const float inv = live ? 127.f / t : 0.f;
+  if (tid == 0)
+    scale[blockIdx.x] = live ? t / 127.f : (t < 1.f ? 0.f : __uint_as_float(0x7fc00000u));
+  if (!live) {
+    for (int k = tid; k < ldc; k += kQT) out[k] = 0;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < kQV; ++i) {
+    const int at = tid + i * kQT;
+    if (at < nv) store_codes(out + at * V::N, keep[i], inv, T());
+  }
+  for (int at = tid + kQV * kQT; at < nv; at += kQT) store_codes(out + at * V::N, rv[at], inv, T());
+  for (int k = nv * V::N + tid; k < K; k += kQT)
+    out[k] = (int8_t)(code_of(V::value(row + k), inv) & 0xffu);
+  for (int k = K + tid; k < ldc; k += kQT) out[k] = 0;
+}
+
+// Rows of codes that do not start on 16 bytes, copied to ones that do.
+__global__ void __launch_bounds__(kQT)
+i8_repack_kernel(const int8_t* __restrict__ x, long long ldx, int8_t* __restrict__ out,
+                 long long ldo, int K) {
+  const int8_t* row = x + (size_t)blockIdx.x * ldx;
+  int8_t* o = out + (size_t)blockIdx.x * ldo;
+  for (int k = threadIdx.x; k < ldo; k += kQT) o[k] = k < K ? row[k] : 0;
+}
+
+// ---------------------------------------------------------------------- PTX
+__device__ __forceinline__ void grid_dependency_wait() {
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+}
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
+}
+__device__ __forceinline__ void mma_i8_pair(uint32_t d, uint64_t adesc, uint64_t bdesc,
+                                            uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
+}
+// Signed 8-bit x signed 8-bit -> 32-bit integer, both operands K-major.
+__host__ __device__ constexpr uint32_t idesc_i8(int M, int N) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) |
+         ((uint32_t)(M >> 4) << 24);
+}
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int c0, int c1,
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3}], [%4];\n" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(smem_u32(bar))
+      : "memory");
+}
+// The same into this CTA's shared memory, completing on a barrier of the pair
+// (a shared::cluster address).
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, int c0, int c1,
+                                                 uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::"
+      "bytes [%0], [%1, {%2, %3}], [%4];\n" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int c0,
+                                             int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];\n" ::"l"(
+          reinterpret_cast<uint64_t>(map)),
+      "r"(smem_u32(src)), "r"(c0), "r"(c1)
+      : "memory");
+}
+// Arrive on the barrier at the same offset in both CTAs of the pair once every
+// MMA issued so far has completed.
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+      "[%0], %1;\n" ::"r"(smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void arrive_remote(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ int4 ld_cluster_int4(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::
+                   : "memory");
+}
+
+struct Out {  // y and what scales it
+  const float *sa, *sb;
+  const void* bias;  // [N] fp32 or bf16, or null
+  void* y;           // [M, N] contiguous, fp32 or bf16
+  int bias_bf16, y_bf16, M, N, K;
+};
+__device__ __forceinline__ float bias_at(const Out& o, int n) {
+  if (!o.bias) return 0.f;
+  return o.bias_bf16 ? __bfloat162float(static_cast<const bf16*>(o.bias)[n])
+                     : static_cast<const float*>(o.bias)[n];
+}
+__device__ __forceinline__ float scaled(int acc, float sa, float sb, float bias) {
+  return __fadd_rn(__fmul_rn(__int2float_rn(acc), __fmul_rn(sa, sb)), bias);
+}
+
+// -------------------------------------------------------------------- narrow
+template <int BN>
+struct Narrow {
+  static constexpr int kStages = BN <= 32 ? 5 : BN == 64 ? 4 : 3;
+  static constexpr int kA = 128 * 128, kB = BN * 128;
+  static constexpr int kCols = BN < 32 ? 32 : BN;  // TMEM columns, a power of two >= 32
+  // operand stages (the partials of a split reuse them), barriers, TMEM address
+  static constexpr size_t kSmem = 1024 + (size_t)kStages * (kA + kB) + 256;
+  static_assert((size_t)kStages * (kA + kB) >= (size_t)BN * 128 * 4, "partials fit");
+};
+
+// Grid: (weight tiles * split, token tiles), clusters of `split` CTAs along x.
+template <int BN>
+__global__ void __launch_bounds__(128)
+i8_narrow_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx,
+                 const Out o, const int split) {
+  using P = Narrow<BN>;
+  constexpr int S = P::kStages;
+  extern __shared__ unsigned char raw[];
+  unsigned char* sm = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + (size_t)S * (P::kA + P::kB));
+  uint64_t* empty = full + S;
+  uint64_t* done = empty + S;
+  uint32_t* tptr = reinterpret_cast<uint32_t*>(done + 1);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = blockIdx.x % split, n0 = blockIdx.x / split * 128, m0 = blockIdx.y * BN;
+  const int KT = (o.K + 127) >> 7;
+  const int kt0 = (int)((long long)KT * rank / split), kt1 = (int)((long long)KT * (rank + 1) / split);
+  const int nk = kt1 - kt0;
+  if (tid == 0) {
+    for (int s = 0; s < S; ++s) tc::mbar_init(full + s, 1), tc::mbar_init(empty + s, 1);
+    tc::mbar_init(done, 1);
+    tc::fence_mbar_init();
+    tc::prefetch_tmap(&tw);
+    tc::prefetch_tmap(&tx);
+  }
+  if (warp == 1) {
+    tc::tmem_alloc(tptr, P::kCols);
+    tc::tmem_relinquish();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = *tptr;
+
+  if (warp == 0 && lane == 0) {
+    // the weights of the first stages do not depend on the launch before (the
+    // quantisation of x): they load while it ends
+    const int pre = min(nk, S);
+    for (int i = 0; i < pre; ++i) {
+      tc::mbar_expect_tx(full + i, P::kA + P::kB);
+      tma_load_2d(sm + (size_t)i * (P::kA + P::kB), &tw, (kt0 + i) * 128, n0, full + i);
+    }
+    grid_dependency_wait();
+    for (int i = 0; i < nk; ++i) {
+      const int s = i % S;
+      unsigned char* st = sm + (size_t)s * (P::kA + P::kB);
+      if (i >= S) {
+        tc::mbar_wait(empty + s, (i / S - 1) & 1, 120);
+        tc::mbar_expect_tx(full + s, P::kA + P::kB);
+        tma_load_2d(st, &tw, (kt0 + i) * 128, n0, full + s);
+      }
+      tma_load_2d(st + P::kA, &tx, (kt0 + i) * 128, m0, full + s);
+    }
+  } else if (warp == 1 && lane == 0) {
+    constexpr uint32_t idesc = idesc_i8(128, BN);
+    for (int i = 0; i < nk; ++i) {
+      const int s = i % S;
+      tc::mbar_wait(full + s, (i / S) & 1, 121);
+      tc::tc_fence_after();
+      const uint32_t a0 = smem_u32(sm + (size_t)s * (P::kA + P::kB));
+      const uint64_t ad = tc::sdesc(a0, 0, 1024), bd = tc::sdesc(a0 + P::kA, 0, 1024);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) mma_i8(tmem, ad + 2 * k, bd + 2 * k, idesc, (i | k) != 0);
+      tc::mma_commit(empty + s);
+    }
+    tc::mma_commit(done);
+  }
+  __syncwarp();
+  grid_dependency_wait();
+  tc::mbar_wait(done, 0, 122);
+  tc::tc_fence_after();
+
+  // lane = weight row n0 + 32 warp + lane, column = token m0 + c
+  const int n = n0 + tid;
+  if (split == 1) {
+    const float sb = n < o.N ? o.sb[n] : 0.f, bias = n < o.N ? bias_at(o, n) : 0.f;
+    const int mt = min(BN, o.M - m0);
+#pragma unroll 1
+    for (int c0 = 0; c0 < mt; c0 += 16) {
+      float v[16];
+      tc::tmem_ld16(tmem + ((uint32_t)(warp * 32) << 16) + c0, v);
+      tc::tmem_wait_ld();
+      if (n < o.N) {
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          if (c0 + c >= mt) break;
+          const size_t at = (size_t)(m0 + c0 + c) * o.N + n;
+          const float y = scaled(__float_as_int(v[c]), o.sa[m0 + c0 + c], sb, bias);
+          if (o.y_bf16)
+            static_cast<bf16*>(o.y)[at] = __float2bfloat16_rn(y);
+          else
+            static_cast<float*>(o.y)[at] = y;
+        }
+      }
+    }
+  } else {
+    int* part = reinterpret_cast<int*>(sm);  // [BN][128]: every load has been consumed
+#pragma unroll 1
+    for (int c0 = 0; c0 < BN; c0 += 16) {
+      float v[16];
+      tc::tmem_ld16(tmem + ((uint32_t)(warp * 32) << 16) + c0, v);
+      tc::tmem_wait_ld();
+      // a share of K may be empty (fewer K tiles than CTAs): its accumulator was never written
+#pragma unroll
+      for (int c = 0; c < 16; ++c) part[(c0 + c) * 128 + tid] = nk ? __float_as_int(v[c]) : 0;
+    }
+    cluster_sync();
+    // the tile's token x channel elements in fours, dealt to the CTAs of the cluster
+    const int mt = min(BN, o.M - m0), quads = mt * 32;
+    const uint32_t base = smem_u32(part);
+    for (int e = rank * 128 + tid; e < quads; e += split * 128) {
+      const int c = e >> 5, q = (e & 31) * 4;
+      int4 sum = make_int4(0, 0, 0, 0);
+      for (int r = 0; r < split; ++r) {
+        const int4 p = ld_cluster_int4(map_to_rank(base + (c * 128 + q) * 4, r));
+        sum.x += p.x;
+        sum.y += p.y;
+        sum.z += p.z;
+        sum.w += p.w;
+      }
+      const float sa = o.sa[m0 + c];
+      const int v[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int nn = n0 + q + i;
+        if (nn >= o.N) break;
+        const float y = scaled(v[i], sa, o.sb[nn], bias_at(o, nn));
+        const size_t at = (size_t)(m0 + c) * o.N + nn;
+        if (o.y_bf16)
+          static_cast<bf16*>(o.y)[at] = __float2bfloat16_rn(y);
+        else
+          static_cast<float*>(o.y)[at] = y;
+      }
+    }
+    cluster_sync();  // peers read this CTA's partials until here
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tc::tmem_dealloc(tmem, P::kCols);
+}
+
+// ---------------------------------------------------------------------- wide
+constexpr int kWS = 6;                       // operand stages
+constexpr int kWHalf = 128 * 128;            // bytes of one operand's half of a stage
+constexpr int kWStage = 2 * kWHalf;          // a CTA's bytes of a stage
+constexpr int kWStaging = 4 * 32 * 128;      // 32 rows x 128 bytes of y for each epilogue warp
+constexpr size_t kWSmem = 1024 + (size_t)kWS * kWStage + kWStaging + 2 * 256 * 4 + 256;
+
+// Warps: 0 TMA, 1 MMA (and TMEM), 2..5 epilogue.
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
+i8_wide_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw,
+               const __grid_constant__ CUtensorMap ty, const Out o, const int ytma) {
+  extern __shared__ unsigned char raw[];
+  unsigned char* sm = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  unsigned char* staging = sm + (size_t)kWS * kWStage;
+  float* sSb = reinterpret_cast<float*>(staging + kWStaging);  // [256] channel scales
+  float* sBias = sSb + 256;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sBias + 256);  // in the leader: both CTAs' bytes
+  uint64_t* empty = full + kWS;
+  uint64_t* acc_full = empty + kWS;    // [2]
+  uint64_t* acc_empty = acc_full + 2;  // [2], in the leader: the eight epilogue warps
+  uint32_t* tptr = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t rank = cluster_rank();
+  if (tid == 0) {
+    for (int s = 0; s < kWS; ++s) tc::mbar_init(full + s, 1), tc::mbar_init(empty + s, 1);
+    for (int i = 0; i < 2; ++i) tc::mbar_init(acc_full + i, 1), tc::mbar_init(acc_empty + i, 8);
+    tc::fence_mbar_init();
+    tc::prefetch_tmap(&tx);
+    tc::prefetch_tmap(&tw);
+    tc::prefetch_tmap(&ty);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(
+                     smem_u32(tptr)),
+                 "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::);
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc::tc_fence_after();
+  const uint32_t tmem = *tptr;
+  const int KT = (o.K + 127) >> 7;
+  const int MT = (o.M + 255) >> 8, NTL = (o.N + 255) >> 8, tiles = MT * NTL;
+  const int cl = blockIdx.x >> 1, ncl = gridDim.x >> 1;
+  // tiles in groups of 8 channel tiles, tokens slower than the channels of a
+  // group: the group's weights stay in L2 while x streams past them once
+  const auto place = [&](int t, int& m, int& n) {
+    const int per = 8 * MT, gidx = t / per, in = t - gidx * per;
+    const int w = min(8, NTL - gidx * 8);
+    m = in / w;
+    n = gidx * 8 + in - m * w;
+  };
+
+  if (warp == 0 && lane == 0) {
+    grid_dependency_wait();
+    uint32_t it = 0;
+    for (int t = cl; t < tiles; t += ncl) {
+      int mt, nt;
+      place(t, mt, nt);
+      const int m = mt * 256 + rank * 128, n = nt * 256 + rank * 128;
+      for (int k = 0; k < KT; ++k, ++it) {
+        const int s = it % kWS;
+        if (it >= kWS) tc::mbar_wait(empty + s, (it / kWS - 1) & 1, 130);
+        const uint32_t bar = map_to_rank(smem_u32(full + s), 0);
+        if (rank == 0) tc::mbar_expect_tx(full + s, 2 * kWStage);
+        unsigned char* st = sm + (size_t)s * kWStage;
+        tma_load_2d_pair(st, &tx, k * 128, m, bar);
+        tma_load_2d_pair(st + kWHalf, &tw, k * 128, n, bar);
+      }
+    }
+    // every stage's last release has arrived before this CTA may leave
+    for (uint32_t i = it > kWS ? it - kWS : 0; i < it; ++i)
+      tc::mbar_wait(empty + i % kWS, (i / kWS) & 1, 134);
+  } else if (warp == 1 && lane == 0 && rank == 0) {
+    constexpr uint32_t idesc = idesc_i8(256, 256);
+    uint32_t it = 0, at = 0;
+    for (int t = cl; t < tiles; t += ncl, ++at) {
+      const int buf = at & 1;
+      if (at >= 2) tc::mbar_wait(acc_empty + buf, (at / 2 - 1) & 1, 131);
+      tc::tc_fence_after();
+      for (int k = 0; k < KT; ++k, ++it) {
+        const int s = it % kWS;
+        tc::mbar_wait(full + s, (it / kWS) & 1, 132);
+        tc::tc_fence_after();
+        const uint32_t a0 = smem_u32(sm + (size_t)s * kWStage);
+        const uint64_t ad = tc::sdesc(a0, 0, 1024), bd = tc::sdesc(a0 + kWHalf, 0, 1024);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          mma_i8_pair(tmem + buf * 256, ad + 2 * q, bd + 2 * q, idesc, (k | q) != 0);
+        commit_pair(empty + s);
+      }
+      commit_pair(acc_full + buf);
+    }
+  } else if (warp >= 2) {
+    const int quad = warp & 3, etid = tid - 64;
+    unsigned char* buf_y = staging + quad * 32 * 128;
+    const uint32_t peer_free[2] = {map_to_rank(smem_u32(acc_empty), 0),
+                                   map_to_rank(smem_u32(acc_empty + 1), 0)};
+    grid_dependency_wait();
+    uint32_t at = 0;
+    for (int t = cl; t < tiles; t += ncl, ++at) {
+      int mt, nt;
+      place(t, mt, nt);
+      const int buf = at & 1, n0 = nt * 256, row0 = mt * 256 + rank * 128 + quad * 32;
+      tc::named_bar_sync(1, 128);  // the scales of the tile before have been used
+      for (int i = etid; i < 256; i += 128) {
+        sSb[i] = n0 + i < o.N ? o.sb[n0 + i] : 0.f;
+        sBias[i] = n0 + i < o.N ? bias_at(o, n0 + i) : 0.f;
+      }
+      const int row = row0 + lane;
+      const float sa = row < o.M ? o.sa[row] : 0.f;
+      tc::named_bar_sync(1, 128);
+      tc::mbar_wait(acc_full + buf, (at / 2) & 1, 133);
+      tc::tc_fence_after();
+      const int per = o.y_bf16 ? 64 : 32;  // columns a 128-byte row of the staging holds
+#pragma unroll 1
+      for (int c0 = 0; c0 < 256; c0 += per) {
+        if (lane == 0) tc::bulk_wait_read0();  // the store before has left the staging
+        __syncwarp();
+        const uint32_t ta = tmem + buf * 256 + c0 + ((uint32_t)(quad * 32) << 16);
+#pragma unroll 1
+        for (int h = 0; h < per; h += 32) {
+          float v[32];
+          tc::tmem_ld32(ta + h, v);
+          tc::tmem_wait_ld();
+          if (c0 + h + 32 >= 256) {  // the accumulator has been read
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_remote(peer_free[buf]);
+          }
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            v[c] = scaled(__float_as_int(v[c]), sa, sSb[c0 + h + c], sBias[c0 + h + c]);
+          if (o.y_bf16) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const uint4 w = make_uint4(
+                  pack_bf16(v[8 * q], v[8 * q + 1]), pack_bf16(v[8 * q + 2], v[8 * q + 3]),
+                  pack_bf16(v[8 * q + 4], v[8 * q + 5]), pack_bf16(v[8 * q + 6], v[8 * q + 7]));
+              *reinterpret_cast<uint4*>(buf_y + lane * 128 + ((((h >> 3) + q) ^ (lane & 7)) << 4)) = w;
+            }
+          } else {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              *reinterpret_cast<float4*>(buf_y + lane * 128 + ((q ^ (lane & 7)) << 4)) =
+                  make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+          }
+        }
+        if (ytma) {
+          tc::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0 && row0 < o.M && n0 + c0 < o.N) {
+            tma_store_2d(&ty, buf_y, n0 + c0, row0);
+            tc::bulk_commit();
+          }
+        } else {
+          __syncwarp();
+          for (int r = 0; r < 32 && row0 + r < o.M; ++r)
+            for (int c = lane; c < per && n0 + c0 + c < o.N; c += 32) {
+              const size_t to = (size_t)(row0 + r) * o.N + n0 + c0 + c;
+              if (o.y_bf16)
+                static_cast<bf16*>(o.y)[to] = *reinterpret_cast<const bf16*>(
+                    buf_y + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
+              else
+                static_cast<float*>(o.y)[to] = *reinterpret_cast<const float*>(
+                    buf_y + r * 128 + (((c >> 2) ^ (r & 7)) << 4) + (c & 3) * 4);
+            }
+          __syncwarp();
+        }
+      }
+    }
+    if (lane == 0) tc::bulk_wait0();
+  }
+  __syncwarp();
+  tc::tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // no signal of the pair is still on its way
+  tc::tc_fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512));
+}
+
+// ---------------------------------------------------------------------- host
+int encode(CUtensorMap* m, const char* what, CUtensorMapDataType type, const void* p, int cols,
+           int rows, long long row_bytes, int box_cols, int box_rows) {
+  auto fn = tc::encode_tiled_fn();
+  if (!fn) {
+    set_error("int8: cuTensorMapEncodeTiled is not available");
+    return LZ_ERR_CUDA;
+  }
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)row_bytes};
+  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
+  const cuuint32_t es[2] = {1, 1};
+  const CUresult r = fn(m, type, 2, const_cast<void*>(p), dims, strides, box, es,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error(std::string("int8: the tensor map of ") + what + " could not be encoded, driver code " +
+              std::to_string((int)r));
+    return LZ_ERR_CUDA;
+  }
+  return LZ_OK;
+}
+
+template <typename K>
+int allow_smem(K kern, size_t bytes, bool* done) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 64 || done[dev]) return LZ_OK;
+  cudaError_t e =
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e != cudaSuccess) {
+    set_error(std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
+    return LZ_ERR_CUDA;
+  }
+  done[dev] = true;
+  return LZ_OK;
+}
+
+int launched(cudaError_t e, const char* what) {
+  if (e != cudaSuccess) {
+    set_error(std::string(what) + ": " + cudaGetErrorString(e));
+    return LZ_ERR_CUDA;
+  }
+  count_launches(1);
+  return check_launch(what);
+}
+
+struct Operand {
+  const int8_t* p;
+  long long ld;  // bytes, a multiple of 16
+  int rows;
+};
+
+template <int BN>
+int launch_narrow(const Operand& x, const Operand& w, const Out& o, bool after_quantize,
+                  cudaStream_t st) {
+  CUtensorMap tw, tx;
+  int rc = encode(&tw, "the weight", CU_TENSOR_MAP_DATA_TYPE_UINT8, w.p, o.K, o.N, w.ld, 128, 128);
+  if (!rc) rc = encode(&tx, "x", CU_TENSOR_MAP_DATA_TYPE_UINT8, x.p, o.K, o.M, x.ld, 128, BN);
+  if (rc) return rc;
+  static bool done[64] = {false};
+  rc = allow_smem(i8_narrow_kernel<BN>, Narrow<BN>::kSmem, done);
+  if (rc) return rc;
+  const int wt = ceil_div(o.N, 128), mt = ceil_div(o.M, BN), KT = ceil_div(o.K, 128);
+  int split = 1;
+  while (split < 8 && wt * mt * split < 148 && KT >= 4 * split) split *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(wt * split, mt);
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = Narrow<BN>::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = split;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = after_quantize ? 2 : 1;
+  return launched(cudaLaunchKernelEx(&cfg, i8_narrow_kernel<BN>, tw, tx, o, split),
+                  "i8_narrow_kernel");
+}
+
+int launch_wide(const Operand& x, const Operand& w, const Out& o, bool after_quantize,
+                cudaStream_t st) {
+  const int es = o.y_bf16 ? 2 : 4;
+  const int ytma = aligned16(o.y) && ((long long)o.N * es) % 16 == 0;
+  CUtensorMap tx, tw, ty;
+  int rc = encode(&tx, "x", CU_TENSOR_MAP_DATA_TYPE_UINT8, x.p, o.K, o.M, x.ld, 128, 128);
+  if (!rc) rc = encode(&tw, "the weight", CU_TENSOR_MAP_DATA_TYPE_UINT8, w.p, o.K, o.N, w.ld, 128, 128);
+  if (!rc && ytma)
+    rc = encode(&ty, "y", o.y_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
+                o.y, o.N, o.M, (long long)o.N * es, 128 / es, 32);
+  if (rc) return rc;
+  if (!ytma) ty = tx;
+  static bool done[64] = {false};
+  rc = allow_smem(i8_wide_kernel, kWSmem, done);
+  if (rc) return rc;
+  const long long tiles = (long long)ceil_div(o.M, 256) * ceil_div(o.N, 256);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * (unsigned)std::min<long long>(tiles, 74));
+  cfg.blockDim = dim3(192);
+  cfg.dynamicSmemBytes = kWSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = after_quantize ? 1 : 0;
+  return launched(cudaLaunchKernelEx(&cfg, i8_wide_kernel, tx, tw, ty, o, ytma), "i8_wide_kernel");
+}
+
+int quantize(const void* x, int x_dtype, long long ldx, int8_t* codes, long long ldc, float* scale,
+             int M, int K, cudaStream_t st) {
+  if (x_dtype == LZ_DTYPE_F32)
+    i8_quantize_kernel<float><<<M, kQT, 0, st>>>(static_cast<const float*>(x), ldx, codes, ldc,
+                                                 scale, K);
+  else
+    i8_quantize_kernel<bf16><<<M, kQT, 0, st>>>(static_cast<const bf16*>(x), ldx, codes, ldc,
+                                                scale, K);
+  count_launches(1);
+  return check_launch("i8_quantize_kernel");
+}
+
+int product(const Operand& x, const Operand& w, const Out& o, bool after_quantize,
+            cudaStream_t st) {
+  if (o.M <= 16) return launch_narrow<16>(x, w, o, after_quantize, st);
+  if (o.M <= 32) return launch_narrow<32>(x, w, o, after_quantize, st);
+  if (o.M <= 64) return launch_narrow<64>(x, w, o, after_quantize, st);
+  if (o.M <= 512) return launch_narrow<128>(x, w, o, after_quantize, st);
+  return launch_wide(x, w, o, after_quantize, st);
+}
+
+long long row16(int K) { return ((long long)K + 15) / 16 * 16; }
+
+// Rows of codes as the kernels take them: as they are, or repacked into *ws.
+int as_operand(Operand* op, const void* p, long long ld, int rows, int K, unsigned char** ws,
+               cudaStream_t st) {
+  op->rows = rows;
+  op->p = static_cast<const int8_t*>(p);
+  if (rows == 1) ld = row16(K);  // a single row's stride is never used
+  op->ld = ld;
+  if (aligned16(p) && ld % 16 == 0) return LZ_OK;
+  int8_t* to = reinterpret_cast<int8_t*>(*ws);
+  *ws += align_up((size_t)rows * row16(K), 256);
+  i8_repack_kernel<<<rows, kQT, 0, st>>>(op->p, ld, to, row16(K), K);
+  count_launches(1);
+  op->p = to;
+  op->ld = row16(K);
+  return check_launch("i8_repack_kernel");
+}
+
+int check_out(const void* bias, int bias_dtype, const void* y, int y_dtype, int M, int N, int K) {
+  LZ_REQUIRE(M >= 1 && N >= 1 && K >= 1, LZ_ERR_INVALID_ARGUMENT, "sizes must be positive");
+  LZ_REQUIRE(K <= kMaxK, LZ_ERR_UNSUPPORTED,
+             "K above 131071 can overflow the 32-bit integer sum");
+  LZ_REQUIRE(N <= (1 << 30) && (M + 15ll) / 16 <= (1ll << 30), LZ_ERR_UNSUPPORTED,
+             "sizes too large");
+  LZ_REQUIRE(y, LZ_ERR_INVALID_ARGUMENT, "null pointer");
+  LZ_REQUIRE(y_dtype == LZ_DTYPE_F32 || y_dtype == LZ_DTYPE_BF16, LZ_ERR_INVALID_ARGUMENT,
+             "y must be LZ_DTYPE_F32 or LZ_DTYPE_BF16");
+  LZ_REQUIRE(!bias || bias_dtype == LZ_DTYPE_F32 || bias_dtype == LZ_DTYPE_BF16,
+             LZ_ERR_INVALID_ARGUMENT, "bias must be LZ_DTYPE_F32 or LZ_DTYPE_BF16");
+  return LZ_OK;
+}
+
+}  // namespace
+int int8_timeout_flag(unsigned int* out) { return tc::read_timeout_flag_here(out); }
+int int8_timeout_clear() { return tc::clear_timeout_flag_here(); }
+}  // namespace lz
+
+extern "C" int lz_int8_quantize(const void* x, int x_dtype, long long x_ld, void* codes,
+                                long long codes_ld, float* scale, int M, int K, void* stream) {
+  using namespace lz;
+  clear_error();
+  LZ_REQUIRE(M >= 1 && K >= 1, LZ_ERR_INVALID_ARGUMENT, "sizes must be positive");
+  LZ_REQUIRE(x && codes && scale, LZ_ERR_INVALID_ARGUMENT, "null pointer");
+  LZ_REQUIRE(x_dtype == LZ_DTYPE_F32 || x_dtype == LZ_DTYPE_BF16, LZ_ERR_INVALID_ARGUMENT,
+             "x must be LZ_DTYPE_F32 or LZ_DTYPE_BF16");
+  LZ_REQUIRE(codes_ld >= K && codes_ld % 16 == 0 && aligned16(codes), LZ_ERR_INVALID_ARGUMENT,
+             "rows of codes must start on 16-byte boundaries");
+  return quantize(x, x_dtype, x_ld, static_cast<int8_t*>(codes), codes_ld, scale, M, K,
+                  static_cast<cudaStream_t>(stream));
+}
+
+extern "C" size_t lz_int8_workspace_bytes(int M, int N, int K) {
+  if (M < 1 || N < 1 || K < 1) return 0;
+  const size_t r = (size_t)lz::row16(K);
+  return lz::align_up((size_t)M * r, 256) + lz::align_up((size_t)M * 4, 256) +
+         lz::align_up((size_t)N * r, 256);
+}
+
+extern "C" size_t lz_int8_linear_workspace_bytes(int M, int K) {
+  if (M < 1 || K < 1) return 0;
+  return lz::align_up((size_t)M * (size_t)lz::row16(K), 256) + lz::align_up((size_t)M * 4, 256);
+}
+
+extern "C" int lz_int8_matmul(const void* a, long long a_ld, const float* a_scale, const void* b,
+                              long long b_ld, const float* b_scale, const void* bias,
+                              int bias_dtype, void* y, int y_dtype, void* workspace,
+                              size_t workspace_bytes, int M, int N, int K, void* stream) {
+  using namespace lz;
+  clear_error();
+  int rc = check_out(bias, bias_dtype, y, y_dtype, M, N, K);
+  if (rc) return rc;
+  LZ_REQUIRE(a && b && a_scale && b_scale, LZ_ERR_INVALID_ARGUMENT, "null pointer");
+  LZ_REQUIRE((M == 1 || a_ld >= K) && (N == 1 || b_ld >= K), LZ_ERR_INVALID_ARGUMENT,
+             "rows of codes overlap");
+  const bool fits = aligned16(a) && (M == 1 || a_ld % 16 == 0) && aligned16(b) &&
+                    (N == 1 || b_ld % 16 == 0);
+  LZ_REQUIRE(fits || (workspace && aligned16(workspace) &&
+                      workspace_bytes >= lz_int8_workspace_bytes(M, N, K)),
+             LZ_ERR_WORKSPACE, "workspace too small, see lz_int8_workspace_bytes");
+  auto st = static_cast<cudaStream_t>(stream);
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  Operand x, w;
+  rc = as_operand(&x, a, a_ld, M, K, &ws, st);
+  if (!rc) rc = as_operand(&w, b, b_ld, N, K, &ws, st);
+  if (rc) return rc;
+  const Out o = {a_scale, b_scale, bias, y, bias_dtype == LZ_DTYPE_BF16, y_dtype == LZ_DTYPE_BF16,
+                 M, N, K};
+  return product(x, w, o, false, st);
+}
+
+extern "C" int lz_int8_linear(const void* x, int x_dtype, long long x_ld, const void* w,
+                              long long w_ld, const float* w_scale, const void* bias,
+                              int bias_dtype, void* y, int y_dtype, void* workspace,
+                              size_t workspace_bytes, int M, int N, int K, void* stream) {
+  using namespace lz;
+  clear_error();
+  int rc = check_out(bias, bias_dtype, y, y_dtype, M, N, K);
+  if (rc) return rc;
+  LZ_REQUIRE(x && w && w_scale, LZ_ERR_INVALID_ARGUMENT, "null pointer");
+  LZ_REQUIRE(x_dtype == LZ_DTYPE_F32 || x_dtype == LZ_DTYPE_BF16, LZ_ERR_INVALID_ARGUMENT,
+             "x must be LZ_DTYPE_F32 or LZ_DTYPE_BF16");
+  LZ_REQUIRE(N == 1 || w_ld >= K, LZ_ERR_INVALID_ARGUMENT, "rows of codes overlap");
+  const bool fits = aligned16(w) && (N == 1 || w_ld % 16 == 0);
+  LZ_REQUIRE(workspace && aligned16(workspace) &&
+                 workspace_bytes >= (fits ? lz_int8_linear_workspace_bytes(M, K)
+                                          : lz_int8_workspace_bytes(M, N, K)),
+             LZ_ERR_WORKSPACE, "workspace too small, see lz_int8_linear_workspace_bytes");
+  auto st = static_cast<cudaStream_t>(stream);
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  int8_t* codes = reinterpret_cast<int8_t*>(ws);
+  ws += align_up((size_t)M * row16(K), 256);
+  float* sa = reinterpret_cast<float*>(ws);
+  ws += align_up((size_t)M * 4, 256);
+  Operand wo;
+  rc = as_operand(&wo, w, w_ld, N, K, &ws, st);
+  if (!rc) rc = quantize(x, x_dtype, x_ld, codes, row16(K), sa, M, K, st);
+  if (rc) return rc;
+  const Operand xo = {codes, row16(K), M};
+  const Out o = {sa, w_scale, bias, y, bias_dtype == LZ_DTYPE_BF16, y_dtype == LZ_DTYPE_BF16,
+                 M, N, K};
+  return product(xo, wo, o, true, st);
+}

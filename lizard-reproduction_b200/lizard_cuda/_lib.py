@@ -6,6 +6,7 @@ every call raises.
 """
 import contextlib
 import ctypes
+import functools
 import threading
 from pathlib import Path
 
@@ -20,6 +21,7 @@ LZ_DTYPE_BF16 = 1
 LZ_ERR_UNSUPPORTED = 2
 
 _c_int, _c_size, _vp = ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p
+_c_ll = ctypes.c_longlong
 _SIGNATURES = {
     "lz_abi_version": (_c_int, []),
     "lz_last_error_string": (ctypes.c_char_p, []),
@@ -81,6 +83,21 @@ _SIGNATURES = {
     "lz_swa_decode": (_c_int, [_vp, _vp, _vp, _c_int] + [ctypes.c_longlong] * 6 + [_vp, _vp, _c_int, ctypes.c_longlong,
                                                                      _vp, _vp, _vp, _vp, _c_int,
                                                                      _vp] + [_c_int] * 5 + [_vp]),
+    "lz_gla_decode_block": (_c_int, [_vp] * 4 + [_c_int] + [_vp] * 7 + [_c_int] * 8 + [_vp]),
+    "lz_swa_decode_block": (_c_int, [_vp] * 3 + [_c_int] + [_vp] * 3 + [_c_int, _c_ll]
+                            + [_vp] * 5 + [_c_ll] + [_vp] * 5 + [_c_int, _vp] + [_c_int] * 7
+                            + [_vp]),
+    "lz_verify_drafts_workspace_bytes": (_c_size, [_c_int] * 3),
+    "lz_verify_drafts": (_c_int, [_vp, _c_ll, _c_ll, _vp, _c_ll, _c_ll, _c_int, _vp, _c_int, _vp,
+                                  _vp, _c_ll, _vp, ctypes.c_float, _vp, _vp, _vp, _vp, _c_size]
+                         + [_c_int] * 3 + [_vp]),
+    "lz_int8_quantize": (_c_int, [_vp, _c_int, _c_ll, _vp, _c_ll, _vp, _c_int, _c_int, _vp]),
+    "lz_int8_workspace_bytes": (_c_size, [_c_int] * 3),
+    "lz_int8_linear_workspace_bytes": (_c_size, [_c_int] * 2),
+    "lz_int8_matmul": (_c_int, [_vp, _c_ll, _vp, _vp, _c_ll, _vp, _vp, _c_int, _vp, _c_int, _vp,
+                                _c_size] + [_c_int] * 3 + [_vp]),
+    "lz_int8_linear": (_c_int, [_vp, _c_int, _c_ll, _vp, _c_ll, _vp, _vp, _c_int, _vp, _c_int,
+                                _vp, _c_size] + [_c_int] * 3 + [_vp]),
     "lz_swa_rope_fwd": (_c_int, [_vp, _vp, _vp, _c_int] + [ctypes.c_longlong] * 9 + [_vp, _vp, _c_int, ctypes.c_longlong,
                                                                      ctypes.c_longlong, _vp, _c_int, _c_int,
                                                                      _vp, _vp, _c_size, _vp, _vp,
@@ -179,6 +196,12 @@ def set_schedule(name):
 def ptr(t):
     """Device address of a tensor as a plain int (ctypes passes it as void*)."""
     return None if t is None else t.data_ptr()
+
+
+@functools.lru_cache(None)
+def longlongs(n):
+    """The ctypes array type of n 64-bit integers (host arguments of strides)."""
+    return ctypes.c_longlong * n
 
 
 def stream_of(t):
