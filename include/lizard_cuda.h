@@ -507,7 +507,7 @@ int lz_swa_decode(const void* q, const void* k, const void* v, int x_dtype,
  * accepted prefix: first the state advances in place by the first count[b]
  * tokens (clamped to 0..T_prev; null = all) of the previous block, fk_prev
  * [B*Hkv, T_prev, F], v_prev [B*Hkv, T_prev, D], log_gamma_prev, then y
- * [B*H, T, D] (bf16, 8-byte aligned) is what T single steps from there would
+ * [B*H, T, D] (bf16, 4-byte aligned) is what T single steps from there would
  * give for fq [B*H, T, F], fk, v, log_gamma ([B, T], or [B*H, T] with
  * gate_per_head); the block itself is not folded in. T = 0 only advances the
  * state (fq, fk, v, log_gamma, y may be null), T_prev = 0 only reads it.

@@ -15,19 +15,28 @@
 // gate of zero (lg = -inf) gives 0 and not inf - inf.
 //
 // Bound: the state is read once and written once, 8 F D bytes a head, against
-// 2 rep T F D multiply-adds: memory. One CTA holds F x 64 (or 32) of a state in
-// registers, laid out as the B fragments of mma.sync m16n8k16: thread (g, j) of
-// a warp holds rows 2j, 2j+1, 2j+8, 2j+9 of each 16-row step and columns
-// 4g..4g+3 of a 32-column group, so a load is one float4 and a warp's load
-// covers four whole 128-byte lines, and tile i of the group stands for columns
-// 4n + i. The update runs in fp32 in those registers (k and v are bf16, their
-// products exact); for q S the registers are split once into bf16 hi + lo parts
-// (relative error 2^-17, against the 2^-9 of the bf16 output). The four warps
-// of a column half each contract a quarter of F and are added through shared
-// memory in a fixed order.
+// 2 rep T F D multiply-adds: memory. A CTA takes 64 (or 32) columns of a state: TMA
+// brings them into shared memory in 128-byte swizzled rows while the keys, gates
+// and queries are staged, and each warp takes 16 columns by half of the F rows into
+// registers, as the B fragments of mma.sync m16n8k16: thread (g, j) holds columns g
+// and 8 + g of rows 2j, 2j+1, 2j+8, 2j+9 of each 16-row step (the swizzle keeps
+// these reads free of bank conflicts). It updates them in fp32 (packed pairs of
+// rows; k and v are bf16, their products exact), writes them back, splits them once
+// into bf16 hi + lo parts (relative error 2^-17, against the 2^-8 of the bf16
+// output) and contracts the queries with them 32 rows at a time; the two halves of
+// F meet at the end, a row tile each. (8 columns by all of F needs no such meeting
+// but reads every key and query value twice as often from shared memory, which then
+// bounds the kernel.)
+// The scores of the block's keys are shared: a quarter of F a warp, added through
+// shared memory. z rides along as two more keys (hi and lo): with M = [exp of the decay from key to token,
+// 0 above the diagonal | d_t for the two z columns], a' = (q K^T) o M has the row
+// sum as its own sum over all columns, and y = (d_t q S + a' V) / sum a' with zero
+// rows of V for z.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
+#include "tc.cuh"
 
 namespace lz {
 namespace {
@@ -42,7 +51,8 @@ struct GlaBlockArgs {
   const int* count;
   float *S, *Z;
   bf16* y;
-  int gph, T, Tp, H, Hkv, Hs, F, D, nsl;
+  // rep query heads a state, kvrep state heads a key/value head
+  int gph, T, Tp, H, Hkv, Hs, F, D, nsl, rep, kvrep;
 };
 
 __device__ __forceinline__ void cluster_arrive() {
@@ -52,307 +62,484 @@ __device__ __forceinline__ void cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
 
-// rows x ncols bf16 (row stride ncols) into shared rows of ld elements, columns
-// ncols..width zeroed; 16-byte loads when rows keep that alignment.
-__device__ __forceinline__ void stage_rows(bf16* s, int ld, int width, const bf16* g, int rows,
-                                           int ncols, int pad_rows, int nthreads) {
-  const bool vec = (ncols & 7) == 0 && (reinterpret_cast<uintptr_t>(g) & 15) == 0;
+// rows x ncols bf16 (row stride ldg) into shared rows of ld elements, zeros to
+// pad_rows x width; 16-byte copies when rows keep that alignment.
+__device__ __forceinline__ void stage_rows(bf16* s, int ld, int width, int ldg, const bf16* g,
+                                           int rows, int ncols, int pad_rows, int nthreads) {
+  const bool vec = ((ldg | ncols) & 7) == 0 && (reinterpret_cast<uintptr_t>(g) & 15) == 0;
   if (vec) {
     const int cpr = width >> 3;
     for (int i = threadIdx.x; i < pad_rows * cpr; i += nthreads) {
       const int r = i / cpr, c = (i - r * cpr) * 8;
-      cp_async16(s + r * ld + c, r < rows && c < ncols ? g + (size_t)r * ncols + c : g,
-                 r < rows && c < ncols);
+      const bool in = r < rows && c < ncols;
+      cp_async16(s + r * ld + c, in ? g + r * ldg + c : g, in);
     }
   } else {
     for (int i = threadIdx.x; i < pad_rows * width; i += nthreads) {
       const int r = i / width, c = i - r * width;
-      s[r * ld + c] = r < rows && c < ncols ? g[(size_t)r * ncols + c] : __float2bfloat16_rn(0.f);
+      s[r * ld + c] = r < rows && c < ncols ? g[r * ldg + c] : __float2bfloat16_rn(0.f);
     }
   }
 }
 
-// KS: 16-row steps of F a warp owns (F <= 64 KS). HALVES: 32-column groups a CTA.
-template <int KS, int HALVES>
-__global__ void __launch_bounds__(128 * HALVES)
-gla_block_kernel(const GlaBlockArgs a) {
-  constexpr int NT = 128 * HALVES, FP = 64 * KS, LD = FP + 8, DN = 32 * HALVES;
-  extern __shared__ __align__(16) unsigned char smraw[];
-  const int T = a.T, Tp = a.Tp, F = a.F, D = a.D;
-  const int TK = (T + 7) & ~7;  // block keys, padded to mma columns
-  const int LDR = DN + TK + 4;  // row of a partial: DN values, TK scores
-  bf16* sQ = reinterpret_cast<bf16*>(smraw);      // [16][LD]
-  bf16* sK = sQ + 16 * LD;                        // [TK][LD] block keys
-  bf16* sKp = sK + TK * LD;                       // [Tp][LD] pending keys
-  float* sV = reinterpret_cast<float*>(sKp + ((Tp + 1) & ~1) * LD);  // [T][DN]
-  float* sVp = sV + T * DN;                       // [Tp][DN], then the partials
-  float* sRed = sVp + Tp * DN;                    // [4][16][LDR]
-  float* sA = sRed + 4 * 16 * LDR;                // [16][TK + 1]
-  float* sM = sA + 16 * (TK + 1);                 // [T][T] decay of key s at token t
-  float* sDec = sM + T * T;                       // [T]
-  float* sW = sDec + T;                           // [Tp]
-  float* sZ = sW + Tp;                            // [FP]
-  float* sQz = sZ + FP;                           // [16]
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int wf = warp & 3, wd = warp >> 2, g = lane >> 2, j = lane & 3;
-  const int sidx = blockIdx.x / a.nsl, sl = blockIdx.x - sidx * a.nsl;
-  const int b = sidx / a.Hs, s = sidx - b * a.Hs;
-  const int rep = a.H / a.Hs, R = rep * T;
-  const int kvh = a.Hs == a.Hkv ? sidx : kv_head(b * a.H + s, a.H, a.H / a.Hkv);
-  const int d0 = sl * DN, dcol = d0 + wd * 32 + 4 * g;
-  const bool dok = dcol < D;
-  const int n = Tp ? (a.count ? min(max(a.count[b], 0), Tp) : Tp) : 0;
-
-  // the state first: every load is in flight before anything waits
-  float4 st[KS][4];
-  float* Sb = a.S + (size_t)sidx * F * D + dcol;
+// Two fp32 values in a 64-bit register, and two operations an instruction.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float x, float y) {
+  f32x2 d;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(d) : "f"(x), "f"(y));
+  return d;
+}
+__device__ __forceinline__ void unpack2(f32x2 v, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// Gates of tokens lane and lane + 32 (x0, x1) become the sums over the tokens after
+// them; returns the sum of all n. Every sum is a running one: a closed gate (-inf)
+// stays -inf for the tokens before it and touches no other.
+__device__ __forceinline__ float after(float& x0, float& x1, int n) {
+  const int lane = threadIdx.x & 31;
+  const auto scan = [&](float& x) {  // inclusive from the right; returns the total
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int f = (wf * KS + ks) * 16 + 2 * j + (u & 1) + (u >> 1) * 8;
-      st[ks][u] = dok && f < F ? *reinterpret_cast<const float4*>(Sb + (size_t)f * D)
-                               : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int o = 1; o < 32; o <<= 1) {
+      const float y = __shfl_down_sync(0xffffffffu, x, o);
+      if (lane + o < 32) x += y;
     }
-  // block and pending keys, values and gates
-  if (T) stage_rows(sK, LD, FP, a.fk + (size_t)kvh * T * F, T, F, TK, NT);
-  if (n) stage_rows(sKp, LD, FP, a.fk_p + (size_t)kvh * Tp * F, n, F, n, NT);
-  const bf16* fq = a.fq + (size_t)(b * a.H + s * rep) * T * F;
-  if (T) stage_rows(sQ, LD, FP, fq, min(R, 16), F, 16, NT);
-  cp_async_commit();
-  for (int i = tid; i < T * DN; i += NT) {
-    const int t = i / DN, d = d0 + i - t * DN;
-    sV[i] = d < D ? __bfloat162float(a.v[((size_t)kvh * T + t) * D + d]) : 0.f;
+    const float all = __shfl_sync(0xffffffffu, x, 0);
+    const float y = __shfl_down_sync(0xffffffffu, x, 1);
+    x = lane < 31 ? y : 0.f;
+    return all;
+  };
+  float high = 0.f;
+  if (n > 32) high = scan(x1);
+  const float all = scan(x0);
+  x0 += high;
+  return all + high;
+}
+
+constexpr int kQRows = 32;  // query rows staged at a time
+constexpr int kPend = 8;    // pending tokens folded in at a time
+
+// Shared memory, in bytes from the 1024-aligned start.
+struct BlockSmem {
+  int q, k, v, kw, vw, a, den, m, bar, total;
+};
+__host__ __device__ inline BlockSmem block_smem(int KS, int HALVES, int T) {
+  const int LD = 64 * KS + 8, DN = 32 * HALVES, TK = (T + 2 + 15) & ~15;
+  BlockSmem s;
+  int n = HALVES * 64 * KS * 128;  // the state's columns
+  // queries, then the halves of F on their way to each other (1 KB a warp)
+  s.q = n, n += kQRows * LD * 2 > HALVES * 4096 ? kQRows * LD * 2 : HALVES * 4096;
+  s.k = n, n += TK * LD * 2;
+  s.v = n, n += TK * (DN + 8) * 2;
+  // pending keys, then (they are done) the partial scores of the quarters of F
+  const int kw = kPend * 64 * KS * 4, parts = 4 * kQRows * 16 * 4;
+  s.kw = n, n += kw > parts ? kw : parts;
+  s.vw = n, n += kPend * DN * 4;
+  s.a = n, n += 2 * kQRows * 48;  // a' hi and lo, rows of 16 and 8 to spare
+  s.den = n, n += kQRows * 8;
+  s.m = n, n += (T > 0 ? T : 1) * TK * 4;
+  s.bar = (n + 7) & ~7, n = s.bar + 8;
+  s.total = n + 1024;
+  return s;
+}
+
+// KS: F <= 64 KS. HALVES: 32-column groups of a CTA, four warps each.
+template <int KS, int HALVES>
+__global__ void __launch_bounds__(128 * HALVES, 2)
+gla_block_kernel(const __grid_constant__ CUtensorMap ts, const GlaBlockArgs a) {
+  constexpr int NT = 128 * HALVES, FP = 64 * KS, LD = FP + 8, DN = 32 * HALVES, LV = DN + 8;
+  constexpr int NH = 2 * KS;  // 16-row steps of half of F
+  extern __shared__ unsigned char raw[];
+  unsigned char* sm = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  const int T = a.T, Tp = a.Tp, F = a.F, D = a.D;
+  const BlockSmem o = block_smem(KS, HALVES, T);
+  const int TK = (T + 2 + 15) & ~15;
+  bf16* sQ = reinterpret_cast<bf16*>(sm + o.q);       // [32][LD]
+  bf16* sK = reinterpret_cast<bf16*>(sm + o.k);       // [TK][LD]: keys, z hi, z lo, zeros
+  bf16* sV = reinterpret_cast<bf16*>(sm + o.v);       // [TK][LV], zero rows from T on
+  float* sKw = reinterpret_cast<float*>(sm + o.kw);   // [8][FP] pending keys
+  float* sVw = reinterpret_cast<float*>(sm + o.vw);   // [8][DN] pending values times their decay
+  float* sP = sKw;                                    // [4][32][16]
+  uint32_t* sAh = reinterpret_cast<uint32_t*>(sm + o.a);  // [32] rows of 48 bytes
+  uint32_t* sAl = sAh + kQRows * 12;
+  float2* sDen = reinterpret_cast<float2*>(sm + o.den);
+  float* sM = reinterpret_cast<float*>(sm + o.m);     // [T][TK]
+  uint64_t* bar = reinterpret_cast<uint64_t*>(sm + o.bar);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, j = lane & 3;
+  const int b = blockIdx.x, s = blockIdx.y, sl = blockIdx.z, sidx = b * a.Hs + s;
+  const int rep = a.rep, R = rep * T;
+  const int kvh = a.kvrep == 1 ? sidx : b * a.Hkv + s / a.kvrep;
+  const int d0 = sl * DN;
+  constexpr int tile = FP * 128;  // bytes of 32 columns
+
+  if (tid == 0) {
+    tc::mbar_init(bar, 1);
+    tc::fence_mbar_init();
+    tc::mbar_expect_tx(bar, HALVES * tile);  // rows F .. FP and columns beyond D arrive as zeros
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h) tc::tma_load_3d(sm + h * tile, &ts, d0 + 32 * h, 0, sidx, bar);
   }
-  for (int i = tid; i < n * DN; i += NT) {
-    const int t = i / DN, d = d0 + i - t * DN;
-    sVp[i] = d < D ? __bfloat162float(a.v_p[((size_t)kvh * Tp + t) * D + d]) : 0.f;
+  const bf16* fq = a.fq + (size_t)(b * a.H + s * rep) * T * F;
+  if (T) {
+    stage_rows(sK, LD, FP, F, a.fk + (size_t)kvh * T * F, T, F, TK, NT);
+    stage_rows(sQ, LD, FP, F, fq, min(R, kQRows), F, kQRows, NT);
+    stage_rows(sV, LV, DN, D, a.v + (size_t)kvh * T * D + d0, T, D - d0, TK, NT);
+    cp_async_commit();
   }
   const size_t grow = a.gph ? (size_t)b * a.H + s : (size_t)b;
-  if (tid < T) {  // column tid of the block's decays: running sums from its own key on
-    const float* lg = a.lg + grow * T;
-    float acc = 0.f;
-    for (int t = 0; t < tid; ++t) sM[t * T + tid] = 0.f;
-    sM[tid * T + tid] = 1.f;
-    for (int t = tid + 1; t < T; ++t) {
-      acc += lg[t];
-      sM[t * T + tid] = expf(acc);
+  // lane r of every warp holds the gates of tokens r and r + 32
+  const float lg0 = lane < T ? a.lg[grow * T + lane] : 0.f;
+  const float lg1 = lane + 32 < T ? a.lg[grow * T + lane + 32] : 0.f;
+  float lgp0 = lane < Tp ? a.lg_p[grow * Tp + lane] : 0.f;
+  float lgp1 = lane + 32 < Tp ? a.lg_p[grow * Tp + lane + 32] : 0.f;
+  const int n = Tp ? (a.count ? min(max(a.count[b], 0), Tp) : Tp) : 0;
+  float* Zs = a.Z + (size_t)sidx * F;
+  constexpr int ZN = (FP + NT - 1) / NT;  // elements of z a thread owns
+  float z[ZN];
+#pragma unroll
+  for (int i = 0; i < ZN; ++i) z[i] = tid + i * NT < F ? Zs[tid + i * NT] : 0.f;
+  // the first pending keys and values, before it is known how many stand
+  const bf16* kp = a.fk_p + (size_t)kvh * Tp * F;
+  const bf16* vp = a.v_p + (size_t)kvh * Tp * D + d0;
+  bf16 kk[ZN][kPend], vv[kPend * DN / NT];
+  const auto fetch = [&](int t0) {
+#pragma unroll
+    for (int i = 0; i < ZN; ++i)
+#pragma unroll
+      for (int t = 0; t < kPend; ++t) {
+        const int f = tid + i * NT;
+        kk[i][t] = t0 + t < Tp && f < F ? kp[(t0 + t) * F + f] : __float2bfloat16_rn(0.f);
+      }
+#pragma unroll
+    for (int i = 0; i < kPend * DN / NT; ++i) {
+      const int t = t0 + (tid + i * NT) / DN, d = (tid + i * NT) % DN;
+      vv[i] = t < Tp && d0 + d < D ? vp[t * D + d] : __float2bfloat16_rn(0.f);
+    }
+  };
+  fetch(0);
+  // decays: M of the block (a warp a token), w of the pending tokens (every warp)
+  for (int t = warp; t < T; t += NT / 32) {
+    float e0 = lane <= t ? lg0 : 0.f, e1 = lane + 32 <= t ? lg1 : 0.f;
+    const float all = expf(after(e0, e1, T));
+    e0 = expf(e0), e1 = expf(e1);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const int k = lane + 32 * i;
+      if (k < TK)
+        sM[t * TK + k] = k <= t ? (i ? e1 : e0) : (k == T || k == T + 1 ? all : 0.f);
     }
   }
-  const int tp = NT - 1 - tid;  // from the other end: other warps
-  if (tp < T) {
-    float acc = 0.f;
-    for (int t = 0; t <= tp; ++t) acc += a.lg[grow * T + t];
-    sDec[tp] = expf(acc);
-  }
-  float gn = 1.f;
-  if (n) {
-    const float* lg = a.lg_p + grow * Tp;
-    float acc = 0.f;
-    for (int t = 0; t < n; ++t) acc += lg[t];
-    gn = expf(acc);
-    if (tid < n) {
-      acc = 0.f;
-      for (int t = tid + 1; t < n; ++t) acc += lg[t];
-      sW[tid] = expf(acc);
+  lgp0 = lane < n ? lgp0 : 0.f;
+  lgp1 = lane + 32 < n ? lgp1 : 0.f;
+  const float gn = expf(after(lgp0, lgp1, n));
+  const float w0 = expf(lgp0), w1 = expf(lgp1);
+  const auto w_of = [&](int t) { return __shfl_sync(0xffffffffu, t < 32 ? w0 : w1, t & 31); };
+  if (n && a.nsl > 1) cluster_arrive();  // every slice reads z before slice 0 writes it
+#pragma unroll
+  for (int i = 0; i < ZN; ++i) z[i] *= gn;
+  // kPend pending tokens to shared memory: keys as they are, values times their decay
+  const auto stage = [&](int t0) {
+#pragma unroll
+    for (int i = 0; i < ZN; ++i) {
+      const int f = tid + i * NT;
+      // within a step the four rows of a thread are neighbours: one 16-byte read
+      const int at = (f & ~15) | (f & 6) << 1 | (f >> 2 & 2) | (f & 1);
+#pragma unroll
+      for (int t = 0; t < kPend; ++t)
+        if (t0 + t < n) {
+          const float x = __bfloat162float(kk[i][t]), w = w_of(t0 + t);
+          if (f < FP) sKw[t * FP + at] = x;
+          z[i] += w * x;
+        }
     }
-  }
-  cp_async_wait_all();
+#pragma unroll
+    for (int i = 0; i < kPend * DN / NT; ++i) {
+      const int t = t0 + (tid + i * NT) / DN;  // the same for a warp
+      if (t < n) sVw[tid + i * NT] = w_of(t) * __bfloat162float(vv[i]);
+    }
+  };
+  if (n) stage(0);
   __syncthreads();
 
-  // the normaliser (every slice's CTA needs it; slice 0 writes it once all have read it)
-  float* Zs = a.Z + (size_t)sidx * F;
-  for (int f = tid; f < FP; f += NT) {
-    float z = f < F ? Zs[f] : 0.f;
-    if (n) {
-      z *= gn;
-      for (int t = 0; t < n; ++t) z += sW[t] * __bfloat162float(sKp[t * LD + f]);
-    }
-    sZ[f] = z;
+  // the state into registers: rows (2j, 2j+1) and (2j+8, 2j+9) of step ks, columns
+  // g and 8 + g of this warp's 16
+  f32x2 st[NH][2][2];  // [step][rows][column]
+  const int cg = warp % (2 * HALVES), fh = warp / (2 * HALVES), half = cg >> 1;
+  const int c = (cg & 1) * 16 + g;  // within the 32 of its tile
+  const bool live = tc::mbar_wait(bar, 0, 95);  // after a timeout nothing is written
+  // (f & 7 is 2j or 2j + 1 whatever the step: two swizzled addresses and constants)
+  float *even[2], *odd[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int cc = c + 8 * i, r = fh * NH * 16 + 2 * j;
+    even[i] = reinterpret_cast<float*>(sm + half * tile + r * 128) +
+              ((((cc >> 2) ^ (2 * j)) << 2) | (cc & 3));
+    odd[i] = reinterpret_cast<float*>(sm + half * tile + (r + 1) * 128) +
+             ((((cc >> 2) ^ (2 * j + 1)) << 2) | (cc & 3));
   }
-  if (n && a.nsl > 1) cluster_arrive();
-
-  // the state: S <- g S + sum w_t k_t^T v_t, in fp32
+#pragma unroll
+  for (int ks = 0; ks < NH; ++ks)
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        st[ks][p][i] = pack2(even[i][(ks * 16 + 8 * p) * 32], odd[i][(ks * 16 + 8 * p) * 32]);
   if (n) {
+    const f32x2 gg = pack2(gn, gn);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
+    for (int ks = 0; ks < NH; ++ks)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        st[ks][u].x *= gn;
-        st[ks][u].y *= gn;
-        st[ks][u].z *= gn;
-        st[ks][u].w *= gn;
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) st[ks][p][i] = mul2(st[ks][p][i], gg);
+    for (int t0 = 0; t0 < n; t0 += kPend) {
+      const int nt = min(kPend, n - t0);
+      if (t0) {
+        fetch(t0);
+        __syncthreads();  // the tokens before have been folded in
+        stage(t0);
+        __syncthreads();
       }
-    for (int t = 0; t < n; ++t) {
-      const float w = sW[t];
-      const float4 vv = *reinterpret_cast<const float4*>(sVp + t * DN + wd * 32 + 4 * g);
+      for (int t = 0; t < nt; ++t) {
+        const float v0 = sVw[t * DN + half * 32 + c], v1 = sVw[t * DN + half * 32 + c + 8];
+        const f32x2 va = pack2(v0, v0), vb = pack2(v1, v1);
+        const ulonglong2* kr =
+            reinterpret_cast<const ulonglong2*>(sKw + t * FP + fh * NH * 16 + 4 * j);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const bf16* kr = sKp + t * LD + (wf * KS + ks) * 16 + 2 * j;
-        const uint32_t k01 = *reinterpret_cast<const uint32_t*>(kr);
-        const uint32_t k89 = *reinterpret_cast<const uint32_t*>(kr + 8);
-        const float kf[4] = {w * bf16_lo(k01), w * bf16_hi(k01), w * bf16_lo(k89),
-                             w * bf16_hi(k89)};
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          st[ks][u].x += kf[u] * vv.x;
-          st[ks][u].y += kf[u] * vv.y;
-          st[ks][u].z += kf[u] * vv.z;
-          st[ks][u].w += kf[u] * vv.w;
+        for (int ks = 0; ks < NH; ++ks) {
+          const ulonglong2 k4 = kr[ks * 4];
+          st[ks][0][0] = fma2(k4.x, va, st[ks][0][0]);
+          st[ks][0][1] = fma2(k4.x, vb, st[ks][0][1]);
+          st[ks][1][0] = fma2(k4.y, va, st[ks][1][0]);
+          st[ks][1][1] = fma2(k4.y, vb, st[ks][1][1]);
         }
       }
     }
+    // back through shared memory (each thread over its own elements) and TMA, which
+    // leaves out what lies beyond F and D
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
+    for (int ks = 0; ks < NH; ++ks)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int f = (wf * KS + ks) * 16 + 2 * j + (u & 1) + (u >> 1) * 8;
-        if (dok && f < F) *reinterpret_cast<float4*>(Sb + (size_t)f * D) = st[ks][u];
-      }
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          unpack2(st[ks][p][i], even[i][(ks * 16 + 8 * p) * 32], odd[i][(ks * 16 + 8 * p) * 32]);
+    tc::fence_proxy_async_smem();
+    __syncthreads();
+    if (tid == 0 && live) {
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h)
+        if (d0 + 32 * h < D) tc::tma_store_3d(&ts, sm + h * tile, d0 + 32 * h, 0, sidx);
+      tc::bulk_commit();
+    }
+    if (a.nsl > 1) cluster_wait();
+    if (sl == 0 && live)
+#pragma unroll
+      for (int i = 0; i < ZN; ++i)
+        if (tid + i * NT < F) Zs[tid + i * NT] = z[i];
   }
-  if (n && a.nsl > 1) cluster_wait();
-  __syncthreads();
-  if (n && sl == 0)
-    for (int f = tid; f < F; f += NT) Zs[f] = sZ[f];
-  if (!T) return;
+  if (!T) {
+    if (tid == 0) tc::bulk_wait_read0();
+    return;
+  }
 
+  // z as two more keys
+  cp_async_wait_all();
+  __syncthreads();  // keys and queries are there (their zero rows too)
+#pragma unroll
+  for (int i = 0; i < ZN; ++i) {
+    const int f = tid + i * NT;
+    if (f < FP) {
+      const bf16 h = __float2bfloat16_rn(z[i]);
+      sK[T * LD + f] = h;
+      sK[(T + 1) * LD + f] = __float2bfloat16_rn(z[i] - __bfloat162float(h));
+    }
+  }
   // B fragments of q S: bf16 hi and lo parts of the registers
-  uint32_t hi[KS][4][2], lo[KS][4][2];
+  uint32_t hi[NH][2][2], lo[NH][2][2];  // [step][column][rows]
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks)
+  for (int ks = 0; ks < NH; ++ks)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int p = 0; p < 2; ++p)
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const float x0 = reinterpret_cast<const float*>(&st[ks][2 * p])[i];
-        const float x1 = reinterpret_cast<const float*>(&st[ks][2 * p + 1])[i];
+      for (int i = 0; i < 2; ++i) {
+        float x0, x1;
+        unpack2(st[ks][p][i], x0, x1);
         const uint32_t h = pack_bf16(x0, x1);
         hi[ks][i][p] = h;
         lo[ks][i][p] = pack_bf16(x0 - bf16_lo(h), x1 - bf16_hi(h));
       }
+  __syncthreads();
 
-  for (int r0 = 0; r0 < R; r0 += 16) {
+  // ldmatrix rows of this lane: queries (A), keys (B), a' (A)
+  const uint32_t aq = smem_u32(sQ) + (lane & 15) * (LD * 2) + (lane >> 4) * 16;
+  const uint32_t ak = smem_u32(sK) + ((lane & 7) + (lane >> 4) * 8) * (LD * 2) + (lane >> 3 & 1) * 16;
+  const uint32_t aa = smem_u32(sAh) + (lane & 15) * 48 + (lane >> 4) * 16;
+  const int vcol = cg * 16;  // this warp's columns of V and y
+  const uint32_t av = smem_u32(sV) + (lane & 15) * (LV * 2) + vcol * 2 + (lane >> 4) * 16;
+  const int quarter = warp & 3;  // of F, for the scores
+  for (int r0 = 0; r0 < R; r0 += kQRows) {
     if (r0) {
-      stage_rows(sQ, LD, FP, fq + (size_t)r0 * F, min(R - r0, 16), F, 16, NT);
+      __syncthreads();
+      stage_rows(sQ, LD, FP, F, fq + (size_t)r0 * F, min(R - r0, kQRows), F, kQRows, NT);
       cp_async_commit();
       cp_async_wait_all();
       __syncthreads();
     }
-    float acc[4][4];
+    // [row tile][column tile] of q S over this half of F, and a' V of row tile fh
+    float x[2][2][4], out[2][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) acc[i][c] = 0.f;
-    uint32_t qa[KS][4];
+      for (int e = 0; e < 4; ++e) x[0][i][e] = x[1][i][e] = out[i][e] = 0.f;
+    float den[kQRows * 8 / NT];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      lda_rm(qa[ks], sQ, LD, 0, (wf * KS + ks) * 16);
+    for (int i = 0; i < kQRows * 8 / NT; ++i) den[i] = 0.f;
+    for (int k0 = 0; k0 < TK; k0 += 16) {
+      // scores of 16 keys: each warp a quarter of F, for one row tile (or, with four warps, both)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        mma16816(acc[i], qa[ks], hi[ks][i][0], hi[ks][i][1]);
-        mma16816(acc[i], qa[ks], lo[ks][i][0], lo[ks][i][1]);
+      for (int rt = warp >> 2; rt < 2; rt += HALVES) {
+        float sc[2][4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[i][e] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          uint32_t qa[4], kb[4];
+          ldsm_x4(qa, aq + rt * (16 * LD * 2) + (quarter * KS + ks) * 32);
+          ldsm_x4(kb, ak + k0 * (LD * 2) + (quarter * KS + ks) * 32);
+          mma16816(sc[0], qa, kb[0], kb[1]);
+          mma16816(sc[1], qa, kb[2], kb[3]);
+        }
+        float* p = sP + (quarter * kQRows + rt * 16 + g) * 16 + 2 * j;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          *reinterpret_cast<float2*>(p + 8 * i) = make_float2(sc[i][0], sc[i][1]);
+          *reinterpret_cast<float2*>(p + 128 + 8 * i) = make_float2(sc[i][2], sc[i][3]);
+        }
+      }
+      if (k0 == 0) {
+#pragma unroll
+        for (int ks = 0; ks < NH; ++ks)
+#pragma unroll
+          for (int rt = 0; rt < 2; ++rt) {
+            uint32_t qa[4];
+            ldsm_x4(qa, aq + rt * (16 * LD * 2) + (fh * NH + ks) * 32);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) mma16816(x[rt][i], qa, hi[ks][i][0], hi[ks][i][1]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) mma16816(x[rt][i], qa, lo[ks][i][0], lo[ks][i][1]);
+          }
+      }
+      __syncthreads();
+      // a' = (q k^T) o M, two keys a thread, and its row sum
+#pragma unroll
+      for (int i = 0; i < kQRows * 8 / NT; ++i) {
+        const int r = (tid + i * NT) >> 3, k = (tid & 7) * 2;
+        float2 p = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float2 v = *reinterpret_cast<const float2*>(sP + (w * kQRows + r) * 16 + k);
+          p.x += v.x;
+          p.y += v.y;
+        }
+        const float2 m = *reinterpret_cast<const float2*>(sM + (r0 + r) % T * TK + k0 + k);
+        p.x *= m.x;
+        p.y *= m.y;
+        den[i] += p.x + p.y;
+        const uint32_t h = pack_bf16(p.x, p.y);
+        sAh[(r * 48 + k * 2) / 4] = h;
+        sAl[(r * 48 + k * 2) / 4] = pack_bf16(p.x - bf16_lo(h), p.y - bf16_hi(h));
+      }
+      __syncthreads();
+      uint32_t vb[4], ph[4], pl[4];  // vb: 16 keys by this warp's two column tiles
+      ldsm_x4_t(vb, av + k0 * (LV * 2));
+      ldsm_x4(ph, aa + fh * (16 * 48));
+      ldsm_x4(pl, aa + kQRows * 48 + fh * (16 * 48));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        mma16816(out[i], ph, vb[2 * i], vb[2 * i + 1]);
+        mma16816(out[i], pl, vb[2 * i], vb[2 * i + 1]);
       }
     }
-    // thread (g, j): rows g, g + 8; tile i's columns 2j, 2j+1 are 4 (2j) + i, 4 (2j+1) + i
-    float* red = sRed + wf * 16 * LDR;
-    const int c0 = wd * 32 + 8 * j;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float* row = red + (g + 8 * h) * LDR + c0;
-      *reinterpret_cast<float4*>(row) =
-          make_float4(acc[0][2 * h], acc[1][2 * h], acc[2][2 * h], acc[3][2 * h]);
-      *reinterpret_cast<float4*>(row + 4) =
-          make_float4(acc[0][2 * h + 1], acc[1][2 * h + 1], acc[2][2 * h + 1], acc[3][2 * h + 1]);
+    for (int i = 0; i < kQRows * 8 / NT; ++i) {
+#pragma unroll
+      for (int w = 1; w < 8; w <<= 1) den[i] += __shfl_xor_sync(0xffffffffu, den[i], w);
+      const int r = (tid + i * NT) >> 3;
+      if ((tid & 7) == 0)  // d_t / den and 1 / den
+        sDen[r] = make_float2(sM[(r0 + r) % T * TK + T], 1.f / fmaxf(den[i], kTiny));
     }
-    // scores of the block's own keys, eight at a time, dealt to the column halves
-    for (int k0 = wd * 8; k0 < TK; k0 += 8 * HALVES) {
-      float sc[4] = {0.f, 0.f, 0.f, 0.f};
+    // the other half's sums of this warp's row tile, over the queries (they are done)
+    float4* sX = reinterpret_cast<float4*>(sQ);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const bf16* kr = sK + (k0 + g) * LD + (wf * KS + ks) * 16 + 2 * j;
-        mma16816(sc, qa[ks], *reinterpret_cast<const uint32_t*>(kr),
-                 *reinterpret_cast<const uint32_t*>(kr + 8));
-      }
+    for (int i = 0; i < 2; ++i)
+      sX[(warp * 2 + i) * 32 + lane] = make_float4(fh ? x[0][i][0] : x[1][i][0],
+                                                   fh ? x[0][i][1] : x[1][i][1],
+                                                   fh ? x[0][i][2] : x[1][i][2],
+                                                   fh ? x[0][i][3] : x[1][i][3]);
+    __syncthreads();
+    const int other = fh ? warp - 2 * HALVES : warp + 2 * HALVES, row = r0 + fh * 16 + g;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float4 o4 = sX[(other * 2 + i) * 32 + lane];
+      const float q[4] = {o4.x, o4.y, o4.z, o4.w};
+      const int dd = d0 + vcol + 8 * i + 2 * j;
+      bf16* yr = a.y + ((size_t)(b * a.H + s * rep) * T + row) * D + dd;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        *reinterpret_cast<float2*>(red + (g + 8 * h) * LDR + DN + k0 + 2 * j) =
-            make_float2(sc[2 * h], sc[2 * h + 1]);
-    }
-    // q . z, a warp per row
-    for (int r = warp; r < 16; r += NT / 32) {
-      float x = 0.f;
+        if (row + 8 * h < R && dd < D && live) {  // D is a multiple of 4
+          const float2 f = sDen[fh * 16 + g + 8 * h];
+          float y[2];
 #pragma unroll
-      for (int f = 0; f < FP / 32; ++f)
-        x += __bfloat162float(sQ[r * LD + lane + 32 * f]) * sZ[lane + 32 * f];
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-      if (lane == 0) sQz[r] = x;
+          for (int e = 0; e < 2; ++e) {
+            const float mine = fh ? x[1][i][2 * h + e] : x[0][i][2 * h + e];
+            y[e] = (f.x * (mine + q[2 * h + e]) + out[i][2 * h + e]) * f.y;
+          }
+          *reinterpret_cast<uint32_t*>(yr + 8 * h * D) = pack_bf16(y[0], y[1]);
+        }
     }
-    __syncthreads();
-    for (int e = tid; e < 16 * T; e += NT) {
-      const int r = e / T, k = e - r * T, t = (r0 + r) % T;
-      float x = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) x += sRed[(w * 16 + r) * LDR + DN + k];
-      sA[r * (TK + 1) + k] = k <= t ? x * sM[t * T + k] : 0.f;
-    }
-    __syncthreads();
-    for (int e = tid; e < 16 * (DN / 4); e += NT) {
-      const int r = e / (DN / 4), c = (e - r * (DN / 4)) * 4, d = d0 + c;
-      if (r0 + r >= R || d >= D) continue;
-      const int t = (r0 + r) % T;
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float4 p = *reinterpret_cast<const float4*>(sRed + (w * 16 + r) * LDR + c);
-        x.x += p.x;
-        x.y += p.y;
-        x.z += p.z;
-        x.w += p.w;
-      }
-      const float dec = sDec[t];
-      float den = dec * sQz[r];
-      x.x *= dec;
-      x.y *= dec;
-      x.z *= dec;
-      x.w *= dec;
-      for (int k = 0; k <= t; ++k) {
-        const float w = sA[r * (TK + 1) + k];
-        const float4 vv = *reinterpret_cast<const float4*>(sV + k * DN + c);
-        den += w;
-        x.x += w * vv.x;
-        x.y += w * vv.y;
-        x.z += w * vv.z;
-        x.w += w * vv.w;
-      }
-      const float inv = 1.f / fmaxf(den, kTiny);
-      bf16* yr = a.y + ((size_t)(b * a.H + s * rep) * T + r0 + r) * D + d;
-      *reinterpret_cast<uint2*>(yr) =
-          make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
-    }
-    __syncthreads();
   }
-}
-
-size_t block_smem(int KS, int HALVES, int T, int Tp) {
-  const int LD = 64 * KS + 8, DN = 32 * HALVES, TK = (T + 7) & ~7, LDR = DN + TK + 4;
-  size_t n = (size_t)(16 + TK + ((Tp + 1) & ~1)) * LD * 2;
-  n += ((size_t)(T + Tp) * DN + 4 * 16 * LDR + 16 * (TK + 1) + (size_t)T * T + T + Tp + 64 * KS +
-        16) * 4;
-  return n;
+  if (tid == 0) tc::bulk_wait_read0();  // the state has left shared memory
 }
 
 template <int KS, int HALVES>
-int launch_gla_block(const GlaBlockArgs& a, unsigned states, cudaStream_t stream) {
-  const size_t smem = block_smem(KS, HALVES, a.T, a.Tp);
-  // the largest block (64 pending and 64 new tokens) needs under the 227 KB limit
+int launch_gla_block(const GlaBlockArgs& a, int B, cudaStream_t stream) {
+  auto fn = tc::encode_tiled_fn();
+  if (!fn) {
+    set_error("lz_gla_decode_block: cuTensorMapEncodeTiled is not available");
+    return LZ_ERR_CUDA;
+  }
+  CUtensorMap ts;
+  const cuuint64_t dims[3] = {(cuuint64_t)a.D, (cuuint64_t)a.F, (cuuint64_t)B * a.Hs};
+  const cuuint64_t strides[2] = {(cuuint64_t)a.D * 4, (cuuint64_t)a.F * a.D * 4};
+  const cuuint32_t box[3] = {32, 64 * KS, 1}, es[3] = {1, 1, 1};
+  const CUresult r = fn(&ts, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, a.S, dims, strides, box, es,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("lz_gla_decode_block: the tensor map of the state could not be encoded, driver code " +
+              std::to_string((int)r));
+    return LZ_ERR_CUDA;
+  }
   static bool done[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 64 && !done[dev]) {
+    const int most = block_smem(KS, HALVES, kMaxBlock).total;
     cudaError_t e = cudaFuncSetAttribute(gla_block_kernel<KS, HALVES>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)block_smem(KS, HALVES, kMaxBlock, kMaxBlock));
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e != cudaSuccess) {
       set_error(std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
       return LZ_ERR_CUDA;
@@ -360,17 +547,17 @@ int launch_gla_block(const GlaBlockArgs& a, unsigned states, cudaStream_t stream
     done[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(states * a.nsl);
+  cfg.gridDim = dim3(B, a.Hs, a.nsl);
   cfg.blockDim = dim3(128 * HALVES);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = block_smem(KS, HALVES, a.T).total;
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = a.nsl;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[0].val.clusterDim.x = at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = a.nsl;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, gla_block_kernel<KS, HALVES>, a);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, gla_block_kernel<KS, HALVES>, ts, a);
   if (e != cudaSuccess) {
     set_error(std::string("gla_block_kernel: ") + cudaGetErrorString(e));
     return LZ_ERR_CUDA;
@@ -380,6 +567,8 @@ int launch_gla_block(const GlaBlockArgs& a, unsigned states, cudaStream_t stream
 }
 
 }  // namespace
+int gla_block_timeout_flag(unsigned int* out) { return tc::read_timeout_flag_here(out); }
+int gla_block_timeout_clear() { return tc::clear_timeout_flag_here(); }
 }  // namespace lz
 
 extern "C" int lz_gla_decode_block(const void* fq, const void* fk, const void* v,
@@ -401,14 +590,15 @@ extern "C" int lz_gla_decode_block(const void* fq, const void* fk, const void* v
              "a block holds at most 64 tokens");
   LZ_REQUIRE(F <= 256 && D % 4 == 0 && D <= 256, LZ_ERR_UNSUPPORTED,
              "decode supports F <= 256 and D a multiple of 4 up to 256");
-  LZ_REQUIRE((long long)B * Hs * 8 < (1ll << 31), LZ_ERR_UNSUPPORTED, "too many state heads");
+  LZ_REQUIRE((long long)B * H * std::max({T, T_prev, 1}) < (1ll << 31) && Hs <= 65535,
+             LZ_ERR_UNSUPPORTED, "too many heads");
   LZ_REQUIRE(state && zstate, LZ_ERR_INVALID_ARGUMENT, "null pointer");
   LZ_REQUIRE(!T || (fq && fk && v && log_gamma && y), LZ_ERR_INVALID_ARGUMENT, "null pointer");
   LZ_REQUIRE(!T_prev || (fk_prev && v_prev && log_gamma_prev), LZ_ERR_INVALID_ARGUMENT,
              "null pointer in the previous block");
   LZ_REQUIRE(aligned16(state), LZ_ERR_INVALID_ARGUMENT, "state must be 16-byte aligned");
-  LZ_REQUIRE(!T || (reinterpret_cast<uintptr_t>(y) & 7) == 0, LZ_ERR_INVALID_ARGUMENT,
-             "y must be 8-byte aligned");
+  LZ_REQUIRE(!T || (reinterpret_cast<uintptr_t>(y) & 3) == 0, LZ_ERR_INVALID_ARGUMENT,
+             "y must be 4-byte aligned");
   GlaBlockArgs a;
   a.fq = static_cast<const bf16*>(fq);
   a.fk = static_cast<const bf16*>(fk);
@@ -430,13 +620,14 @@ extern "C" int lz_gla_decode_block(const void* fq, const void* fk, const void* v
   a.F = F;
   a.D = D;
   auto st = static_cast<cudaStream_t>(stream);
-  const unsigned states = (unsigned)(B * Hs);
   const int ks = ceil_div(F, 64), halves = D > 32 ? 2 : 1;
   a.nsl = ceil_div(D, 32 * halves);
+  a.rep = H / Hs;
+  a.kvrep = Hs / Hkv;
 #define LZ_GB(K_)                                                      \
   case K_:                                                             \
-    return halves == 2 ? launch_gla_block<K_, 2>(a, states, st) \
-                       : launch_gla_block<K_, 1>(a, states, st);
+    return halves == 2 ? launch_gla_block<K_, 2>(a, B, st) \
+                       : launch_gla_block<K_, 1>(a, B, st);
   switch (ks) {
     LZ_GB(1) LZ_GB(2) LZ_GB(3) LZ_GB(4)
   }
