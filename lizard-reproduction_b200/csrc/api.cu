@@ -30,6 +30,7 @@ int swa_tc_timeout_flag(unsigned int* out);
 int decode_timeout_flag(unsigned int* out);
 int int8_timeout_flag(unsigned int* out);
 int gla_block_timeout_flag(unsigned int* out);
+int swa_block_timeout_flag(unsigned int* out);
 int gla_fwd_tc_timeout_clear();
 int gla_fwd_tc64_timeout_clear();
 int gla_bwd_tc_timeout_clear();
@@ -40,6 +41,7 @@ int swa_tc_timeout_clear();
 int decode_timeout_clear();
 int int8_timeout_clear();
 int gla_block_timeout_clear();
+int swa_block_timeout_clear();
 }  // namespace lz
 
 extern "C" int lz_device_timeout_flag(unsigned int* site) {
@@ -49,7 +51,7 @@ extern "C" int lz_device_timeout_flag(unsigned int* site) {
       lz::gla_fwd_tc_timeout_flag, lz::gla_fwd_tc64_timeout_flag, lz::gla_bwd_tc_timeout_flag,
       lz::gla_out_tc_timeout_flag, lz::hedgehog_timeout_flag,     lz::swa_timeout_flag,
       lz::swa_tc_timeout_flag,     lz::decode_timeout_flag,    lz::int8_timeout_flag,
-      lz::gla_block_timeout_flag};
+      lz::gla_block_timeout_flag,  lz::swa_block_timeout_flag};
   *site = 0;
   for (auto rd : readers) {
     unsigned int v = 0;
@@ -69,7 +71,7 @@ extern "C" int lz_device_timeout_clear(void) {
       lz::gla_fwd_tc_timeout_clear, lz::gla_fwd_tc64_timeout_clear, lz::gla_bwd_tc_timeout_clear,
       lz::gla_out_tc_timeout_clear, lz::hedgehog_timeout_clear,     lz::swa_timeout_clear,
       lz::swa_tc_timeout_clear,     lz::decode_timeout_clear,     lz::int8_timeout_clear,
-      lz::gla_block_timeout_clear};
+      lz::gla_block_timeout_clear,  lz::swa_block_timeout_clear};
   for (auto cl : clearers) {
     const int rc = cl();
     if (rc) return rc;

@@ -9,15 +9,27 @@
 // over the keys at positions base + t - W < position <= base + t. The block's
 // own keys never enter the ring here, so a refused token leaves no trace.
 //
-// One CTA per (batch row, key/value head): the ring is read once for all rep T
-// query rows of the group. 64 keys at a time are staged in shared memory as
-// bf16 hi + lo parts (the ring is fp32; hi hi + hi lo + lo hi keeps 2^-17 of
-// the product, well under the bf16 output) and contracted with mma.sync
-// m16n8k16; each of the four warps of a 16-row tile takes 16 of the 64 keys
-// with its own running maximum and sum, and the four are merged at the end, so
-// a block of few rows still keeps every warp busy. Bound: 8 (W + T) D bytes of
-// ring a head against 4 rep T (W + T) D operations: memory.
+// One CTA per (batch row, key/value head) for all rep T query rows of the group.
+// Bound: 8 (W + T) D bytes of ring a head against 4 rep T (W + T) D operations:
+// memory. TMA brings the whole ring (of a long window, a part at a time) into
+// shared memory as it is, fp32 in 128-byte swizzled rows, while the queries and the
+// new keys are rotated; the accepted tokens are written over their slots there and
+// in global memory. A warp takes a 16-row tile of queries over 16 keys at a time: it
+// reads the keys as the B fragments of mma.sync m16n8k16, splits them into bf16 hi + lo
+// in registers (hi hi + hi lo + lo hi keeps 2^-17 of a product, well under the bf16
+// output) and keeps its own maximum and sum; the warps' outputs meet at the end,
+// scaled to the common maximum, so a block of few rows keeps every warp busy. Nothing
+// converted is written back to shared memory. (A warp on two row tiles converts a
+// key once instead of twice, but its registers leave 16 warps an SM for 24, and
+// the nine 16-key tiles of a window of 128 and its block do not divide over eight.)
+//
+// Fragments. Within a step of 16 columns thread j takes d = 4j .. 4j+3 (the
+// queries are stored in that order), so a key is one 16-byte read; column tile i
+// of 32 stands for d = 4n + i, so a value is one 16-byte read too. The keys of an
+// 8-tile sit in rows 0 5 2 7 4 1 6 3: with the swizzle (16-byte chunk ^ row & 7)
+// both reads are then free of bank conflicts.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "tc.cuh"
@@ -27,7 +39,7 @@ namespace {
 
 constexpr int kMaxBlock = 64;    // tokens a block
 constexpr int kMaxWindow = 1024;  // as the single-token step
-constexpr int kKeys = 64;        // keys a staged tile
+constexpr int kWarps = 10;        // most warps a CTA
 
 struct Heads {  // [B, heads, T, D] in place: strides in elements, last dimension contiguous
   const void* p;
@@ -46,6 +58,9 @@ struct SwaBlockArgs {
   float *kr, *vr;
   bf16* y;
   int n_meta, T, Tp, H, Hkv, W, D;
+  int rep;    // query heads a key/value head
+  int part;   // ring rows in shared memory at a time, a multiple of 16
+  int tma;    // the rings can be read by TMA
 };
 
 template <typename T>
@@ -58,299 +73,528 @@ template <>
 __device__ __forceinline__ float ldx<bf16>(const void* p, long long i) {
   return __bfloat162float(static_cast<const bf16*>(p)[i]);
 }
-__device__ __forceinline__ float ldr(const void* p, long long i, int is_bf16) {
-  return is_bf16 ? ldx<bf16>(p, i) : ldx<float>(p, i);
+// N (1 or 2) neighbouring values.
+template <typename XT, int N>
+__device__ __forceinline__ float2 ldn(const XT* p) {
+  if constexpr (N == 1) {
+    return make_float2(ldx<XT>(p, 0), 0.f);
+  } else if constexpr (sizeof(XT) == 4) {
+    return *reinterpret_cast<const float2*>(p);
+  } else {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+    return make_float2(bf16_lo(w), bf16_hi(w));
+  }
+}
+// cos and sin at columns d .. d + N - 1 and the same plus D / 2 of one token.
+struct Angle {
+  float2 c1, c2, s1, s2;
+};
+template <int N>
+__device__ __forceinline__ Angle angle(const Rotary& r, long long at, int half) {
+  if (r.bf16_) {
+    const bf16 *c = static_cast<const bf16*>(r.cos) + at, *s = static_cast<const bf16*>(r.sin) + at;
+    return {ldn<bf16, N>(c), ldn<bf16, N>(c + half), ldn<bf16, N>(s), ldn<bf16, N>(s + half)};
+  }
+  const float *c = static_cast<const float*>(r.cos) + at, *s = static_cast<const float*>(r.sin) + at;
+  return {ldn<float, N>(c), ldn<float, N>(c + half), ldn<float, N>(s), ldn<float, N>(s + half)};
+}
+// The rotated columns of a row's x1 (d ..) and x2 (d + D / 2 ..), each product and
+// sum rounded once, as the single-token step rounds them.
+__device__ __forceinline__ void rotate(float2& x1, float2& x2, const Angle& a) {
+  const float2 y1 = x1, y2 = x2;
+  x1.x = __fadd_rn(__fmul_rn(y1.x, a.c1.x), -__fmul_rn(y2.x, a.s1.x));
+  x1.y = __fadd_rn(__fmul_rn(y1.y, a.c1.y), -__fmul_rn(y2.y, a.s1.y));
+  x2.x = __fadd_rn(__fmul_rn(y2.x, a.c2.x), __fmul_rn(y1.x, a.s2.x));
+  x2.y = __fadd_rn(__fmul_rn(y2.y, a.c2.y), __fmul_rn(y1.y, a.s2.y));
 }
 
-// The rotated pair (d, d + D / 2) of a row, each product and sum rounded once,
-// as the single-token step rounds them.
-template <typename XT>
-__device__ __forceinline__ float2 rotated(const void* x, long long row, const Rotary& r,
-                                          long long crow, int d, int half) {
-  const float x1 = ldx<XT>(x, row + d), x2 = ldx<XT>(x, row + d + half);
-  const float c1 = ldr(r.cos, crow + d, r.bf16_), s1 = ldr(r.sin, crow + d, r.bf16_);
-  const float c2 = ldr(r.cos, crow + d + half, r.bf16_), s2 = ldr(r.sin, crow + d + half, r.bf16_);
-  return make_float2(__fadd_rn(__fmul_rn(x1, c1), -__fmul_rn(x2, s1)),
-                     __fadd_rn(__fmul_rn(x2, c2), __fmul_rn(x1, s2)));
+// The place of column d of row r in a tile of DP / 32 boxes of `rows` swizzled
+// 128-byte rows each, in floats.
+__device__ __forceinline__ int spot(int rows, int r, int d) {
+  return ((d >> 5) * rows + r) * 32 + ((((d >> 2) & 7) ^ (r & 7)) << 2) + (d & 3);
+}
+// The place of query column d in its row: thread j's four columns of a step are
+// the mma's k slots 2j, 2j + 1, 2j + 8, 2j + 9.
+__device__ __forceinline__ int slot_of(int d) {
+  return (d & ~15) + ((d >> 2) & 3) * 2 + (d & 1) + ((d >> 1) & 1) * 8;
+}
+// The row of an 8-tile that holds key n of the mma.
+__device__ __forceinline__ int key_row(int n) { return n ^ ((n & 1) << 2); }
+
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  hi = pack_bf16(x, y);
+  lo = pack_bf16(x - bf16_lo(hi), y - bf16_hi(hi));
+}
+// N columns to their places (neighbours stay neighbours).
+template <int N>
+__device__ __forceinline__ void put(float* p, float2 x) {
+  if constexpr (N == 2)
+    *reinterpret_cast<float2*>(p) = x;
+  else
+    *p = x.x;
+}
+template <int N>
+__device__ __forceinline__ void put_split(bf16* hi, bf16* lo, int at, float2 x) {
+  uint32_t h, l;
+  split2(x.x, x.y, h, l);
+  if constexpr (N == 2) {
+    *reinterpret_cast<uint32_t*>(hi + at) = h;
+    *reinterpret_cast<uint32_t*>(lo + at) = l;
+  } else {
+    hi[at] = __ushort_as_bfloat16((unsigned short)h);
+    lo[at] = __ushort_as_bfloat16((unsigned short)l);
+  }
 }
 
-__device__ __forceinline__ void put(bf16* hi, bf16* lo, int at, float x) {
-  const bf16 h = __float2bfloat16_rn(x);
-  hi[at] = h;
-  lo[at] = __float2bfloat16_rn(x - __bfloat162float(h));
-}
-__device__ __forceinline__ void put4(bf16* hi, bf16* lo, int at, float4 x) {
-  const uint32_t h0 = pack_bf16(x.x, x.y), h1 = pack_bf16(x.z, x.w);
-  *reinterpret_cast<uint2*>(hi + at) = make_uint2(h0, h1);
-  *reinterpret_cast<uint2*>(lo + at) =
-      make_uint2(pack_bf16(x.x - bf16_lo(h0), x.y - bf16_hi(h0)),
-                 pack_bf16(x.z - bf16_lo(h1), x.w - bf16_hi(h1)));
+// Shared memory, in bytes from the 1024-aligned start.
+struct SwaSmem {
+  int k, v, nk, nv, q, stat, bar, total;
+};
+__host__ __device__ inline SwaSmem swa_smem(int DP, int QT, int part, int T, int warps) {
+  SwaSmem s;
+  const int new_rows = (T + 15) & ~15;
+  int n = 0;
+  s.k = n, n += part * DP * 4;
+  s.v = n, n += part * DP * 4;
+  s.nk = n, n += new_rows * DP * 4;
+  s.nv = n, n += new_rows * DP * 4;
+  const int merge = warps * 16 * (DP + 4) * 4;  // the warps' outputs, over the keys
+  if (n < merge) n = (merge + 1023) & ~1023;
+  s.q = n, n += 2 * 16 * QT * (DP + 8) * 2;
+  s.stat = n, n += 3 * warps * 16 * 4;
+  s.bar = n, n += 8;
+  s.total = n + 1024;
+  return s;
 }
 
-constexpr size_t swa_block_smem(int DP, int RT) {
-  return (size_t)(4 * kKeys + 2 * 16 * RT) * (DP + 8) * 2 + (kKeys + 2 * 64 * RT) * 4;
-}
-
-// DP: D padded to whole mma steps. RT: 16-row tiles of queries at once.
-template <typename XT, int DP, int RT>
-__global__ void __launch_bounds__(128 * RT)
-swa_block_kernel(const SwaBlockArgs a) {
-  constexpr int NT = 128 * RT, LD = DP + 8, NS = DP / 16;
-  extern __shared__ __align__(16) unsigned char smraw[];
-  bf16* sKh = reinterpret_cast<bf16*>(smraw);
-  bf16* sKl = sKh + kKeys * LD;
-  bf16* sVh = sKl + kKeys * LD;
-  bf16* sVl = sVh + kKeys * LD;
-  bf16* sQh = sVl + kKeys * LD;
-  bf16* sQl = sQh + 16 * RT * LD;
-  int* sRel = reinterpret_cast<int*>(sQl + 16 * RT * LD);  // [64] position - base
-  float* sMax = reinterpret_cast<float*>(sRel + kKeys);    // [RT][4][16]
-  float* sSum = sMax + 64 * RT;
-  float* sO = reinterpret_cast<float*>(smraw);             // [RT][4][16][DP], after the last tile
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int wk = warp & 3, rt = warp >> 2, g = lane >> 2, j = lane & 3;
-  const int T = a.T, W = a.W, D = a.D, half = D / 2;
-  const int bk = blockIdx.x, b = bk / a.Hkv, hk = bk - b * a.Hkv;
-  const int rep = a.H / a.Hkv, R = rep * T;
-  const int pos = a.pos[b];
-  const int n = a.Tp ? (a.count ? min(max(a.count[b], 0), a.Tp) : a.Tp) : 0;
+// DP: D padded to whole 32s. QT: 16-row tiles of queries at once, one a warp. N:
+// columns a thread rotates at once (2 where alignment allows).
+template <typename XT, int DP, int QT, int N>
+__global__ void __launch_bounds__(32 * kWarps, DP <= 64 ? 2 : 1)
+swa_block_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                 const SwaBlockArgs a) {
+  constexpr int LQ = DP + 8, NS = DP / 16, NG = DP / 32, LO = DP + 4, RQ = 16 * QT;
+  extern __shared__ unsigned char raw[];
+  unsigned char* sm = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, nw = nt >> 5;
+  const int g = lane >> 2, j = lane & 3;
+  const int T = a.T, W = a.W, D = a.D, half = D / 2, part = a.part;
+  const int TN = (T + 15) & ~15;  // rows of the new tokens' tile
+  const SwaSmem o = swa_smem(DP, QT, part, T, nw);
+  float* sK = reinterpret_cast<float*>(sm + o.k);
+  float* sV = reinterpret_cast<float*>(sm + o.v);
+  float* sNK = reinterpret_cast<float*>(sm + o.nk);
+  float* sNV = reinterpret_cast<float*>(sm + o.nv);
+  float* sO = reinterpret_cast<float*>(sm);             // [warp][16][LO], after the last key
+  bf16* sQh = reinterpret_cast<bf16*>(sm + o.q);        // [RQ][LQ]
+  bf16* sQl = sQh + RQ * LQ;
+  float* sMax = reinterpret_cast<float*>(sm + o.stat);  // [warp][16]
+  float* sSum = sMax + nw * 16;
+  float* sCof = sSum + nw * 16;
+  uint64_t* bar = reinterpret_cast<uint64_t*>(sm + o.bar);
+  const int b = blockIdx.x, hk = blockIdx.y, bk = b * a.Hkv + hk;
+  const int rep = a.rep, R = rep * T;
   float* kring = a.kr + (size_t)bk * W * D;
   float* vring = a.vr + (size_t)bk * W * D;
+  const int parts = (W + part - 1) / part;
+  uint32_t phase = 0;
 
-  // accepted tokens of the previous block (of more than W, the last W)
-  const int t0 = max(0, n - W);
-  for (int e = tid; e < (n - t0) * half; e += NT) {
-    const int t = t0 + e / half, d = e % half, slot = (int)(((long long)pos + t) % W);
-    const float2 kk = rotated<XT>(a.kp.p, b * a.kp.sb + hk * a.kp.sh + t * a.kp.st, a.rot_p,
-                                  b * a.rot_p.sb + (long long)t * D, d, half);
-    kring[(size_t)slot * D + d] = kk.x;
-    kring[(size_t)slot * D + d + half] = kk.y;
-    const long long vrow = b * a.vp.sb + hk * a.vp.sh + t * a.vp.st;
-    vring[(size_t)slot * D + d] = ldx<XT>(a.vp.p, vrow + d);
-    vring[(size_t)slot * D + d + half] = ldx<XT>(a.vp.p, vrow + d + half);
-  }
-  if (!T) return;
-  const long long base = (long long)pos + n;
-  const int nr = base < W ? (int)base : W;  // ring rows that hold a token
-  const int last = (int)((base - 1 + W) % W);  // slot of the newest (W >= 1)
-  const int N = nr + T;
-  const float scale = rsqrtf((float)D) * kLog2e;
-  const bool vec = (D & 3) == 0 && ((reinterpret_cast<uintptr_t>(a.kr) |
-                                     reinterpret_cast<uintptr_t>(a.vr)) & 15) == 0;
-
-  for (int r0 = 0; r0 < R; r0 += 16 * RT) {
-    __syncthreads();  // the ring writes above; the merge of the rows before
-    for (int e = tid; e < 16 * RT * (DP / 2); e += NT) {
-      const int r = e / (DP / 2), d = e - r * (DP / 2), row = r0 + r;
-      if (row < R && d < half) {
-        const int h = row / T, t = row - h * T;
-        const float2 x =
-            rotated<XT>(a.q.p, b * a.q.sb + (hk * rep + h) * a.q.sh + t * a.q.st, a.rot,
-                        b * a.rot.sb + (long long)t * D, d, half);
-        put(sQh, sQl, r * LD + d, x.x);
-        put(sQh, sQl, r * LD + d + half, x.y);
-      } else if (row >= R) {
-        put(sQh, sQl, r * LD + 2 * d, 0.f);
-        put(sQh, sQl, r * LD + 2 * d + 1, 0.f);
-      } else {  // the padding columns D .. DP
-        put(sQh, sQl, r * LD + 2 * d, 0.f);
-        put(sQh, sQl, r * LD + 2 * d + 1, 0.f);
+  // ring rows [p part, (p + 1) part) into sK / sV
+  const auto load_part = [&](int p) {
+    if (a.tma) {
+      if (tid == 0) {
+        tc::mbar_expect_tx(bar, 2 * part * DP * 4);  // rows and columns beyond the ring: zeros
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+          tc::tma_load_3d(sK + i * part * 32, &tk, 32 * i, p * part, bk, bar);
+          tc::tma_load_3d(sV + i * part * 32, &tv, 32 * i, p * part, bk, bar);
+        }
+      }
+    } else {
+      for (int e = tid; e < part * DP; e += nt) {
+        const int r = e / DP, d = e - r * DP, slot = p * part + r;
+        const bool in = slot < W && d < D;
+        sK[spot(part, r, d)] = in ? kring[(size_t)slot * D + d] : 0.f;
+        sV[spot(part, r, d)] = in ? vring[(size_t)slot * D + d] : 0.f;
       }
     }
-    float m[2] = {-1e30f, -1e30f}, l[2] = {0.f, 0.f};
-    float o[DP / 8][4];
-#pragma unroll
-    for (int i = 0; i < DP / 8; ++i)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) o[i][c] = 0.f;
-    // this thread's two rows: their token within the block
-    const int rowa = r0 + rt * 16 + g;
-    const int ta = rowa % T, tb = (rowa + 8) % T;
+  };
+  if (tid == 0) {
+    tc::mbar_init(bar, 1);
+    tc::fence_mbar_init();
+  }
+  if (T) load_part(0);
 
-    for (int k0 = 0; k0 < N; k0 += kKeys) {
-      if (k0) __syncthreads();  // the tile before has been used
-      const int nring = min(max(nr - k0, 0), kKeys);  // ring rows of this tile
-      for (int e = tid; e < kKeys * (DP / 4); e += NT) {
-        const int r = e / (DP / 4), c = (e - r * (DP / 4)) * 4;
-        float4 kk = make_float4(0.f, 0.f, 0.f, 0.f), vv = kk;
-        if (r < nring) {
-          const size_t at = (size_t)(k0 + r) * D + c;
-          if (vec) {
-            if (c < D) {
-              kk = *reinterpret_cast<const float4*>(kring + at);
-              vv = *reinterpret_cast<const float4*>(vring + at);
-            }
+  const int pos = a.pos[b];
+  const int n = a.Tp ? (a.count ? min(max(a.count[b], 0), a.Tp) : a.Tp) : 0;
+  const int t0 = max(0, n - W);  // of more accepted tokens than the window, the last W
+  const int first = pos % W;
+  // Half a warp takes a token, a lane N columns and those D / 2 further.
+  const int unit = tid >> 4, units = nt >> 4, lane16 = tid & 15;
+  // accepted token t: its rotated key and its value
+  struct Entry {
+    float2 k1, k2, v1, v2;
+  };
+  const XT* kp = static_cast<const XT*>(a.kp.p) + b * a.kp.sb + hk * a.kp.sh;
+  const XT* vp = static_cast<const XT*>(a.vp.p) + b * a.vp.sb + hk * a.vp.sh;
+  const auto entry = [&](int t, int d) {
+    const XT *k = kp + t * a.kp.st + d, *v = vp + t * a.vp.st + d;
+    Entry e = {ldn<XT, N>(k), ldn<XT, N>(k + half), ldn<XT, N>(v), ldn<XT, N>(v + half)};
+    rotate(e.k1, e.k2, angle<N>(a.rot_p, b * a.rot_p.sb + (long long)t * D + d, half));
+    return e;
+  };
+  // to the ring, and to the copy of its rows row0 .. in shared memory
+  const auto put_entry = [&](const Entry& e, int t, int d, int row0, bool ring) {
+    const int slot = (first + t) % W, at = slot - row0;
+    if (T && at >= 0 && at < part) {
+      const int s1 = spot(part, at, d), s2 = spot(part, at, d + half);
+      put<N>(sK + s1, e.k1);
+      put<N>(sK + s2, e.k2);
+      put<N>(sV + s1, e.v1);
+      put<N>(sV + s2, e.v2);
+    }
+    if (ring) {
+      put<N>(kring + slot * D + d, e.k1);
+      put<N>(kring + slot * D + d + half, e.k2);
+      put<N>(vring + slot * D + d, e.v1);
+      put<N>(vring + slot * D + d + half, e.v2);
+    }
+  };
+  if (!T) {
+    for (int t = t0 + unit; t < n; t += units)
+      for (int d = lane16 * N; d < half; d += 16 * N) put_entry(entry(t, d), t, d, 0, true);
+    return;
+  }
+  // a token a unit loads now and waits in registers for the ring; others come later
+  const int mine = t0 + unit, dm = lane16 * N;
+  Entry early = {};
+  if (mine < n && dm < half) early = entry(mine, dm);
+
+  const int nr = (int)min((long long)pos + n, (long long)W);  // ring rows that hold a token
+  const int last = (first + n - 1 + W) % W;                   // slot of the newest (W >= 1)
+  const float scale = rsqrtf((float)D) * kLog2e;
+  const int krow = key_row(g), eight = 8 % T;
+  const int rt = QT == 1 ? 0 : warp % QT;                     // this warp's row tile
+  const int kw = QT == 1 ? warp : warp / QT, kws = nw / QT;   // and its turn among the keys
+  bool live = true;  // after a timeout nothing is written
+
+  for (int r0 = 0; r0 < R; r0 += RQ) {
+    if (r0) {  // the merge of the rows before went over the keys: both again
+      tc::fence_proxy_async_smem();
+      __syncthreads();
+      load_part(0);
+    }
+    // zeros: keys T .. TN, query rows beyond R, columns D .. DP
+    for (int e = tid; e < (TN - T) * DP; e += nt) {
+      const int at = spot(TN, T + e / DP, e % DP);
+      sNK[at] = sNV[at] = 0.f;
+    }
+    for (int e = (R - r0) * LQ + tid; e < RQ * LQ; e += nt)
+      sQh[e] = sQl[e] = __float2bfloat16_rn(0.f);
+    if (D < DP) {
+      for (int e = tid; e < T * (DP - D); e += nt) {
+        const int at = spot(TN, e / (DP - D), D + e % (DP - D));
+        sNK[at] = sNV[at] = 0.f;
+      }
+      for (int e = tid; e < RQ * (DP - D); e += nt) {
+        const int at = e / (DP - D) * LQ + slot_of(D + e % (DP - D));
+        sQh[at] = sQl[at] = __float2bfloat16_rn(0.f);
+      }
+    }
+    {
+      // a token's rows two at a time: two query heads, or its key and value
+      const XT* qp = static_cast<const XT*>(a.q.p) + b * a.q.sb + hk * rep * a.q.sh;
+      const XT* kb = static_cast<const XT*>(a.k.p) + b * a.k.sb + hk * a.k.sh;
+      const XT* vb = static_cast<const XT*>(a.v.p) + b * a.v.sb + hk * a.v.sh;
+      const int groups = (rep + 1) / 2 + 1;
+      for (int i = unit; i < T * groups; i += units) {
+        const int grp = i / T, t = i - grp * T, h = 2 * grp;
+        const bool kv = grp + 1 == groups;
+        const XT* pa = kv ? kb + t * a.k.st : qp + h * a.q.sh + t * a.q.st;
+        const XT* pb = kv ? vb + t * a.v.st : pa + a.q.sh;
+        const int ra = h * T + t - r0, rb = ra + T;  // query rows of this pass
+        const bool two = kv || h + 1 < rep;
+        for (int d = lane16 * N; d < half; d += 16 * N) {
+          const Angle ang = angle<N>(a.rot, b * a.rot.sb + (long long)t * D + d, half);
+          float2 a1 = ldn<XT, N>(pa + d), a2 = ldn<XT, N>(pa + d + half), b1 = {}, b2 = {};
+          if (two) b1 = ldn<XT, N>(pb + d), b2 = ldn<XT, N>(pb + d + half);
+          rotate(a1, a2, ang);
+          if (kv) {
+            const int s1 = spot(TN, t, d), s2 = spot(TN, t, d + half);
+            put<N>(sNK + s1, a1);
+            put<N>(sNK + s2, a2);
+            put<N>(sNV + s1, b1);
+            put<N>(sNV + s2, b2);
           } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (c + i < D) {
-                reinterpret_cast<float*>(&kk)[i] = kring[at + i];
-                reinterpret_cast<float*>(&vv)[i] = vring[at + i];
-              }
+            rotate(b1, b2, ang);
+            const int c1 = slot_of(d), c2 = slot_of(d + half);
+            if (ra >= 0 && ra < RQ) {
+              put_split<N>(sQh, sQl, ra * LQ + c1, a1);
+              put_split<N>(sQh, sQl, ra * LQ + c2, a2);
+            }
+            if (two && rb >= 0 && rb < RQ) {
+              put_split<N>(sQh, sQl, rb * LQ + c1, b1);
+              put_split<N>(sQh, sQl, rb * LQ + c2, b2);
+            }
           }
         }
-        put4(sKh, sKl, r * LD + c, kk);
-        put4(sVh, sVl, r * LD + c, vv);
       }
-      for (int r = tid; r < kKeys; r += NT) {
-        const int i = k0 + r;
-        // a ring slot holds the last position before base that falls on it
-        const int back = last - i;
-        sRel[r] = i < nr ? -1 - (back < 0 ? back + W : back) : (i < N ? i - nr : 1 << 30);
+    }
+    float m[2] = {-1e30f, -1e30f}, l[2] = {0.f, 0.f}, acc[4 * NG][4];
+#pragma unroll
+    for (int i = 0; i < 4 * NG; ++i)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[i][c] = 0.f;
+    int tq[2];  // the tokens of this thread's rows
+    tq[0] = (r0 + rt * 16 + g) % T;
+    tq[1] = tq[0] + eight;
+    if (tq[1] >= T) tq[1] -= T;
+
+    for (int p = 0; p < parts; ++p) {
+      if (p) {
+        tc::fence_proxy_async_smem();
+        __syncthreads();  // the part before has been used
+        load_part(p);
       }
-      if (nring < kKeys) {  // the block's own keys follow the ring's
-        __syncthreads();    // over the zeros written above
-        const int s0 = k0 + nring - nr, ns = min(kKeys - nring, T - s0);
-        for (int e = tid; e < ns * half; e += NT) {
-          const int i = e / half, d = e - i * half, s = s0 + i, at = (nring + i) * LD + d;
-          const float2 kk = rotated<XT>(a.k.p, b * a.k.sb + hk * a.k.sh + s * a.k.st, a.rot,
-                                        b * a.rot.sb + (long long)s * D, d, half);
-          put(sKh, sKl, at, kk.x);
-          put(sKh, sKl, at + half, kk.y);
-          const long long vrow = b * a.v.sb + hk * a.v.sh + s * a.v.st;
-          put(sVh, sVl, at, ldx<XT>(a.v.p, vrow + d));
-          put(sVh, sVl, at + half, ldx<XT>(a.v.p, vrow + d + half));
-        }
+      if (!p && !r0) __syncthreads();  // the barrier is initialised
+      if (a.tma) {
+        live = tc::mbar_wait(bar, phase, 96) && live;
+        phase ^= 1;
+      } else {
+        __syncthreads();
+      }
+      // the accepted tokens over what came, and (once) into the ring
+      const bool ring = !p && !r0 && live;
+      if (mine < n) {
+        if (dm < half) put_entry(early, mine, dm, p * part, ring);
+        for (int t = mine; t < n; t += units)
+          for (int d = t == mine ? dm + 16 * N : dm; d < half; d += 16 * N)
+            put_entry(entry(t, d), t, d, p * part, ring);
       }
       __syncthreads();
-      // scores of this warp's 16 keys
-      float sc[2][4];
+      const int held = min(max(nr - p * part, 0), part);  // rows of this part that hold a token
+      const int ring_tiles = (held + 15) >> 4;
+      const int tiles = ring_tiles + (p + 1 == parts ? TN >> 4 : 0);
+      for (int tl = kw; tl < tiles; tl += kws) {
+        const bool own = tl >= ring_tiles;
+        const int rows = own ? TN : part, row0 = (own ? tl - ring_tiles : tl) * 16;
+        const float* kt = own ? sNK : sK;
+        const float* vt = own ? sNV : sV;
+        // scores of 16 keys
+        float sc[2][4];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) sc[i][c] = 0.f;
+          for (int c = 0; c < 4; ++c) sc[i][c] = 0.f;
+        const float* kg = kt + (row0 + krow) * 32;
 #pragma unroll
-      for (int ks = 0; ks < NS; ++ks) {
-        uint32_t qh[4], ql[4], kh[4], kl[4];
-        lda_rm(qh, sQh, LD, rt * 16, ks * 16);
-        lda_rm(ql, sQl, LD, rt * 16, ks * 16);
-        ldb_nk(kh, sKh, LD, wk * 16, ks * 16);
-        ldb_nk(kl, sKl, LD, wk * 16, ks * 16);
+        for (int ks = 0; ks < NS; ++ks) {
+          uint32_t qh[4], ql[4];
+          lda_rm(qh, sQh, LQ, rt * 16, ks * 16);
+          lda_rm(ql, sQl, LQ, rt * 16, ks * 16);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          mma16816(sc[i], qh, kh[2 * i], kh[2 * i + 1]);
-          mma16816(sc[i], qh, kl[2 * i], kl[2 * i + 1]);
-          mma16816(sc[i], ql, kh[2 * i], kh[2 * i + 1]);
+          for (int i = 0; i < 2; ++i) {
+            const float4 x = *reinterpret_cast<const float4*>(
+                kg + ((ks >> 1) * rows + 8 * i) * 32 + ((((ks & 1) * 4 + j) ^ krow) << 2));
+            uint32_t kh[2], kl[2];
+            split2(x.x, x.y, kh[0], kl[0]);
+            split2(x.z, x.w, kh[1], kl[1]);
+            mma16816(sc[i], qh, kh[0], kh[1]);
+            mma16816(sc[i], qh, kl[0], kl[1]);
+            mma16816(sc[i], ql, kh[0], kh[1]);
+          }
         }
-      }
-      float mx[2] = {m[0], m[1]};
+        // position - base of this thread's keys 8 i + 2 j + c; a ring slot holds the
+        // last position before base that falls on it
+        int rel[4];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int rel = sRel[wk * 16 + i * 8 + 2 * j + (c & 1)], t = c < 2 ? ta : tb;
-          sc[i][c] = rel <= t && rel > t - W ? sc[i][c] * scale : -INFINITY;
-          mx[c >> 1] = fmaxf(mx[c >> 1], sc[i][c]);
+        for (int i = 0; i < 4; ++i) {
+          const int k = row0 + (i >> 1) * 8 + key_row(2 * j + (i & 1));
+          const int back = last - (p * part + k);
+          rel[i] = own ? (k < T ? k : 1 << 30)
+                       : (k < held ? -1 - (back < 0 ? back + W : back) : 1 << 30);
         }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-        const float f = tc::ex2(m[h] - mx[h]);
-        m[h] = mx[h];
-        l[h] *= f;
-#pragma unroll
-        for (int i = 0; i < DP / 8; ++i) {
-          o[i][2 * h] *= f;
-          o[i][2 * h + 1] *= f;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          sc[i][c] = tc::ex2(sc[i][c] - m[c >> 1]);
-          l[c >> 1] += sc[i][c];
-        }
-      uint32_t ph[4], pl[4];
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
+        uint32_t ph[4], pl[4];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float x0 = sc[i][2 * h], x1 = sc[i][2 * h + 1];
-          const uint32_t p = pack_bf16(x0, x1);
-          ph[2 * i + h] = p;
-          pl[2 * i + h] = pack_bf16(x0 - bf16_lo(p), x1 - bf16_hi(p));
+          const int t = tq[h];
+          float mx = m[h];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float& x = sc[i >> 1][2 * h + (i & 1)];
+            x = rel[i] <= t && rel[i] > t - W ? x * scale : -INFINITY;
+            mx = fmaxf(mx, x);
+          }
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          if (tl != kw || p) {  // not the first keys: rescale
+            const float f = tc::ex2(m[h] - mx);
+            l[h] *= f;
+#pragma unroll
+            for (int i = 0; i < 4 * NG; ++i) {
+              acc[i][2 * h] *= f;
+              acc[i][2 * h + 1] *= f;
+            }
+          }
+          m[h] = mx;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float x0 = tc::ex2(sc[i][2 * h] - mx), x1 = tc::ex2(sc[i][2 * h + 1] - mx);
+            l[h] += x0 + x1;
+            split2(x0, x1, ph[2 * i + h], pl[2 * i + h]);
+          }
         }
+        // values: rows of keys 2j, 2j + 1, 2j + 8, 2j + 9, columns 4 g .. 4 g + 3 of each 32
+        const int va = row0 + key_row(2 * j), vb = row0 + key_row(2 * j + 1);
+        const int lim = own ? T : held;  // rows beyond hold nothing (perhaps not numbers)
 #pragma unroll
-      for (int i = 0; i < DP / 16; ++i) {
-        uint32_t vh[4], vl[4];
-        ldb_kn(vh, sVh, LD, wk * 16, i * 16);
-        ldb_kn(vl, sVl, LD, wk * 16, i * 16);
+        for (int q = 0; q < NG; ++q) {
+          float4 x[4];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          mma16816(o[2 * i + u], ph, vh[2 * u], vh[2 * u + 1]);
-          mma16816(o[2 * i + u], ph, vl[2 * u], vl[2 * u + 1]);
-          mma16816(o[2 * i + u], pl, vh[2 * u], vh[2 * u + 1]);
+          for (int u = 0; u < 4; ++u) {
+            const int r = (u & 1 ? vb : va) + (u >> 1) * 8;
+            x[u] = *reinterpret_cast<const float4*>(vt + (q * rows + r) * 32 + ((g ^ (r & 7)) << 2));
+            if (r >= lim) x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t vh[2], vl[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+              split2(reinterpret_cast<const float*>(&x[2 * u])[i],
+                     reinterpret_cast<const float*>(&x[2 * u + 1])[i], vh[u], vl[u]);
+            mma16816(acc[4 * q + i], ph, vh[0], vh[1]);
+            mma16816(acc[4 * q + i], ph, vl[0], vl[1]);
+            mma16816(acc[4 * q + i], pl, vh[0], vh[1]);
+          }
         }
       }
     }
-    __syncthreads();
-    // merge the four key quarters and the sinks
+    // the warps meet: a coefficient for each warp's row, from the common maximum and
+    // sum and the sinks, then the outputs times it, written over the keys and added
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
       if (j == 0) {
-        sMax[(rt * 4 + wk) * 16 + g + 8 * h] = m[h];
-        sSum[(rt * 4 + wk) * 16 + g + 8 * h] = l[h];
+        sMax[warp * 16 + g + 8 * h] = m[h];
+        sSum[warp * 16 + g + 8 * h] = l[h];
       }
-#pragma unroll
-      for (int i = 0; i < DP / 8; ++i)
-        *reinterpret_cast<float2*>(sO + ((rt * 4 + wk) * 16 + g + 8 * h) * DP + i * 8 + 2 * j) =
-            make_float2(o[i][2 * h], o[i][2 * h + 1]);
     }
     __syncthreads();
-    for (int e = tid; e < 16 * RT * half; e += NT) {
-      const int r = e / half, d = (e - r * half) * 2, row = r0 + r;
-      if (row >= R) continue;
-      const int q4 = (r >> 4) * 4, rr = r & 15;
-      float mm = -1e30f;
+    for (int e = tid >> 4; e < RQ; e += units) {  // a row a half warp, a lane a warp of its tile
+      const int w = (lane16 * QT + (e >> 4)), at = w * 16 + (e & 15);
+      const bool in = lane16 < kws;
+      const float mw = in ? sMax[at] : -1e30f;
+      float top = mw;
+      for (int i = lane16; i < a.n_meta; i += 16) top = fmaxf(top, a.meta[i] * kLog2e);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sMax[(q4 + w) * 16 + rr]);
-      for (int i = 0; i < a.n_meta; ++i) mm = fmaxf(mm, a.meta[i] * kLog2e);
-      float sum = 0.f, x = 0.f, y = 0.f;
+      for (int x = 1; x < 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      const float f = tc::ex2(mw - top);
+      float sum = in ? f * sSum[at] : 0.f;
+      for (int i = lane16; i < a.n_meta; i += 16) sum += tc::ex2(a.meta[i] * kLog2e - top);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float f = tc::ex2(sMax[(q4 + w) * 16 + rr] - mm);
-        const float2 v = *reinterpret_cast<const float2*>(sO + ((q4 + w) * 16 + rr) * DP + d);
-        sum += f * sSum[(q4 + w) * 16 + rr];
-        x += f * v.x;
-        y += f * v.y;
+      for (int x = 1; x < 16; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      if (in) sCof[at] = f / sum;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float f = sCof[warp * 16 + g + 8 * h];
+      float* row = sO + (warp * 16 + g + 8 * h) * LO + 8 * j;
+#pragma unroll
+      for (int q = 0; q < NG; ++q)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)  // columns 8 j + 4 u + (0 .. 3)
+          *reinterpret_cast<float4*>(row + 32 * q + 4 * u) =
+              make_float4(f * acc[4 * q][2 * h + u], f * acc[4 * q + 1][2 * h + u],
+                          f * acc[4 * q + 2][2 * h + u], f * acc[4 * q + 3][2 * h + u]);
+    }
+    __syncthreads();
+    for (int e = tid; e < RQ * (DP / 4); e += nt) {
+      const int r = e / (DP / 4), d = (e - r * (DP / 4)) * 4, row = r0 + r;
+      if (row >= R || d >= D || !live) continue;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int w = 0; w < kws; ++w) {
+        const float4 v = *reinterpret_cast<const float4*>(
+            sO + ((w * QT + (r >> 4)) * 16 + (r & 15)) * LO + d);
+        x.x += v.x;
+        x.y += v.y;
+        x.z += v.z;
+        x.w += v.w;
       }
-      for (int i = 0; i < a.n_meta; ++i) sum += tc::ex2(a.meta[i] * kLog2e - mm);
-      const float inv = 1.f / sum;
-      *reinterpret_cast<uint32_t*>(
-          a.y + ((size_t)(b * a.H + hk * rep) * T + row) * D + d) = pack_bf16(x * inv, y * inv);
+      bf16* yr = a.y + ((size_t)(b * a.H + hk * rep) * T + row) * D + d;  // D is even
+      *reinterpret_cast<uint32_t*>(yr) = pack_bf16(x.x, x.y);
+      if (d + 2 < D) *reinterpret_cast<uint32_t*>(yr + 2) = pack_bf16(x.z, x.w);
     }
   }
 }
 
-template <typename XT, int DP, int RT>
-int launch_swa_block(const SwaBlockArgs& a, int grid, cudaStream_t st) {
-  constexpr size_t smem = swa_block_smem(DP, RT);
+int ring_map(CUtensorMap* m, const float* p, const SwaBlockArgs& a, int heads) {
+  auto fn = tc::encode_tiled_fn();
+  if (!fn) {
+    set_error("lz_swa_decode_block: cuTensorMapEncodeTiled is not available");
+    return LZ_ERR_CUDA;
+  }
+  const cuuint64_t dims[3] = {(cuuint64_t)a.D, (cuuint64_t)a.W, (cuuint64_t)heads};
+  const cuuint64_t strides[2] = {(cuuint64_t)a.D * 4, (cuuint64_t)a.W * a.D * 4};
+  const cuuint32_t box[3] = {32, (cuuint32_t)a.part, 1}, es[3] = {1, 1, 1};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float*>(p), dims,
+                        strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("lz_swa_decode_block: the tensor map of a ring could not be encoded, driver code " +
+              std::to_string((int)r));
+    return LZ_ERR_CUDA;
+  }
+  return LZ_OK;
+}
+
+template <typename XT, int DP, int QT, int N>
+int launch_swa_block(SwaBlockArgs& a, int grid, cudaStream_t st) {
+  // the ring in shared memory, in parts of 64 KB of keys and values at most
+  a.part = std::min((a.W + 15) & ~15, 64 * 1024 / (DP * 8));
+  const int tiles = a.part / 16 + ((a.T + 15) >> 4);
+  // as many warps as there are 16-key tiles for each row tile, in as few equal turns
+  // as fit
+  const int most_w = kWarps / QT, turns = ceil_div(tiles, most_w);
+  const int warps = QT * std::max(ceil_div(tiles, turns), 4 / QT);
+  const size_t smem = swa_smem(DP, QT, a.part, a.T, warps).total;
+  a.tma = a.D % 4 == 0 && aligned16(a.kr) && aligned16(a.vr);
+  CUtensorMap tk = {}, tv = {};
+  if (a.tma && a.T) {
+    int rc = ring_map(&tk, a.kr, a, grid);
+    if (!rc) rc = ring_map(&tv, a.vr, a, grid);
+    if (rc) return rc;
+  }
   static bool done[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
-  if (smem > 48 * 1024 && dev < 64 && !done[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(swa_block_kernel<XT, DP, RT>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (dev < 64 && !done[dev]) {
+    const int most = swa_smem(DP, QT, 64 * 1024 / (DP * 8), kMaxBlock, kWarps).total;
+    cudaError_t e = cudaFuncSetAttribute(swa_block_kernel<XT, DP, QT, N>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e != cudaSuccess) {
       set_error(std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
       return LZ_ERR_CUDA;
     }
     done[dev] = true;
   }
-  swa_block_kernel<XT, DP, RT><<<grid, 128 * RT, smem, st>>>(a);
+  swa_block_kernel<XT, DP, QT, N>
+      <<<dim3(grid / a.Hkv, a.Hkv), 32 * warps, smem, st>>>(tk, tv, a);
   count_launches(1);
   return check_launch("swa_block_kernel");
 }
 
 template <typename XT>
-int pick_swa_block(const SwaBlockArgs& a, int grid, cudaStream_t st) {
-  const bool one = a.H / a.Hkv * a.T <= 16;
-#define LZ_SB(DP_) \
-  return one ? launch_swa_block<XT, DP_, 1>(a, grid, st) : launch_swa_block<XT, DP_, 2>(a, grid, st)
+int pick_swa_block(SwaBlockArgs& a, bool pairs, int grid, cudaStream_t st) {
+  const bool one = a.rep * a.T <= 16;
+#define LZ_SB(DP_)                                                  \
+  return !pairs ? launch_swa_block<XT, DP_, 1, 1>(a, grid, st)      \
+         : one  ? launch_swa_block<XT, DP_, 1, 2>(a, grid, st)      \
+                : launch_swa_block<XT, DP_, 2, 2>(a, grid, st)
   if (a.D <= 32) LZ_SB(32);
   if (a.D <= 64) LZ_SB(64);
   if (a.D <= 128) LZ_SB(128);
@@ -359,6 +603,8 @@ int pick_swa_block(const SwaBlockArgs& a, int grid, cudaStream_t st) {
 }
 
 }  // namespace
+int swa_block_timeout_flag(unsigned int* out) { return tc::read_timeout_flag_here(out); }
+int swa_block_timeout_clear() { return tc::clear_timeout_flag_here(); }
 }  // namespace lz
 
 extern "C" int lz_swa_decode_block(const void* q, const void* k, const void* v, int x_dtype,
@@ -381,7 +627,7 @@ extern "C" int lz_swa_decode_block(const void* q, const void* k, const void* v, 
              "a block holds at most 64 tokens");
   LZ_REQUIRE(D <= 256 && window <= kMaxWindow, LZ_ERR_UNSUPPORTED,
              "decode supports D <= 256 and windows up to 1024");
-  LZ_REQUIRE((long long)B * Hkv < (1ll << 31) && (long long)H / Hkv * T < (1ll << 30),
+  LZ_REQUIRE((long long)B * Hkv < (1ll << 31) && Hkv <= 65535 && (long long)H / Hkv * T < (1ll << 24),
              LZ_ERR_UNSUPPORTED, "too many heads");
   LZ_REQUIRE(n_meta >= 0 && n_meta <= 32 && (n_meta == 0 || meta), LZ_ERR_INVALID_ARGUMENT,
              "meta must hold n_meta (<= 32) values");
@@ -421,7 +667,22 @@ extern "C" int lz_swa_decode_block(const void* q, const void* k, const void* v, 
   a.Hkv = Hkv;
   a.W = window;
   a.D = D;
+  a.rep = H / Hkv;
+  // two columns at a time: even strides and halves, bases on two elements
+  const size_t xs = 2 * (x_dtype == LZ_DTYPE_BF16 ? 2 : 4), cs2 = 2 * (cb ? 2 : 4);
+  const auto even = [](const Heads& h, size_t to) {
+    return reinterpret_cast<uintptr_t>(h.p) % to == 0 && ((h.sb | h.sh | h.st) & 1) == 0;
+  };
+  const auto even_r = [&](const Rotary& r) {
+    return (reinterpret_cast<uintptr_t>(r.cos) | reinterpret_cast<uintptr_t>(r.sin)) % cs2 == 0 &&
+           (r.sb & 1) == 0;
+  };
+  const bool pairs =
+      D % 4 == 0 &&
+            ((reinterpret_cast<uintptr_t>(k_ring) | reinterpret_cast<uintptr_t>(v_ring)) & 7) == 0 &&
+            even(a.q, xs) && even(a.k, xs) && even(a.v, xs) && even(a.kp, xs) &&
+            even(a.vp, xs) && even_r(a.rot) && even_r(a.rot_p);
   auto st = static_cast<cudaStream_t>(stream);
-  return x_dtype == LZ_DTYPE_F32 ? pick_swa_block<float>(a, B * Hkv, st)
-                                 : pick_swa_block<bf16>(a, B * Hkv, st);
+  return x_dtype == LZ_DTYPE_F32 ? pick_swa_block<float>(a, pairs, B * Hkv, st)
+                                 : pick_swa_block<bf16>(a, pairs, B * Hkv, st);
 }
