@@ -205,7 +205,36 @@ def longlongs(n):
 
 
 def stream_of(t):
-    return torch.cuda.current_stream(t.device).cuda_stream
+    """The current stream of t's device as an address (without building a Stream object,
+    which costs more than a small launch)."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def call(index, fn, *args):
+    """fn(*args) with device `index` current."""
+    if index == torch._C._cuda_getDevice():
+        return fn(*args)
+    with torch.cuda.device(index):
+        return fn(*args)
+
+
+def same_device(first, *rest):
+    """Whether every tensor is on the CUDA device of the first (require_cuda names the one
+    that is not)."""
+    i = first.get_device()
+    if i < 0:
+        return False
+    for t in rest:
+        if t.get_device() != i:
+            return False
+    return True
+
+
+def as_dtype(t, dtype):
+    """t contiguous in dtype; t itself when it is that already."""
+    if t.dtype is not dtype:
+        t = t.to(dtype)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def on_device(device):

@@ -134,11 +134,11 @@ def swa_decode(q, k, v, cos, sin, meta, k_ring, v_ring, pos):
 MAX_BLOCK = 64  # tokens a block
 
 
-def _pending_count(count, B, device):
+def _pending_count(count, B, index):
     if count is None:
         return None
-    if count.dtype != torch.int32 or tuple(count.shape) != (B,) or count.device != device:
-        raise ValueError(f"count must be int32 [{B}] on {device}, got {count.dtype} "
+    if count.dtype is not torch.int32 or count.shape != (B,) or count.get_device() != index:
+        raise ValueError(f"count must be int32 [{B}] on device {index}, got {count.dtype} "
                          f"{tuple(count.shape)} on {count.device}")
     return count.contiguous()
 
@@ -152,64 +152,72 @@ def gla_decode_block(fq, fk, v, log_gamma, state, zstate, pending=None):
     which first advances state and zstate (fp32 [B, Hs, F, D] and [B, Hs, F], in
     place) by the first count[b] (int32 [B], None = all) of its tokens.
     T = 0 (empty fq, fk, v, log_gamma) only advances the state."""
-    _lib.require_cuda(fq, fk, v, log_gamma, state, zstate)
-    if fq.dim() != 4 or fk.dim() != 4 or v.dim() != 4:
-        raise ValueError("fq, fk and v must be [B, heads, T, dim]")
+    given = (fq, fk, v, log_gamma, state, zstate)
+    if not _lib.same_device(*given):
+        _lib.require_cuda(*given)
+    if fq.dim() != 4 or fk.dim() != 4 or v.dim() != 4 or state.dim() != 4:
+        raise ValueError("fq, fk, v must be [B, heads, T, dim] and state [B, Hs, F, D]")
     B, H, T, F = fq.shape
-    Hkv, D = fk.shape[1], v.shape[-1]
-    if tuple(fk.shape) != (B, Hkv, T, F) or tuple(v.shape) != (B, Hkv, T, D):
+    Hkv, D, Hs, index = fk.shape[1], v.shape[3], state.shape[1], fq.get_device()
+    if fk.shape != (B, Hkv, T, F) or v.shape != (B, Hkv, T, D):
         raise ValueError(f"fk and v must be [B, Hkv, T, F] and [B, Hkv, T, D] matching fq "
                          f"{tuple(fq.shape)}, got {tuple(fk.shape)}, {tuple(v.shape)}")
-    Hs = state.shape[1]
-    if (state.dtype != torch.float32 or zstate.dtype != torch.float32
+    if (state.dtype is not torch.float32 or zstate.dtype is not torch.float32
             or not state.is_contiguous() or not zstate.is_contiguous()):
         raise ValueError("state and zstate must be contiguous fp32 tensors")
-    if tuple(state.shape) != (B, Hs, F, D) or tuple(zstate.shape) != (B, Hs, F):
+    if state.shape != (B, Hs, F, D) or zstate.shape != (B, Hs, F):
         raise ValueError(f"state must be [B, Hs, F, D] and zstate [B, Hs, F], got "
                          f"{tuple(state.shape)}, {tuple(zstate.shape)}")
-    per_head = {(B, T): 0, (B, H, T): 1}.get(tuple(log_gamma.shape))
-    if per_head is None:
+    per_head = 1 if log_gamma.dim() == 3 else 0
+    if log_gamma.shape != ((B, H, T) if per_head else (B, T)):
         raise ValueError(f"log_gamma must be [B, T] or [B, H, T], got {tuple(log_gamma.shape)}")
     fkp = vp = lgp = count = None
     Tp = 0
     if pending is not None:
         fkp, vp, lgp, count = pending
-        _lib.require_cuda(fq, fkp, vp, lgp)
+        if not _lib.same_device(fq, fkp, vp, lgp):
+            _lib.require_cuda(fq, fkp, vp, lgp)
         Tp = fkp.shape[2]
-        if tuple(fkp.shape) != (B, Hkv, Tp, F) or tuple(vp.shape) != (B, Hkv, Tp, D):
+        if fkp.shape != (B, Hkv, Tp, F) or vp.shape != (B, Hkv, Tp, D):
             raise ValueError(f"pending fk and v must be [B, Hkv, T, F] and [B, Hkv, T, D], got "
                              f"{tuple(fkp.shape)}, {tuple(vp.shape)}")
-        if tuple(lgp.shape) != ((B, H, Tp) if per_head else (B, Tp)):
+        if lgp.shape != ((B, H, Tp) if per_head else (B, Tp)):
             raise ValueError(f"pending log_gamma must have log_gamma's layout, got "
                              f"{tuple(lgp.shape)}")
-        count = _pending_count(count, B, fq.device)
-        fkp, vp = fkp.to(torch.bfloat16).contiguous(), vp.to(torch.bfloat16).contiguous()
-        lgp = lgp.float().contiguous()
-    y = torch.empty(B, H, T, D, device=fq.device, dtype=torch.bfloat16)
-    if T == 0 and Tp == 0:
+        count = _pending_count(count, B, index)
+        fkp, vp = _lib.as_dtype(fkp, torch.bfloat16), _lib.as_dtype(vp, torch.bfloat16)
+        lgp = _lib.as_dtype(lgp, torch.float32)
+    y = torch.empty((B, H, T, D), device=fq.device, dtype=torch.bfloat16)
+    if B == 0 or T == 0 and Tp == 0:
         return y
-    lib = _lib.load()
-    fq16, fk16, v16 = (t.to(torch.bfloat16).contiguous() for t in (fq, fk, v))
-    lg = log_gamma.float().contiguous()
-    with _lib.on_device(fq.device):
-        rc = lib.lz_gla_decode_block(
-            _lib.ptr(fq16), _lib.ptr(fk16), _lib.ptr(v16), _lib.ptr(lg), per_head, _lib.ptr(fkp),
-            _lib.ptr(vp), _lib.ptr(lgp), _lib.ptr(count), _lib.ptr(state), _lib.ptr(zstate),
-            _lib.ptr(y), B, H, Hkv, Hs, T, Tp, F, D, _lib.stream_of(fq))
-    _lib.check(rc, "gla decode block")
+    fq, fk, v = (_lib.as_dtype(t, torch.bfloat16) for t in (fq, fk, v))
+    lg = _lib.as_dtype(log_gamma, torch.float32)
+    rc = _lib.call(
+        index, _lib.load().lz_gla_decode_block, fq.data_ptr(), fk.data_ptr(), v.data_ptr(),
+        lg.data_ptr(), per_head, _lib.ptr(fkp), _lib.ptr(vp), _lib.ptr(lgp), _lib.ptr(count),
+        state.data_ptr(), zstate.data_ptr(), y.data_ptr(), B, H, Hkv, Hs, T, Tp, F, D,
+        _lib.stream_of(fq))
+    if rc:
+        _lib.check(rc, "gla decode block")
     return y
 
 
-def _tables(cos, sin, B, T, D):
-    """cos / sin as contiguous [B or 1, T, D] of one supported type, and the batch stride."""
-    if cos.dtype != sin.dtype or cos.dtype not in _DT:
-        cos, sin = cos.float(), sin.float()
-    for t in (cos, sin):
-        if t.dim() != 3 or tuple(t.shape[1:]) != (T, D) or t.shape[0] not in (1, B):
-            raise ValueError(f"cos and sin must be [{B} or 1, {T}, {D}], got {tuple(t.shape)}")
-    if cos.shape[0] != sin.shape[0]:
-        cos, sin = cos.expand(B, T, D), sin.expand(B, T, D)
-    return cos.contiguous(), sin.contiguous(), T * D if cos.shape[0] > 1 else 0
+def _tables(cos, sin, dtype, B, T, D):
+    """cos / sin as contiguous [B or 1, T, D] of dtype, and the batch stride."""
+    n = cos.shape[0]
+    if cos.shape != (n, T, D) or sin.shape != (n, T, D) or n != B and n != 1:
+        for t in (cos, sin):
+            if t.dim() != 3 or t.shape[1:] != (T, D) or t.shape[0] not in (1, B):
+                raise ValueError(f"cos and sin must be [{B} or 1, {T}, {D}], got {tuple(t.shape)}")
+        cos, sin, n = cos.expand(B, T, D), sin.expand(B, T, D), B
+    return _lib.as_dtype(cos, dtype), _lib.as_dtype(sin, dtype), T * D if n > 1 else 0
+
+
+def _rows(t, dtype):
+    """t in dtype with a contiguous last dimension, in place where it has one."""
+    if t.dtype is not dtype:
+        t = t.to(dtype)
+    return t if t.stride(3) == 1 else t.contiguous()
 
 
 def swa_decode_block(q, k, v, cos, sin, meta, k_ring, v_ring, pos, pending=None):
@@ -223,60 +231,56 @@ def swa_decode_block(q, k, v, cos, sin, meta, k_ring, v_ring, pos, pending=None)
     [B], None = all) of its tokens to slots (pos[b] + t) % W. pos counts the
     tokens the rings hold before the call, without the pending ones; the caller
     then advances it by count. T = 0 only advances the rings."""
-    _lib.require_cuda(q, k, v, cos, sin, meta, k_ring, v_ring, pos)
-    if q.dim() != 4 or k.dim() != 4:
-        raise ValueError("q, k and v must be [B, heads, T, D]")
+    given = (q, k, v, cos, sin, meta, k_ring, v_ring, pos)
+    if not _lib.same_device(*given):
+        _lib.require_cuda(*given)
+    if q.dim() != 4 or k.dim() != 4 or k_ring.dim() != 4:
+        raise ValueError("q, k, v must be [B, heads, T, D] and the rings [B, Hkv, W, D]")
     B, H, T, D = q.shape
-    Hkv, W = k.shape[1], k_ring.shape[2]
-    if tuple(k.shape) != (B, Hkv, T, D) or v.shape != k.shape:
+    Hkv, W, index = k.shape[1], k_ring.shape[2], q.get_device()
+    if k.shape != (B, Hkv, T, D) or v.shape != k.shape:
         raise ValueError(f"k and v must be [B, Hkv, T, D] matching q {tuple(q.shape)}, got "
                          f"{tuple(k.shape)}, {tuple(v.shape)}")
     for ring in (k_ring, v_ring):
-        if (tuple(ring.shape) != (B, Hkv, W, D) or ring.dtype != torch.float32
+        if (ring.shape != (B, Hkv, W, D) or ring.dtype is not torch.float32
                 or not ring.is_contiguous()):
             raise ValueError(f"the rings must be contiguous fp32 [B, Hkv, W, D], got "
                              f"{ring.dtype} {tuple(ring.shape)}")
-    if pos.dtype != torch.int32 or tuple(pos.shape) != (B,):
+    if pos.dtype is not torch.int32 or pos.shape != (B,):
         raise ValueError("pos must be int32 [B]")
-    kp = vp = cp = sp = count = None
-    Tp = 0
+    xdt = q.dtype if q.dtype in _DT else torch.float32
+    cdt = cos.dtype if cos.dtype is sin.dtype and cos.dtype in _DT else torch.float32
+    kp = vp = cp = sp = count = stp = None
+    Tp = cp_sb = 0
     if pending is not None:
         kp, vp, cp, sp, count = pending
-        _lib.require_cuda(q, kp, vp, cp, sp)
+        if not _lib.same_device(q, kp, vp, cp, sp):
+            _lib.require_cuda(q, kp, vp, cp, sp)
         Tp = kp.shape[2]
-        if tuple(kp.shape) != (B, Hkv, Tp, D) or vp.shape != kp.shape:
+        if kp.shape != (B, Hkv, Tp, D) or vp.shape != kp.shape:
             raise ValueError(f"pending k and v must be [B, Hkv, T, D], got {tuple(kp.shape)}, "
                              f"{tuple(vp.shape)}")
-        count = _pending_count(count, B, q.device)
-    y = torch.empty(B, H, T, D, device=q.device, dtype=torch.bfloat16)
-    if T == 0 and Tp == 0:
+        count = _pending_count(count, B, index)
+        if Tp:
+            cp, sp, cp_sb = _tables(cp, sp, cdt, B, Tp, D)
+            kp, vp = _rows(kp, xdt), _rows(vp, xdt)
+            stp = _lib.longlongs(6)(*kp.stride()[:3], *vp.stride()[:3])
+    y = torch.empty((B, H, T, D), device=q.device, dtype=torch.bfloat16)
+    if B == 0 or T == 0 and Tp == 0:
         return y
-    xdt = q.dtype if q.dtype in _DT else torch.float32
-
-    def rows(t):
-        return t if t.dtype == xdt and t.stride(-1) == 1 else t.to(xdt).contiguous()
-
-    cos, sin, cs_sb = _tables(cos, sin, B, T, D)
-    q, k, v = rows(q), rows(k), rows(v)
-    st = (_lib.longlongs(9))(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
-    stp, cp_sb = None, 0
-    if Tp:
-        if cp.dtype != cos.dtype or sp.dtype != cos.dtype:
-            cp, sp = cp.to(cos.dtype), sp.to(cos.dtype)
-        cp, sp, cp_sb = _tables(cp, sp, B, Tp, D)
-        kp, vp = rows(kp), rows(vp)
-        stp = (_lib.longlongs(6))(*kp.stride()[:3], *vp.stride()[:3])
-    meta32 = meta.float().contiguous()
-    lib = _lib.load()
-    with _lib.on_device(q.device):
-        rc = lib.lz_swa_decode_block(
-            _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _DT[xdt], st, _lib.ptr(cos), _lib.ptr(sin),
-            _DT[cos.dtype], cs_sb, _lib.ptr(kp) if Tp else None, _lib.ptr(vp) if Tp else None, stp,
-            _lib.ptr(cp) if Tp else None, _lib.ptr(sp) if Tp else None, cp_sb, _lib.ptr(count),
-            _lib.ptr(k_ring), _lib.ptr(v_ring), _lib.ptr(pos.contiguous()),
-            _lib.ptr(meta32) if meta32.numel() else None, meta32.numel(), _lib.ptr(y), B, H, Hkv,
-            T, Tp, W, D, _lib.stream_of(q))
-    _lib.check(rc, "swa decode block")
+    cos, sin, cs_sb = _tables(cos, sin, cdt, B, T, D)
+    q, k, v = _rows(q, xdt), _rows(k, xdt), _rows(v, xdt)
+    st = _lib.longlongs(9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+    meta32, pos = _lib.as_dtype(meta, torch.float32), pos.contiguous()
+    p = _lib.ptr if Tp else (lambda t: None)
+    rc = _lib.call(
+        index, _lib.load().lz_swa_decode_block, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+        _DT[xdt], st, cos.data_ptr(), sin.data_ptr(), _DT[cdt], cs_sb, p(kp), p(vp), stp, p(cp),
+        p(sp), cp_sb, _lib.ptr(count), k_ring.data_ptr(), v_ring.data_ptr(), pos.data_ptr(),
+        meta32.data_ptr() or None, meta32.numel(), y.data_ptr(), B, H, Hkv, T, Tp, W, D,
+        _lib.stream_of(q))
+    if rc:
+        _lib.check(rc, "swa decode block")
     return y
 
 

@@ -22,14 +22,19 @@ _DT = {torch.float32: _lib.LZ_DTYPE_F32, torch.bfloat16: _lib.LZ_DTYPE_BF16}
 
 def _rows(t):
     """t [..., K] as rows [M, K] with a contiguous last dimension (a view where it can be)."""
-    t = t.unsqueeze(0) if t.dim() == 1 else t.flatten(0, -2)
-    if t.stride(-1) != 1 and t.shape[-1] > 1 or t.stride(0) < t.shape[-1] and t.shape[0] > 1:
+    if t.dim() != 2:
+        t = t.unsqueeze(0) if t.dim() == 1 else t.flatten(0, -2)
+    if t.is_contiguous():
+        return t
+    if t.stride(1) != 1 and t.shape[1] > 1 or t.stride(0) < t.shape[1] and t.shape[0] > 1:
         t = t.contiguous()
     return t
 
 
 def _no_grad(*tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if not torch.is_grad_enabled():
+        return
+    if any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError("8-bit products have no backward; call them under torch.no_grad()")
 
 
@@ -55,17 +60,16 @@ def int8_quantize(x):
     return codes.view(*lead, codes.shape[1])[..., :K], scale.view(lead)
 
 
-def _output(x, M, N, K, b, b_scale, bias, dtype):
-    if b.dim() != 2 or b.dtype != torch.int8 or b.shape[1] != K or N < 1 or K < 1:
+def _check(K, N, b, b_scale, bias, dtype):
+    if b.dim() != 2 or b.dtype is not torch.int8 or b.shape[1] != K or N < 1 or K < 1:
         raise ValueError(f"the weight codes must be int8 [N, {K}], got {b.dtype} {tuple(b.shape)}")
-    if b_scale.dtype != torch.float32 or tuple(b_scale.shape) != (N,):
+    if b_scale.dtype is not torch.float32 or b_scale.shape != (N,):
         raise ValueError(f"the weight's scale must be fp32 [{N}], got {b_scale.dtype} "
                          f"{tuple(b_scale.shape)}")
-    if bias is not None and (tuple(bias.shape) != (N,) or bias.dtype not in _DT):
+    if bias is not None and (bias.shape != (N,) or bias.dtype not in _DT):
         raise ValueError(f"bias must be fp32 or bf16 [{N}], got {bias.dtype} {tuple(bias.shape)}")
     if dtype not in _DT:
         raise ValueError(f"the output type must be float32 or bfloat16, got {dtype}")
-    return torch.empty(M, N, device=x.device, dtype=dtype)
 
 
 def _aligned(t):
@@ -75,18 +79,20 @@ def _aligned(t):
 def int8_matmul(a, a_scale, b, b_scale, bias=None, dtype=torch.bfloat16):
     """y [..., N] = (a b^T) * a_scale * b_scale + bias for codes a int8 [..., K],
     b int8 [N, K] and scales fp32 [...] and [N], in `dtype` (bf16 or fp32)."""
-    _lib.require_cuda(a, a_scale, b, b_scale, *(() if bias is None else (bias,)))
+    given = (a, a_scale, b, b_scale) if bias is None else (a, a_scale, b, b_scale, bias)
+    if not _lib.same_device(*given):
+        _lib.require_cuda(*given)
     _no_grad(a_scale, b_scale, bias)
-    if a.dim() < 1 or a.dtype != torch.int8:
+    if a.dim() < 1 or a.dtype is not torch.int8:
         raise ValueError(f"a must be int8 [..., K], got {a.dtype} {tuple(a.shape)}")
-    lead, K = a.shape[:-1], a.shape[-1]
-    if a_scale.dtype != torch.float32 or a_scale.shape != lead:
+    lead, K, N = a.shape[:-1], a.shape[-1], b.shape[0]
+    if a_scale.dtype is not torch.float32 or a_scale.shape != lead:
         raise ValueError(f"a's scale must be fp32 {tuple(lead)}, got {a_scale.dtype} "
                          f"{tuple(a_scale.shape)}")
-    N = b.shape[0]
+    _check(K, N, b, b_scale, bias, dtype)
+    y = torch.empty((*lead, N), device=a.device, dtype=dtype)
     ar = _rows(a)
     M = ar.shape[0]
-    y = _output(a, M, N, K, b, b_scale, bias, dtype)
     if M:
         br = _rows(b)
         sa, sb = a_scale.contiguous(), b_scale.contiguous()
@@ -95,43 +101,49 @@ def int8_matmul(a, a_scale, b, b_scale, bias=None, dtype=torch.bfloat16):
         if not (_aligned(ar) and _aligned(br)):
             ws = torch.empty(_lib.size_query("lz_int8_workspace_bytes", M, N, K), device=a.device,
                              dtype=torch.uint8)
-        with _lib.on_device(a.device):
-            rc = _lib.load().lz_int8_matmul(
-                _lib.ptr(ar), ar.stride(0), _lib.ptr(sa), _lib.ptr(br), br.stride(0),
-                _lib.ptr(sb), _lib.ptr(bias), 0 if bias is None else _DT[bias.dtype], _lib.ptr(y),
-                _DT[dtype], _lib.ptr(ws), 0 if ws is None else ws.numel(), M, N, K,
-                _lib.stream_of(a))
-        _lib.check(rc, "int8 matmul")
-    return y.view(*lead, N)
+        rc = _lib.call(
+            a.get_device(), _lib.load().lz_int8_matmul, ar.data_ptr(), ar.stride(0),
+            sa.data_ptr(), br.data_ptr(), br.stride(0), sb.data_ptr(), _lib.ptr(bias),
+            0 if bias is None else _DT[bias.dtype], y.data_ptr(), _DT[dtype], _lib.ptr(ws),
+            0 if ws is None else ws.numel(), M, N, K, _lib.stream_of(a))
+        if rc:
+            _lib.check(rc, "int8 matmul")
+    return y
 
 
 def int8_linear(x, weight, weight_scale, bias=None, dtype=None):
     """y [..., N] = x W^T + bias with x [..., K] (fp32 or bf16) quantised row by
     row and the weight given as codes int8 [N, K] with a scale fp32 [N] for each
     channel (int8_quantize of an nn.Linear weight), in `dtype` (x's by default)."""
-    _lib.require_cuda(x, weight, weight_scale, *(() if bias is None else (bias,)))
+    given = (x, weight, weight_scale) if bias is None else (x, weight, weight_scale, bias)
+    if not _lib.same_device(*given):
+        _lib.require_cuda(*given)
     _no_grad(x, weight_scale, bias)
     if x.dim() < 1:
         raise ValueError(f"x must be [..., K], got {tuple(x.shape)}")
+    if x.dtype not in _DT:
+        x = x.float()
     lead, K, N = x.shape[:-1], x.shape[-1], weight.shape[0]
-    xr = _rows(x if x.dtype in _DT else x.float())
-    M = xr.shape[0]
     if dtype is None:
-        dtype = xr.dtype
-    y = _output(x, M, N, K, weight, weight_scale, bias, dtype)
+        dtype = x.dtype
+    _check(K, N, weight, weight_scale, bias, dtype)
+    y = torch.empty((*lead, N), device=x.device, dtype=dtype)
+    xr = _rows(x)
+    M = xr.shape[0]
     if M:
         w, ws = _rows(weight), weight_scale.contiguous()
         bias = None if bias is None else bias.contiguous()
         size = (_lib.size_query("lz_int8_linear_workspace_bytes", M, K) if _aligned(w)
                 else _lib.size_query("lz_int8_workspace_bytes", M, N, K))
         work = torch.empty(size, device=x.device, dtype=torch.uint8)
-        with _lib.on_device(x.device):
-            rc = _lib.load().lz_int8_linear(
-                _lib.ptr(xr), _DT[xr.dtype], xr.stride(0), _lib.ptr(w), w.stride(0), _lib.ptr(ws),
-                _lib.ptr(bias), 0 if bias is None else _DT[bias.dtype], _lib.ptr(y), _DT[dtype],
-                _lib.ptr(work), size, M, N, K, _lib.stream_of(x))
-        _lib.check(rc, "int8 linear")
-    return y.view(*lead, N)
+        rc = _lib.call(
+            x.get_device(), _lib.load().lz_int8_linear, xr.data_ptr(), _DT[xr.dtype],
+            xr.stride(0), w.data_ptr(), w.stride(0), ws.data_ptr(), _lib.ptr(bias),
+            0 if bias is None else _DT[bias.dtype], y.data_ptr(), _DT[dtype], work.data_ptr(),
+            size, M, N, K, _lib.stream_of(x))
+        if rc:
+            _lib.check(rc, "int8 linear")
+    return y
 
 
 class Int8Linear(nn.Module):
