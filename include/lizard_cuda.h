@@ -587,6 +587,11 @@ int lz_int8_matmul(const void* a, long long a_ld, const float* a_scale,
                    const void* bias, int bias_dtype, void* y, int y_dtype,
                    void* workspace, size_t workspace_bytes, int M, int N, int K, void* stream);
 
+/* Kernel of the 8-bit products: 0 = chosen by size (default), 1 = the one for few
+ * tokens, 2 = the one for many. Results are identical. Returns the previous
+ * setting, or -LZ_ERR_INVALID_ARGUMENT. A hook for tests and tuning, process-wide. */
+int lz_int8_set_path(int path);
+
 /* lz_int8_quantize of x and lz_int8_matmul with the weight codes w [N, K] in
  * one call. Workspace: lz_int8_linear_workspace_bytes(M, K) when rows of w start
  * on 16-byte boundaries, else lz_int8_workspace_bytes(M, N, K). */

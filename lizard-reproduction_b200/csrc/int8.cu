@@ -13,14 +13,16 @@
 // both sides, as activations and nn.Linear weights lie). Two kernels:
 //   narrow: few tokens. The weights stream once, so the kernel is bound by
 //     memory; weight rows take the 128 accumulator lanes (they are the long
-//     side) and 16 .. 128 tokens the columns. Where the tiles of N do not fill
-//     the machine, a cluster of 2 .. 8 CTAs splits K and adds its integer
-//     partials through distributed shared memory.
+//     side) and 16 .. 128 tokens the columns. Two persistent CTAs an SM walk the
+//     tiles, the next one's operands loading under this one's epilogue. Where the
+//     tiles do not fill the machine, a cluster of 2 .. 8 CTAs splits K and adds its
+//     integer partials through distributed shared memory.
 //   wide: many tokens. Bound by the tensor cores. A pair of CTAs (cta_group::2)
 //     shares a 256 x 256 tile: each loads half of either operand, so a byte in
 //     shared memory feeds twice the math; two accumulators of 256 TMEM columns
 //     let the epilogue of a tile run under the next one's products.
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 #include "tc.cuh"
@@ -30,9 +32,12 @@ namespace {
 
 constexpr int kMaxK = 131071;  // 128 * 128 * K < 2^31
 
+__device__ __forceinline__ void launch_dependents() {
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+}
+
 // ------------------------------------------------------------------ quantise
-constexpr int kQT = 256;   // threads a row
-constexpr int kQV = 4;     // 16-byte vectors a thread keeps
+constexpr int kQT = 256;   // threads a CTA
 
 template <typename T>
 struct Vec;
@@ -75,58 +80,64 @@ __device__ __forceinline__ void store_codes(int8_t* p, const uint4& w, float inv
                        code_of(bf16_lo(w.w), inv), code_of(bf16_hi(w.w), inv)));
 }
 
-// One CTA a row: the row is read once into registers (the part beyond kQT * kQV
-// vectors, and rows that do not start on 16 bytes, twice). The largest |x| is
-// taken on the bits, where infinities and NaN are larger than every number: such
-// a row gets the scale NaN, and so NaN outputs.
-template <typename T>
+// ROW threads a row (a warp for short rows, the CTA for long ones): the row is read
+// once into registers, KEEP 16-byte vectors a thread (the part beyond, and rows that
+// do not start on 16 bytes, twice). The largest |x| is taken on the bits, where
+// infinities and NaN are larger than every number: such a row gets the scale NaN, and
+// so NaN outputs. Bound by memory: 32768 rows of 8192 bf16 in 117 us, 6.9 TB/s.
+template <typename T, int ROW, int KEEP>
 __global__ void __launch_bounds__(kQT)
 i8_quantize_kernel(const T* __restrict__ x, long long ldx, int8_t* __restrict__ codes,
-                   long long ldc, float* __restrict__ scale, int K) {
+                   long long ldc, float* __restrict__ scale, int M, int K) {
   using V = Vec<T>;
   __shared__ uint32_t sTop[kQT / 32];
-  const int tid = threadIdx.x;
-  const T* row = x + (size_t)blockIdx.x * ldx;
-  int8_t* out = codes + (size_t)blockIdx.x * ldc;
+  launch_dependents();  // the product's CTAs may start on the weights
+  const int tid = threadIdx.x % ROW;
+  const long long m = (long long)blockIdx.x * (kQT / ROW) + threadIdx.x / ROW;
+  if (m >= M) return;  // whole warps
+  const T* row = x + m * ldx;
+  int8_t* out = codes + m * ldc;
   const bool vec = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
   const int nv = vec ? K / V::N : 0;
   const uint4* rv = reinterpret_cast<const uint4*>(row);
-  uint4 keep[kQV];
+  uint4 keep[KEEP];
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < kQV; ++i) {
-    const int at = tid + i * kQT;
-    keep[i] = at < nv ? rv[at] : make_uint4(0, 0, 0, 0);
+  for (int i = 0; i < KEEP; ++i) {
+    const int at = tid + i * ROW;
+    keep[i] = at < nv ? __ldg(rv + at) : make_uint4(0, 0, 0, 0);
   }
 #pragma unroll
-  for (int i = 0; i < kQV; ++i) top = max(top, V::top(keep[i]));
-  for (int at = tid + kQV * kQT; at < nv; at += kQT) top = max(top, V::top(rv[at]));
-  for (int k = nv * V::N + tid; k < K; k += kQT)
+  for (int i = 0; i < KEEP; ++i) top = max(top, V::top(keep[i]));
+  for (int at = tid + KEEP * ROW; at < nv; at += ROW) top = max(top, V::top(rv[at]));
+  for (int k = nv * V::N + tid; k < K; k += ROW)
     top = max(top, __float_as_uint(V::value(row + k)) & 0x7fffffffu);
   top = __reduce_max_sync(0xffffffffu, top);
-  if ((tid & 31) == 0) sTop[tid >> 5] = top;
-  __syncthreads();
+  if constexpr (ROW == kQT) {
+    if ((tid & 31) == 0) sTop[tid >> 5] = top;
+    __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kQT / 32; ++w) top = max(top, sTop[w]);
+    for (int w = 0; w < kQT / 32; ++w) top = max(top, sTop[w]);
+  }
   const float t = __uint_as_float(top);
   // below 4e-37 the reciprocal leaves the fp32 range: the row counts as zero
   const bool live = t >= 4e-37f && t < INFINITY;
   const float inv = live ? 127.f / t : 0.f;
-  if (tid == 0)
-    scale[blockIdx.x] = live ? t / 127.f : (t < 1.f ? 0.f : __uint_as_float(0x7fc00000u));
+  if (tid == 0) scale[m] = live ? t / 127.f : (t < 1.f ? 0.f : __uint_as_float(0x7fc00000u));
   if (!live) {
-    for (int k = tid; k < ldc; k += kQT) out[k] = 0;
+    for (int k = tid; k < ldc; k += ROW) out[k] = 0;
     return;
   }
 #pragma unroll
-  for (int i = 0; i < kQV; ++i) {
-    const int at = tid + i * kQT;
+  for (int i = 0; i < KEEP; ++i) {
+    const int at = tid + i * ROW;
     if (at < nv) store_codes(out + at * V::N, keep[i], inv, T());
   }
-  for (int at = tid + kQV * kQT; at < nv; at += kQT) store_codes(out + at * V::N, rv[at], inv, T());
-  for (int k = nv * V::N + tid; k < K; k += kQT)
+  for (int at = tid + KEEP * ROW; at < nv; at += ROW)
+    store_codes(out + at * V::N, rv[at], inv, T());
+  for (int k = nv * V::N + tid; k < K; k += ROW)
     out[k] = (int8_t)(code_of(V::value(row + k), inv) & 0xffu);
-  for (int k = K + tid; k < ldc; k += kQT) out[k] = 0;
+  for (int k = K + tid; k < ldc; k += ROW) out[k] = 0;
 }
 
 // Rows of codes that do not start on 16 bytes, copied to ones that do.
@@ -241,44 +252,57 @@ __device__ __forceinline__ float scaled(int acc, float sa, float sb, float bias)
 }
 
 // -------------------------------------------------------------------- narrow
+constexpr int kNStaging = 8192;  // bytes of y on their way out: 32 tokens x 128 channels (bf16)
 template <int BN>
 struct Narrow {
   static constexpr int kStages = BN <= 32 ? 5 : BN == 64 ? 4 : 3;
   static constexpr int kA = 128 * 128, kB = BN * 128;
-  static constexpr int kCols = BN < 32 ? 32 : BN;  // TMEM columns, a power of two >= 32
-  // operand stages (the partials of a split reuse them), barriers, TMEM address
-  static constexpr size_t kSmem = 1024 + (size_t)kStages * (kA + kB) + 256;
+  static constexpr int kCols = BN < 32 ? 32 : BN;  // TMEM columns of an accumulator
+  // operand stages (the partials of a split reuse them), staging, token scales,
+  // barriers, TMEM address; two CTAs fit an SM
+  static constexpr size_t kSmem =
+      1024 + (size_t)kStages * (kA + kB) + kNStaging + 2 * BN * 4 + 256;
   static_assert((size_t)kStages * (kA + kB) >= (size_t)BN * 128 * 4, "partials fit");
+  static_assert(kSmem <= 115712, "two CTAs an SM");
 };
 
-// Grid: (weight tiles * split, token tiles), clusters of `split` CTAs along x.
+// Warps: 0 TMA, 1 MMA (and TMEM), 2..5 epilogue. split == 1: a CTA walks the (weight
+// tile, token tile) pairs blockIdx.x, + gridDim.x, ..., weight tiles fastest. split
+// > 1: clusters of `split` CTAs, one tile each, K dealt over the cluster.
 template <int BN>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(192)
 i8_narrow_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx,
-                 const Out o, const int split) {
+                 const __grid_constant__ CUtensorMap ty, const Out o, const int split,
+                 const int ytma) {
   using P = Narrow<BN>;
   constexpr int S = P::kStages;
   extern __shared__ unsigned char raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-  uint64_t* full = reinterpret_cast<uint64_t*>(sm + (size_t)S * (P::kA + P::kB));
+  unsigned char* staging = sm + (size_t)S * (P::kA + P::kB);
+  float* sSa = reinterpret_cast<float*>(staging + kNStaging);  // [2][BN] token scales
+  uint64_t* full = reinterpret_cast<uint64_t*>(sSa + 2 * BN);
   uint64_t* empty = full + S;
-  uint64_t* done = empty + S;
-  uint32_t* tptr = reinterpret_cast<uint32_t*>(done + 1);
+  uint64_t* acc_full = empty + S;      // [2]
+  uint64_t* acc_empty = acc_full + 2;  // [2]
+  uint32_t* tptr = reinterpret_cast<uint32_t*>(acc_empty + 2);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int rank = blockIdx.x % split, n0 = blockIdx.x / split * 128, m0 = blockIdx.y * BN;
+  const int rank = split > 1 ? blockIdx.x % split : 0;
+  const int wt = (o.N + 127) >> 7, tiles = wt * ((o.M + BN - 1) / BN);
+  const int first = blockIdx.x / split, stride = gridDim.x / split;
   const int KT = (o.K + 127) >> 7;
-  const int kt0 = (int)((long long)KT * rank / split), kt1 = (int)((long long)KT * (rank + 1) / split);
-  const int nk = kt1 - kt0;
+  const int kt0 = split > 1 ? KT * rank / split : 0;
+  const int nk = (split > 1 ? KT * (rank + 1) / split : KT) - kt0;
   if (tid == 0) {
     for (int s = 0; s < S; ++s) tc::mbar_init(full + s, 1), tc::mbar_init(empty + s, 1);
-    tc::mbar_init(done, 1);
+    for (int i = 0; i < 2; ++i) tc::mbar_init(acc_full + i, 1), tc::mbar_init(acc_empty + i, 4);
     tc::fence_mbar_init();
     tc::prefetch_tmap(&tw);
     tc::prefetch_tmap(&tx);
+    tc::prefetch_tmap(&ty);
   }
   if (warp == 1) {
-    tc::tmem_alloc(tptr, P::kCols);
+    tc::tmem_alloc(tptr, 2 * P::kCols);
     tc::tmem_relinquish();
   }
   tc::tc_fence_before();
@@ -289,82 +313,137 @@ i8_narrow_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__
   if (warp == 0 && lane == 0) {
     // the weights of the first stages do not depend on the launch before (the
     // quantisation of x): they load while it ends
-    const int pre = min(nk, S);
+    const int pre = min(nk, S), n0 = first % wt * 128;
     for (int i = 0; i < pre; ++i) {
       tc::mbar_expect_tx(full + i, P::kA + P::kB);
       tma_load_2d(sm + (size_t)i * (P::kA + P::kB), &tw, (kt0 + i) * 128, n0, full + i);
     }
     grid_dependency_wait();
-    for (int i = 0; i < nk; ++i) {
-      const int s = i % S;
-      unsigned char* st = sm + (size_t)s * (P::kA + P::kB);
-      if (i >= S) {
-        tc::mbar_wait(empty + s, (i / S - 1) & 1, 120);
-        tc::mbar_expect_tx(full + s, P::kA + P::kB);
-        tma_load_2d(st, &tw, (kt0 + i) * 128, n0, full + s);
+    uint32_t it = 0;
+    for (int t = first; t < tiles; t += stride) {
+      const int n = t % wt * 128, m = t / wt * BN;
+      for (int k = 0; k < nk; ++k, ++it) {
+        const int s = it % S;
+        unsigned char* st = sm + (size_t)s * (P::kA + P::kB);
+        if (it >= (uint32_t)pre) {
+          if (it >= S) tc::mbar_wait(empty + s, (it / S - 1) & 1, 120);
+          tc::mbar_expect_tx(full + s, P::kA + P::kB);
+          tma_load_2d(st, &tw, (kt0 + k) * 128, n, full + s);
+        }
+        tma_load_2d(st + P::kA, &tx, (kt0 + k) * 128, m, full + s);
       }
-      tma_load_2d(st + P::kA, &tx, (kt0 + i) * 128, m0, full + s);
     }
   } else if (warp == 1 && lane == 0) {
     constexpr uint32_t idesc = idesc_i8(128, BN);
-    for (int i = 0; i < nk; ++i) {
-      const int s = i % S;
-      tc::mbar_wait(full + s, (i / S) & 1, 121);
+    uint32_t it = 0, at = 0;
+    for (int t = first; t < tiles; t += stride, ++at) {
+      const int buf = at & 1;
+      if (at >= 2) tc::mbar_wait(acc_empty + buf, (at / 2 - 1) & 1, 123);
       tc::tc_fence_after();
-      const uint32_t a0 = smem_u32(sm + (size_t)s * (P::kA + P::kB));
-      const uint64_t ad = tc::sdesc(a0, 0, 1024), bd = tc::sdesc(a0 + P::kA, 0, 1024);
+      for (int k = 0; k < nk; ++k, ++it) {
+        const int s = it % S;
+        tc::mbar_wait(full + s, (it / S) & 1, 121);
+        tc::tc_fence_after();
+        const uint32_t a0 = smem_u32(sm + (size_t)s * (P::kA + P::kB));
+        const uint64_t ad = tc::sdesc(a0, 0, 1024), bd = tc::sdesc(a0 + P::kA, 0, 1024);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) mma_i8(tmem, ad + 2 * k, bd + 2 * k, idesc, (i | k) != 0);
-      tc::mma_commit(empty + s);
+        for (int q = 0; q < 4; ++q)
+          mma_i8(tmem + buf * P::kCols, ad + 2 * q, bd + 2 * q, idesc, (k | q) != 0);
+        tc::mma_commit(empty + s);
+      }
+      tc::mma_commit(acc_full + buf);
     }
-    tc::mma_commit(done);
-  }
-  __syncwarp();
-  grid_dependency_wait();
-  tc::mbar_wait(done, 0, 122);
-  tc::tc_fence_after();
-
-  // lane = weight row n0 + 32 warp + lane, column = token m0 + c
-  const int n = n0 + tid;
-  if (split == 1) {
-    const float sb = n < o.N ? o.sb[n] : 0.f, bias = n < o.N ? bias_at(o, n) : 0.f;
-    const int mt = min(BN, o.M - m0);
-#pragma unroll 1
-    for (int c0 = 0; c0 < mt; c0 += 16) {
-      float v[16];
-      tc::tmem_ld16(tmem + ((uint32_t)(warp * 32) << 16) + c0, v);
-      tc::tmem_wait_ld();
-      if (n < o.N) {
+  } else if (warp >= 2 && split == 1) {
+    const int quad = warp & 3, ch = quad * 32 + lane;  // lane = weight row n0 + ch
+    const int es = o.y_bf16 ? 2 : 4, chunk = min(BN, kNStaging / (128 * es));
+    grid_dependency_wait();
+    uint32_t at = 0;
+    for (int t = first; t < tiles; t += stride, ++at) {
+      const int buf = at & 1, n0 = t % wt * 128, m0 = t / wt * BN, n = n0 + ch;
+      const float sb = n < o.N ? o.sb[n] : 0.f, bias = n < o.N ? bias_at(o, n) : 0.f;
+      float* sa = sSa + buf * BN;
+      for (int i = tid - 64; i < BN; i += 128) sa[i] = m0 + i < o.M ? o.sa[m0 + i] : 0.f;
+      tc::mbar_wait(acc_full + buf, (at / 2) & 1, 122);
+      tc::tc_fence_after();
+      const int mt = min(BN, o.M - m0);
+      for (int c0 = 0; c0 < mt; c0 += chunk) {
+        if (tid == 64) tc::bulk_wait_read0();  // the store before has left the staging
+        tc::named_bar_sync(1, 128);            // (and the scales are there)
+        for (int c1 = 0; c1 < chunk; c1 += 16) {
+          float v[16];
+          tc::tmem_ld16(tmem + buf * P::kCols + ((uint32_t)(quad * 32) << 16) + c0 + c1, v);
+          tc::tmem_wait_ld();
 #pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          if (c0 + c >= mt) break;
-          const size_t at = (size_t)(m0 + c0 + c) * o.N + n;
-          const float y = scaled(__float_as_int(v[c]), o.sa[m0 + c0 + c], sb, bias);
-          if (o.y_bf16)
-            static_cast<bf16*>(o.y)[at] = __float2bfloat16_rn(y);
-          else
-            static_cast<float*>(o.y)[at] = y;
+          for (int c = 0; c < 16; c += 4) {
+            const float4 s4 = *reinterpret_cast<const float4*>(sa + c0 + c1 + c);
+            const float ss[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float y = scaled(__float_as_int(v[c + e]), ss[e], sb, bias);
+              if (o.y_bf16)
+                reinterpret_cast<bf16*>(staging)[(c1 + c + e) * 128 + ch] = __float2bfloat16_rn(y);
+              else
+                reinterpret_cast<float*>(staging)[(c1 + c + e) * 128 + ch] = y;
+            }
+          }
+        }
+        if (c0 + chunk >= mt) {  // the accumulator has been read
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(acc_empty + buf);
+        }
+        if (ytma) {
+          tc::fence_proxy_async_smem();
+          tc::named_bar_sync(1, 128);
+          if (tid == 64) {
+            tma_store_2d(&ty, staging, n0, m0 + c0);
+            tc::bulk_commit();
+          }
+        } else {
+          tc::named_bar_sync(1, 128);
+          if (n < o.N) {
+            const int rows = min(chunk, mt - c0);
+            if (o.y_bf16)
+              for (int r = 0; r < rows; ++r)
+                static_cast<bf16*>(o.y)[(size_t)(m0 + c0 + r) * o.N + n] =
+                    reinterpret_cast<const bf16*>(staging)[r * 128 + ch];
+            else
+              for (int r = 0; r < rows; ++r)
+                static_cast<float*>(o.y)[(size_t)(m0 + c0 + r) * o.N + n] =
+                    reinterpret_cast<const float*>(staging)[r * 128 + ch];
+          }
         }
       }
     }
-  } else {
-    int* part = reinterpret_cast<int*>(sm);  // [BN][128]: every load has been consumed
+    if (tid == 64) tc::bulk_wait0();
+  }
+  __syncwarp();
+  if (split > 1) {  // one tile: n0, m0
+    const int n0 = first % wt * 128, m0 = first / wt * BN;
+    int* part = reinterpret_cast<int*>(sm);  // [BN][128], once every load has been consumed
+    if (warp >= 2) {
+      const int quad = warp & 3;
+      grid_dependency_wait();
+      tc::mbar_wait(acc_full, 0, 124);
+      tc::tc_fence_after();
 #pragma unroll 1
-    for (int c0 = 0; c0 < BN; c0 += 16) {
-      float v[16];
-      tc::tmem_ld16(tmem + ((uint32_t)(warp * 32) << 16) + c0, v);
-      tc::tmem_wait_ld();
-      // a share of K may be empty (fewer K tiles than CTAs): its accumulator was never written
+      for (int c0 = 0; c0 < BN; c0 += 16) {
+        float v[16];
+        tc::tmem_ld16(tmem + ((uint32_t)(quad * 32) << 16) + c0, v);
+        tc::tmem_wait_ld();
 #pragma unroll
-      for (int c = 0; c < 16; ++c) part[(c0 + c) * 128 + tid] = nk ? __float_as_int(v[c]) : 0;
+        for (int c = 0; c < 16; ++c)
+          part[(c0 + c) * 128 + quad * 32 + lane] = __float_as_int(v[c]);
+      }
     }
     cluster_sync();
     // the tile's token x channel elements in fours, dealt to the CTAs of the cluster
     const int mt = min(BN, o.M - m0), quads = mt * 32;
     const uint32_t base = smem_u32(part);
-    for (int e = rank * 128 + tid; e < quads; e += split * 128) {
+    for (int e = rank * 192 + tid; e < quads; e += split * 192) {
       const int c = e >> 5, q = (e & 31) * 4;
       int4 sum = make_int4(0, 0, 0, 0);
+#pragma unroll 4
       for (int r = 0; r < split; ++r) {
         const int4 p = ld_cluster_int4(map_to_rank(base + (c * 128 + q) * 4, r));
         sum.x += p.x;
@@ -374,34 +453,48 @@ i8_narrow_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__
       }
       const float sa = o.sa[m0 + c];
       const int v[4] = {sum.x, sum.y, sum.z, sum.w};
+      const size_t at = (size_t)(m0 + c) * o.N + n0 + q;
+      float y[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int nn = n0 + q + i;
-        if (nn >= o.N) break;
-        const float y = scaled(v[i], sa, o.sb[nn], bias_at(o, nn));
-        const size_t at = (size_t)(m0 + c) * o.N + nn;
-        if (o.y_bf16)
-          static_cast<bf16*>(o.y)[at] = __float2bfloat16_rn(y);
-        else
-          static_cast<float*>(o.y)[at] = y;
+        const int nn = min(n0 + q + i, o.N - 1);
+        y[i] = scaled(v[i], sa, o.sb[nn], bias_at(o, nn));
+      }
+      if (n0 + q + 4 <= o.N && (o.N & 3) == 0) {  // y is 16-byte aligned or ytma is off
+        if (ytma && o.y_bf16)
+          *reinterpret_cast<uint2*>(static_cast<bf16*>(o.y) + at) =
+              make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+        else if (ytma)
+          *reinterpret_cast<float4*>(static_cast<float*>(o.y) + at) =
+              make_float4(y[0], y[1], y[2], y[3]);
+      }
+      if (!(ytma && n0 + q + 4 <= o.N && (o.N & 3) == 0)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (n0 + q + i >= o.N) break;
+          if (o.y_bf16)
+            static_cast<bf16*>(o.y)[at + i] = __float2bfloat16_rn(y[i]);
+          else
+            static_cast<float*>(o.y)[at + i] = y[i];
+        }
       }
     }
     cluster_sync();  // peers read this CTA's partials until here
   }
   tc::tc_fence_before();
   __syncthreads();
-  if (warp == 1) tc::tmem_dealloc(tmem, P::kCols);
+  if (warp == 1) tc::tmem_dealloc(tmem, 2 * P::kCols);
 }
 
 // ---------------------------------------------------------------------- wide
-constexpr int kWS = 6;                       // operand stages
+constexpr int kWS = 5;                       // operand stages
 constexpr int kWHalf = 128 * 128;            // bytes of one operand's half of a stage
 constexpr int kWStage = 2 * kWHalf;          // a CTA's bytes of a stage
-constexpr int kWStaging = 4 * 32 * 128;      // 32 rows x 128 bytes of y for each epilogue warp
+constexpr int kWStaging = 8 * 32 * 128;      // 32 rows x 128 bytes of y for each epilogue warp
 constexpr size_t kWSmem = 1024 + (size_t)kWS * kWStage + kWStaging + 2 * 256 * 4 + 256;
 
-// Warps: 0 TMA, 1 MMA (and TMEM), 2..5 epilogue.
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
+// Warps: 0 TMA, 1 MMA (and TMEM), 2..9 epilogue (two a lane quadrant, 128 columns each).
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1)
 i8_wide_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw,
                const __grid_constant__ CUtensorMap ty, const Out o, const int ytma) {
   extern __shared__ unsigned char raw[];
@@ -413,13 +506,13 @@ i8_wide_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ C
   uint64_t* full = reinterpret_cast<uint64_t*>(sBias + 256);  // in the leader: both CTAs' bytes
   uint64_t* empty = full + kWS;
   uint64_t* acc_full = empty + kWS;    // [2]
-  uint64_t* acc_empty = acc_full + 2;  // [2], in the leader: the eight epilogue warps
+  uint64_t* acc_empty = acc_full + 2;  // [2], in the leader: the sixteen epilogue warps
   uint32_t* tptr = reinterpret_cast<uint32_t*>(acc_empty + 2);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = cluster_rank();
   if (tid == 0) {
     for (int s = 0; s < kWS; ++s) tc::mbar_init(full + s, 1), tc::mbar_init(empty + s, 1);
-    for (int i = 0; i < 2; ++i) tc::mbar_init(acc_full + i, 1), tc::mbar_init(acc_empty + i, 8);
+    for (int i = 0; i < 2; ++i) tc::mbar_init(acc_full + i, 1), tc::mbar_init(acc_empty + i, 16);
     tc::fence_mbar_init();
     tc::prefetch_tmap(&tx);
     tc::prefetch_tmap(&tw);
@@ -489,72 +582,89 @@ i8_wide_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ C
       commit_pair(acc_full + buf);
     }
   } else if (warp >= 2) {
-    const int quad = warp & 3, etid = tid - 64;
-    unsigned char* buf_y = staging + quad * 32 * 128;
+    const int quad = warp & 3, col0 = (warp - 2) / 4 * 128, etid = tid - 64;
+    unsigned char* buf_y = staging + (warp - 2) * 32 * 128;
     const uint32_t peer_free[2] = {map_to_rank(smem_u32(acc_empty), 0),
                                    map_to_rank(smem_u32(acc_empty + 1), 0)};
+    const int per = o.y_bf16 ? 64 : 32;  // columns a 128-byte row of the staging holds
     grid_dependency_wait();
     uint32_t at = 0;
     for (int t = cl; t < tiles; t += ncl, ++at) {
       int mt, nt;
       place(t, mt, nt);
       const int buf = at & 1, n0 = nt * 256, row0 = mt * 256 + rank * 128 + quad * 32;
-      tc::named_bar_sync(1, 128);  // the scales of the tile before have been used
-      for (int i = etid; i < 256; i += 128) {
-        sSb[i] = n0 + i < o.N ? o.sb[n0 + i] : 0.f;
-        sBias[i] = n0 + i < o.N ? bias_at(o, n0 + i) : 0.f;
+      tc::named_bar_sync(1, 256);  // the scales of the tile before have been used
+      if (n0 + etid < o.N) {
+        sSb[etid] = o.sb[n0 + etid];
+        sBias[etid] = bias_at(o, n0 + etid);
       }
       const int row = row0 + lane;
       const float sa = row < o.M ? o.sa[row] : 0.f;
-      tc::named_bar_sync(1, 128);
+      tc::named_bar_sync(1, 256);
       tc::mbar_wait(acc_full + buf, (at / 2) & 1, 133);
       tc::tc_fence_after();
-      const int per = o.y_bf16 ? 64 : 32;  // columns a 128-byte row of the staging holds
-#pragma unroll 1
-      for (int c0 = 0; c0 < 256; c0 += per) {
-        if (lane == 0) tc::bulk_wait_read0();  // the store before has left the staging
-        __syncwarp();
-        const uint32_t ta = tmem + buf * 256 + c0 + ((uint32_t)(quad * 32) << 16);
-#pragma unroll 1
-        for (int h = 0; h < per; h += 32) {
-          float v[32];
-          tc::tmem_ld32(ta + h, v);
-          tc::tmem_wait_ld();
-          if (c0 + h + 32 >= 256) {  // the accumulator has been read
-            tc::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) arrive_remote(peer_free[buf]);
-          }
+      const uint32_t ta = tmem + buf * 256 + col0 + ((uint32_t)(quad * 32) << 16);
+      float v[2][32];
+      tc::tmem_ld32(ta, v[0]);
 #pragma unroll
-          for (int c = 0; c < 32; ++c)
-            v[c] = scaled(__float_as_int(v[c]), sa, sSb[c0 + h + c], sBias[c0 + h + c]);
-          if (o.y_bf16) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const uint4 w = make_uint4(
-                  pack_bf16(v[8 * q], v[8 * q + 1]), pack_bf16(v[8 * q + 2], v[8 * q + 3]),
-                  pack_bf16(v[8 * q + 4], v[8 * q + 5]), pack_bf16(v[8 * q + 6], v[8 * q + 7]));
-              *reinterpret_cast<uint4*>(buf_y + lane * 128 + ((((h >> 3) + q) ^ (lane & 7)) << 4)) = w;
-            }
-          } else {
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-              *reinterpret_cast<float4*>(buf_y + lane * 128 + ((q ^ (lane & 7)) << 4)) =
-                  make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-          }
+      for (int q = 0; q < 4; ++q) {  // 32 columns at a time, the next ones loading
+        tc::tmem_wait_ld();
+        if (q < 3) {
+          tc::tmem_ld32(ta + 32 * (q + 1), v[(q + 1) & 1]);
+        } else {  // the accumulator has been read
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_remote(peer_free[buf]);
         }
+        float(&x)[32] = v[q & 1];
+        const int c0 = col0 + 32 * q;
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+          const float4 s4 = *reinterpret_cast<const float4*>(sSb + c0 + c);
+          const float ss[4] = {s4.x, s4.y, s4.z, s4.w};
+          float bb[4] = {0.f, 0.f, 0.f, 0.f};
+          if (o.bias) {
+            const float4 b4 = *reinterpret_cast<const float4*>(sBias + c0 + c);
+            bb[0] = b4.x, bb[1] = b4.y, bb[2] = b4.z, bb[3] = b4.w;
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            x[c + e] = scaled(__float_as_int(x[c + e]), sa, ss[e], bb[e]);
+        }
+        const bool starts = (32 * q) % per == 0, ends = (32 * (q + 1)) % per == 0;
+        if (starts) {
+          if (lane == 0) tc::bulk_wait_read0();  // the store before has left the staging
+          __syncwarp();
+        }
+        if (o.y_bf16) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const uint4 w = make_uint4(
+                pack_bf16(x[8 * u], x[8 * u + 1]), pack_bf16(x[8 * u + 2], x[8 * u + 3]),
+                pack_bf16(x[8 * u + 4], x[8 * u + 5]), pack_bf16(x[8 * u + 6], x[8 * u + 7]));
+            *reinterpret_cast<uint4*>(buf_y + lane * 128 +
+                                      ((((q & 1) * 4 + u) ^ (lane & 7)) << 4)) = w;
+          }
+        } else {
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            *reinterpret_cast<float4*>(buf_y + lane * 128 + ((u ^ (lane & 7)) << 4)) =
+                make_float4(x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]);
+        }
+        if (!ends) continue;
+        const int cs = n0 + c0 + 32 - per;  // first column of the staging
         if (ytma) {
           tc::fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0 && row0 < o.M && n0 + c0 < o.N) {
-            tma_store_2d(&ty, buf_y, n0 + c0, row0);
+          if (lane == 0 && row0 < o.M && cs < o.N) {
+            tma_store_2d(&ty, buf_y, cs, row0);
             tc::bulk_commit();
           }
         } else {
           __syncwarp();
           for (int r = 0; r < 32 && row0 + r < o.M; ++r)
-            for (int c = lane; c < per && n0 + c0 + c < o.N; c += 32) {
-              const size_t to = (size_t)(row0 + r) * o.N + n0 + c0 + c;
+            for (int c = lane; c < per && cs + c < o.N; c += 32) {
+              const size_t to = (size_t)(row0 + r) * o.N + cs + c;
               if (o.y_bf16)
                 static_cast<bf16*>(o.y)[to] = *reinterpret_cast<const bf16*>(
                     buf_y + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
@@ -579,7 +689,8 @@ i8_wide_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ C
 
 // ---------------------------------------------------------------------- host
 int encode(CUtensorMap* m, const char* what, CUtensorMapDataType type, const void* p, int cols,
-           int rows, long long row_bytes, int box_cols, int box_rows) {
+           int rows, long long row_bytes, int box_cols, int box_rows,
+           CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
   auto fn = tc::encode_tiled_fn();
   if (!fn) {
     set_error("int8: cuTensorMapEncodeTiled is not available");
@@ -590,7 +701,7 @@ int encode(CUtensorMap* m, const char* what, CUtensorMapDataType type, const voi
   const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
   const cuuint32_t es[2] = {1, 1};
   const CUresult r = fn(m, type, 2, const_cast<void*>(p), dims, strides, box, es,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_error(std::string("int8: the tensor map of ") + what + " could not be encoded, driver code " +
@@ -630,22 +741,38 @@ struct Operand {
   int rows;
 };
 
+// Shares of K of the narrow kernel: K is split while the tiles leave SMs idle and
+// every share keeps two steps of 128.
+int k_split(long long tiles, int KT) {
+  int split = 1;
+  while (split < 8 && tiles * split < 148 && KT >= 4 * split) split *= 2;
+  return split;
+}
+
 template <int BN>
 int launch_narrow(const Operand& x, const Operand& w, const Out& o, bool after_quantize,
                   cudaStream_t st) {
-  CUtensorMap tw, tx;
+  const int es = o.y_bf16 ? 2 : 4;
+  const int ytma = aligned16(o.y) && ((long long)o.N * es) % 16 == 0;
+  const int wt = ceil_div(o.N, 128), mt = ceil_div(o.M, BN), KT = ceil_div(o.K, 128);
+  const int split = k_split((long long)wt * mt, KT);
+  CUtensorMap tw, tx, ty;
   int rc = encode(&tw, "the weight", CU_TENSOR_MAP_DATA_TYPE_UINT8, w.p, o.K, o.N, w.ld, 128, 128);
   if (!rc) rc = encode(&tx, "x", CU_TENSOR_MAP_DATA_TYPE_UINT8, x.p, o.K, o.M, x.ld, 128, BN);
+  if (!rc && ytma && split == 1)
+    rc = encode(&ty, "y", o.y_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
+                o.y, o.N, o.M, (long long)o.N * es, 128, std::min(BN, kNStaging / (128 * es)),
+                CU_TENSOR_MAP_SWIZZLE_NONE);
+  else
+    ty = tx;
   if (rc) return rc;
   static bool done[64] = {false};
   rc = allow_smem(i8_narrow_kernel<BN>, Narrow<BN>::kSmem, done);
   if (rc) return rc;
-  const int wt = ceil_div(o.N, 128), mt = ceil_div(o.M, BN), KT = ceil_div(o.K, 128);
-  int split = 1;
-  while (split < 8 && wt * mt * split < 148 && KT >= 4 * split) split *= 2;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(wt * split, mt);
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = split > 1 ? dim3(wt * mt * split)
+                          : dim3((unsigned)std::min<long long>((long long)wt * mt, 296));
+  cfg.blockDim = dim3(192);
   cfg.dynamicSmemBytes = Narrow<BN>::kSmem;
   cfg.stream = st;
   cudaLaunchAttribute at[2];
@@ -656,7 +783,7 @@ int launch_narrow(const Operand& x, const Operand& w, const Out& o, bool after_q
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = after_quantize ? 2 : 1;
-  return launched(cudaLaunchKernelEx(&cfg, i8_narrow_kernel<BN>, tw, tx, o, split),
+  return launched(cudaLaunchKernelEx(&cfg, i8_narrow_kernel<BN>, tw, tx, ty, o, split, ytma),
                   "i8_narrow_kernel");
 }
 
@@ -678,7 +805,7 @@ int launch_wide(const Operand& x, const Operand& w, const Out& o, bool after_qua
   const long long tiles = (long long)ceil_div(o.M, 256) * ceil_div(o.N, 256);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * (unsigned)std::min<long long>(tiles, 74));
-  cfg.blockDim = dim3(192);
+  cfg.blockDim = dim3(320);
   cfg.dynamicSmemBytes = kWSmem;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
@@ -689,25 +816,57 @@ int launch_wide(const Operand& x, const Operand& w, const Out& o, bool after_qua
   return launched(cudaLaunchKernelEx(&cfg, i8_wide_kernel, tx, tw, ty, o, ytma), "i8_wide_kernel");
 }
 
+template <typename T>
+void launch_quantize(const void* x, long long ldx, int8_t* codes, long long ldc, float* scale,
+                     int M, int K, cudaStream_t st) {
+  const T* p = static_cast<const T*>(x);
+  // a warp holds 8 vectors a lane: 2048 bf16 or 1024 fp32
+  if (K <= 256 * Vec<T>::N)
+    i8_quantize_kernel<T, 32, 8>
+        <<<ceil_div(M, kQT / 32), kQT, 0, st>>>(p, ldx, codes, ldc, scale, M, K);
+  else
+    i8_quantize_kernel<T, kQT, 4><<<M, kQT, 0, st>>>(p, ldx, codes, ldc, scale, M, K);
+}
+
 int quantize(const void* x, int x_dtype, long long ldx, int8_t* codes, long long ldc, float* scale,
              int M, int K, cudaStream_t st) {
   if (x_dtype == LZ_DTYPE_F32)
-    i8_quantize_kernel<float><<<M, kQT, 0, st>>>(static_cast<const float*>(x), ldx, codes, ldc,
-                                                 scale, K);
+    launch_quantize<float>(x, ldx, codes, ldc, scale, M, K, st);
   else
-    i8_quantize_kernel<bf16><<<M, kQT, 0, st>>>(static_cast<const bf16*>(x), ldx, codes, ldc,
-                                                scale, K);
+    launch_quantize<bf16>(x, ldx, codes, ldc, scale, M, K, st);
   count_launches(1);
   return check_launch("i8_quantize_kernel");
 }
 
+std::atomic<int> g_path{0};
+
+// Which kernel, by an estimate of both in hundredths of a us, fitted to measured
+// times (quantisation included) over M = 64 .. 2048, K = 512 .. 8192, N = 512 ..
+// 128256. A step of 128 of K costs a 256 x 256 tile of a CTA pair 0.29 us and a
+// 128 x 128 tile 0.5 us with two CTAs on the SM; a tile costs 2 and 2.5 us more.
+// Measured, narrow / wide: M = 256, K = 8192: N = 512 11.0 / 24.7 us, N = 128256
+// 337 / 214 us; M = 512, K = 8192: N = 2048 17.6 / 25.9, N = 8192 35.7 / 30.9;
+// M = 256, N = 512: K = 512 10.2 / 8.2, K = 2048 8.5 / 11.5. Up to 64 tokens the
+// narrow one is never slower.
+bool use_wide(int M, int N, int K) {
+  if (M <= 64) return false;
+  const long long KT = ceil_div(K, 128);
+  const long long small = (long long)ceil_div(M, 128) * ceil_div(N, 128);
+  const long long large = (long long)ceil_div(M, 256) * ceil_div(N, 256);
+  const int split = k_split(small, (int)KT);
+  const long long narrow = 550 + (small * split + 295) / 296 * (50 * KT / split + 250);
+  const long long wide = 500 + (large + 73) / 74 * (29 * KT + 200);
+  return wide < narrow;
+}
+
 int product(const Operand& x, const Operand& w, const Out& o, bool after_quantize,
             cudaStream_t st) {
+  const int path = g_path.load(std::memory_order_relaxed);
+  if (path ? path == 2 : use_wide(o.M, o.N, o.K)) return launch_wide(x, w, o, after_quantize, st);
   if (o.M <= 16) return launch_narrow<16>(x, w, o, after_quantize, st);
   if (o.M <= 32) return launch_narrow<32>(x, w, o, after_quantize, st);
   if (o.M <= 64) return launch_narrow<64>(x, w, o, after_quantize, st);
-  if (o.M <= 512) return launch_narrow<128>(x, w, o, after_quantize, st);
-  return launch_wide(x, w, o, after_quantize, st);
+  return launch_narrow<128>(x, w, o, after_quantize, st);
 }
 
 long long row16(int K) { return ((long long)K + 15) / 16 * 16; }
@@ -733,8 +892,8 @@ int check_out(const void* bias, int bias_dtype, const void* y, int y_dtype, int 
   LZ_REQUIRE(M >= 1 && N >= 1 && K >= 1, LZ_ERR_INVALID_ARGUMENT, "sizes must be positive");
   LZ_REQUIRE(K <= kMaxK, LZ_ERR_UNSUPPORTED,
              "K above 131071 can overflow the 32-bit integer sum");
-  LZ_REQUIRE(N <= (1 << 30) && (M + 15ll) / 16 <= (1ll << 30), LZ_ERR_UNSUPPORTED,
-             "sizes too large");
+  LZ_REQUIRE(N <= (1 << 30) && M <= (1 << 30) && (N / 128 + 1ll) * (M / 16 + 1ll) < (1ll << 31),
+             LZ_ERR_UNSUPPORTED, "sizes too large");
   LZ_REQUIRE(y, LZ_ERR_INVALID_ARGUMENT, "null pointer");
   LZ_REQUIRE(y_dtype == LZ_DTYPE_F32 || y_dtype == LZ_DTYPE_BF16, LZ_ERR_INVALID_ARGUMENT,
              "y must be LZ_DTYPE_F32 or LZ_DTYPE_BF16");
@@ -747,6 +906,14 @@ int check_out(const void* bias, int bias_dtype, const void* y, int y_dtype, int 
 int int8_timeout_flag(unsigned int* out) { return tc::read_timeout_flag_here(out); }
 int int8_timeout_clear() { return tc::clear_timeout_flag_here(); }
 }  // namespace lz
+
+extern "C" int lz_int8_set_path(int path) {
+  if (path < 0 || path > 2) {
+    lz::set_error("path must be 0 (chosen by size), 1 (narrow) or 2 (wide)");
+    return -LZ_ERR_INVALID_ARGUMENT;
+  }
+  return lz::g_path.exchange(path);
+}
 
 extern "C" int lz_int8_quantize(const void* x, int x_dtype, long long x_ld, void* codes,
                                 long long codes_ld, float* scale, int M, int K, void* stream) {

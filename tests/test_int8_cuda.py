@@ -109,6 +109,27 @@ def test_matmul_bit_for_bit(M, K, N, dtype):
         assert _same(y, _product(a, sa, b, sb, bi, dtype)), (M, K, N)
 
 
+@pytest.mark.parametrize("path", [1, 2])
+@pytest.mark.parametrize("M,K,N", [(1, 200, 300), (20, 16, 1), (100, 700, 2000), (300, 129, 257),
+                                   (1000, 4096, 136), (260, 384, 5000), (3000, 65, 700),
+                                   (129, 300, 40000)])
+def test_both_kernels_at_any_size(M, K, N, path):
+    """Few and many tokens, tiles more and fewer than the machine holds, K in one step
+    or split, y that TMA can and cannot write: both kernels give the same bits."""
+    from lizard_cuda import _lib, int8_matmul
+    g = torch.Generator(device=DEV).manual_seed(M + K + N)
+    a, b = _codes(M, K, g), _codes(N, K, g)
+    sa, sb = (torch.rand(n, generator=g, device=DEV) + 0.01 for n in (M, N))
+    bias = torch.randn(N, generator=g, device=DEV)
+    old = _lib.load().lz_int8_set_path(path)
+    try:
+        for dtype in (torch.bfloat16, torch.float32):
+            y = int8_matmul(a, sa, b, sb, bias, dtype=dtype)
+            assert _same(y, _product(a, sa, b, sb, bias, dtype))
+    finally:
+        assert _lib.load().lz_int8_set_path(old) == path
+
+
 @pytest.mark.parametrize("M,K,N", [(1, 130, 77), (40, 1001, 300), (800, 250, 301)])
 def test_linear_bit_for_bit_and_in_any_layout(M, K, N):
     from lizard_cuda import int8_linear, int8_matmul, int8_quantize
