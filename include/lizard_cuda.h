@@ -530,7 +530,9 @@ int lz_gla_decode_block(const void* fq, const void* fk, const void* v,
  * strides = {batch, head, token} in elements for q, k, v in turn (9 values;
  * strides_prev 6), host memory, last dimension contiguous; cos, sin [T, D] per
  * batch row, cs_sb elements apart (0: one table for all). Rings fp32
- * [B*Hkv, window, D], D even up to 256, window up to 1024. */
+ * [B*Hkv, window, D], D even up to 256, window up to 1024. The workspace (16-byte
+ * aligned, lz_swa_decode_block_workspace_bytes; 0 for T = 0) holds the rotated block. */
+size_t lz_swa_decode_block_workspace_bytes(int B, int H, int Hkv, int T, int D);
 int lz_swa_decode_block(const void* q, const void* k, const void* v, int x_dtype,
                         const long long* strides, const void* cos, const void* sin,
                         int cs_dtype, long long cs_sb,
@@ -538,6 +540,7 @@ int lz_swa_decode_block(const void* q, const void* k, const void* v, int x_dtype
                         const void* cos_prev, const void* sin_prev, long long cs_prev_sb,
                         const int* count, float* k_ring, float* v_ring, const int* pos,
                         const float* meta, int n_meta, void* y,
+                        void* workspace, size_t workspace_bytes,
                         int B, int H, int Hkv, int T, int T_prev, int window, int D,
                         void* stream);
 

@@ -9,18 +9,21 @@
 // over the keys at positions base + t - W < position <= base + t. The block's
 // own keys never enter the ring here, so a refused token leaves no trace.
 //
-// One CTA per (batch row, key/value head) for all rep T query rows of the group.
-// Bound: 8 (W + T) D bytes of ring a head against 4 rep T (W + T) D operations:
-// memory. TMA brings the whole ring (of a long window, a part at a time) into
-// shared memory as it is, fp32 in 128-byte swizzled rows, while the queries and the
-// new keys are rotated; the accepted tokens are written over their slots there and
-// in global memory. A warp takes a 16-row tile of queries over 16 keys at a time: it
+// Two kernels. The first rotates: the accepted keys and their values go into the
+// ring, the block's queries (split into bf16 hi + lo) and keys into a workspace, laid
+// out as the second wants them in shared memory; a thread takes the same columns of
+// all heads of a token, so cos and sin are read once. The second, launched under
+// the first, attends: one CTA per (batch row, key/value head) for all rep T query
+// rows of the group. Bound: 8 (W + T) D bytes of ring a head against 4 rep T (W + T) D
+// operations: memory. Everything it reads arrives by TMA and bulk copies, the ring
+// as it is, fp32 in 128-byte swizzled rows (of a long window, a part at a time).
+// A warp takes a 16-row tile of queries over 16 keys at a time: it
 // reads the keys as the B fragments of mma.sync m16n8k16, splits them into bf16 hi + lo
 // in registers (hi hi + hi lo + lo hi keeps 2^-17 of a product, well under the bf16
 // output) and keeps its own maximum and sum; the warps' outputs meet at the end,
 // scaled to the common maximum, so a block of few rows keeps every warp busy. Nothing
 // converted is written back to shared memory. (A warp on two row tiles converts a
-// key once instead of twice, but its registers leave 16 warps an SM for 24, and
+// key once instead of twice, but its registers leave 16 warps an SM for 20, and
 // the nine 16-key tiles of a window of 128 and its block do not divide over eight.)
 //
 // Fragments. Within a step of 16 columns thread j takes d = 4j .. 4j+3 (the
@@ -57,6 +60,7 @@ struct SwaBlockArgs {
   const float* meta;
   float *kr, *vr;
   bf16* y;
+  unsigned char* ws;  // SwaWork a (batch row, key/value head)
   int n_meta, T, Tp, H, Hkv, W, D;
   int rep;    // query heads a key/value head
   int part;   // ring rows in shared memory at a time, a multiple of 16
@@ -146,7 +150,97 @@ __device__ __forceinline__ void put_split(bf16* hi, bf16* lo, int at, float2 x) 
   }
 }
 
-// Shared memory, in bytes from the 1024-aligned start.
+// Workspace of a (batch row, key/value head), in bytes: queries hi and lo, a pass of
+// 16 QT rows after another ([hi | lo][16 QT][DP + 8]), then the new keys and values
+// ([DP / 32 boxes][T rounded up to 16][32], swizzled).
+struct SwaWork {
+  int q, k, v, total;
+};
+__host__ __device__ inline SwaWork swa_work(int DP, int QT, int R, int T) {
+  const int passes = (R + 16 * QT - 1) / (16 * QT), rows = (T + 15) & ~15;
+  SwaWork w;
+  w.q = 0;
+  w.k = passes * 2 * 16 * QT * (DP + 8) * 2;
+  w.v = w.k + rows * DP * 4;
+  w.total = w.v + rows * DP * 4;
+  return w;
+}
+
+// The first kernel. blockIdx = (block of 256 threads over the (token, columns) of a
+// pair of heads, head, batch row); tokens 0 .. TN are the block's, the rest the
+// pending ones. N: columns a thread takes (2 where alignment allows).
+template <typename XT, int DP, int QT, int N>
+__global__ void __launch_bounds__(256) swa_rotate_kernel(const SwaBlockArgs a) {
+  constexpr int LQ = DP + 8, RQ = 16 * QT, PER = DP / 2 / N;  // threads a token
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  const int i = blockIdx.x * 256 + threadIdx.x, row = i / PER, d = i % PER * N;
+  const int b = blockIdx.z, hk = blockIdx.y, T = a.T, D = a.D, half = D / 2;
+  const int TN = (T + 15) & ~15, rep = a.rep, R = rep * T;
+  if (row < TN) {
+    const SwaWork o = swa_work(DP, QT, R, T);
+    unsigned char* ws = a.ws + (size_t)(b * a.Hkv + hk) * o.total;
+    float* wk = reinterpret_cast<float*>(ws + o.k);
+    float* wv = reinterpret_cast<float*>(ws + o.v);
+    const int t = row;
+    const bool in = t < T && d < half;
+    const XT* kp = static_cast<const XT*>(a.k.p) + b * a.k.sb + hk * a.k.sh + t * a.k.st + d;
+    const XT* vp = static_cast<const XT*>(a.v.p) + b * a.v.sb + hk * a.v.sh + t * a.v.st + d;
+    const XT* qp = static_cast<const XT*>(a.q.p) + b * a.q.sb + hk * rep * a.q.sh + t * a.q.st + d;
+    // columns d .. and half + d .. of the rotation; beyond D, the zeros of the padding
+    const int e1 = d < half ? d : 2 * d, e2 = d < half ? d + half : 2 * d + N;
+    Angle ang = {};
+    float2 x1 = {}, x2 = {}, v1 = {}, v2 = {};
+    if (in) {
+      ang = angle<N>(a.rot, b * a.rot.sb + (long long)t * D + d, half);
+      x1 = ldn<XT, N>(kp), x2 = ldn<XT, N>(kp + half);
+      v1 = ldn<XT, N>(vp), v2 = ldn<XT, N>(vp + half);
+      rotate(x1, x2, ang);
+    }
+    put<N>(wk + spot(TN, t, e1), x1);
+    put<N>(wk + spot(TN, t, e2), x2);
+    put<N>(wv + spot(TN, t, e1), v1);
+    put<N>(wv + spot(TN, t, e2), v2);
+    if (t < T) {
+      const int c1 = slot_of(e1), c2 = slot_of(e2);
+#pragma unroll 4
+      for (int h = 0; h < rep; ++h) {
+        float2 q1 = {}, q2 = {};
+        if (in) {
+          q1 = ldn<XT, N>(qp + h * a.q.sh), q2 = ldn<XT, N>(qp + h * a.q.sh + half);
+          rotate(q1, q2, ang);
+        }
+        const int r = h * T + t;
+        bf16* hi = reinterpret_cast<bf16*>(ws) + (r / RQ) * (2 * RQ * LQ) + (r % RQ) * LQ;
+        put_split<N>(hi, hi + RQ * LQ, c1, q1);
+        put_split<N>(hi, hi + RQ * LQ, c2, q2);
+      }
+    }
+    // rows of the last pass beyond R: zeros, dealt to the block's rows
+    const int pads = (R + RQ - 1) / RQ * RQ - R;
+    for (int p = t; p < pads; p += TN) {
+      const int r = R + p;
+      bf16* hi = reinterpret_cast<bf16*>(ws) + (r / RQ) * (2 * RQ * LQ) + (r % RQ) * LQ;
+      put_split<N>(hi, hi + RQ * LQ, slot_of(e1), make_float2(0.f, 0.f));
+      put_split<N>(hi, hi + RQ * LQ, slot_of(e2), make_float2(0.f, 0.f));
+    }
+  } else if (row < TN + a.Tp && d < half) {
+    const int t = row - TN, W = a.W;
+    const int n = a.count ? min(max(a.count[b], 0), a.Tp) : a.Tp;
+    if (t >= n || t < n - W) return;  // of more accepted tokens than the window, the last W
+    const XT* kp = static_cast<const XT*>(a.kp.p) + b * a.kp.sb + hk * a.kp.sh + t * a.kp.st + d;
+    const XT* vp = static_cast<const XT*>(a.vp.p) + b * a.vp.sb + hk * a.vp.sh + t * a.vp.st + d;
+    float2 x1 = ldn<XT, N>(kp), x2 = ldn<XT, N>(kp + half);
+    rotate(x1, x2, angle<N>(a.rot_p, b * a.rot_p.sb + (long long)t * D + d, half));
+    const int slot = (a.pos[b] % W + t) % W;
+    const size_t at = ((size_t)(b * a.Hkv + hk) * W + slot) * D + d;
+    put<N>(a.kr + at, x1);
+    put<N>(a.kr + at + half, x2);
+    put<N>(a.vr + at, ldn<XT, N>(vp));
+    put<N>(a.vr + at + half, ldn<XT, N>(vp + half));
+  }
+}
+
+// Shared memory of the second kernel, in bytes from the 1024-aligned start.
 struct SwaSmem {
   int k, v, nk, nv, q, stat, bar, total;
 };
@@ -167,9 +261,8 @@ __host__ __device__ inline SwaSmem swa_smem(int DP, int QT, int part, int T, int
   return s;
 }
 
-// DP: D padded to whole 32s. QT: 16-row tiles of queries at once, one a warp. N:
-// columns a thread rotates at once (2 where alignment allows).
-template <typename XT, int DP, int QT, int N>
+// DP: D padded to whole 32s. QT: 16-row tiles of queries at once, one a warp.
+template <int DP, int QT>
 __global__ void __launch_bounds__(32 * kWarps, DP <= 64 ? 2 : 1)
 swa_block_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                  const SwaBlockArgs a) {
@@ -179,7 +272,7 @@ swa_block_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__
       (reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, nw = nt >> 5;
   const int g = lane >> 2, j = lane & 3;
-  const int T = a.T, W = a.W, D = a.D, half = D / 2, part = a.part;
+  const int T = a.T, W = a.W, D = a.D, part = a.part;
   const int TN = (T + 15) & ~15;  // rows of the new tokens' tile
   const SwaSmem o = swa_smem(DP, QT, part, T, nw);
   float* sK = reinterpret_cast<float*>(sm + o.k);
@@ -195,84 +288,56 @@ swa_block_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__
   uint64_t* bar = reinterpret_cast<uint64_t*>(sm + o.bar);
   const int b = blockIdx.x, hk = blockIdx.y, bk = b * a.Hkv + hk;
   const int rep = a.rep, R = rep * T;
-  float* kring = a.kr + (size_t)bk * W * D;
-  float* vring = a.vr + (size_t)bk * W * D;
+  const float* kring = a.kr + (size_t)bk * W * D;
+  const float* vring = a.vr + (size_t)bk * W * D;
   const int parts = (W + part - 1) / part;
+  const SwaWork wo = swa_work(DP, QT, R, T);
+  const unsigned char* ws = a.ws + (size_t)bk * wo.total;
+  constexpr int kQBytes = 2 * RQ * LQ * 2;
   uint32_t phase = 0;
 
-  // ring rows [p part, (p + 1) part) into sK / sV
-  const auto load_part = [&](int p) {
-    if (a.tma) {
-      if (tid == 0) {
-        tc::mbar_expect_tx(bar, 2 * part * DP * 4);  // rows and columns beyond the ring: zeros
+  // ring rows [p part, (p + 1) part) into sK / sV; with the first part, the queries of
+  // pass `pass` and the new keys and values
+  const auto load = [&](int pass, int p) {
+    if (tid == 0 && (a.tma || !p)) {
+      const int nb = TN * DP * 4;
+      tc::mbar_expect_tx(bar, (a.tma ? 2 * part * DP * 4 : 0) + (p ? 0 : kQBytes + 2 * nb));
+      if (a.tma) {
 #pragma unroll
-        for (int i = 0; i < NG; ++i) {
+        for (int i = 0; i < NG; ++i) {  // rows and columns beyond the ring arrive as zeros
           tc::tma_load_3d(sK + i * part * 32, &tk, 32 * i, p * part, bk, bar);
           tc::tma_load_3d(sV + i * part * 32, &tv, 32 * i, p * part, bk, bar);
         }
       }
-    } else {
+      if (!p) {
+        tc::bulk_load(sQh, ws + wo.q + pass * kQBytes, kQBytes, bar);
+        tc::bulk_load(sNK, ws + wo.k, nb, bar);
+        tc::bulk_load(sNV, ws + wo.v, nb, bar);
+      }
+    }
+    if (!a.tma)
       for (int e = tid; e < part * DP; e += nt) {
         const int r = e / DP, d = e - r * DP, slot = p * part + r;
         const bool in = slot < W && d < D;
         sK[spot(part, r, d)] = in ? kring[(size_t)slot * D + d] : 0.f;
         sV[spot(part, r, d)] = in ? vring[(size_t)slot * D + d] : 0.f;
       }
-    }
   };
+  const int pos = a.pos[b];
+  const int n = a.Tp ? (a.count ? min(max(a.count[b], 0), a.Tp) : a.Tp) : 0;
   if (tid == 0) {
     tc::mbar_init(bar, 1);
     tc::fence_mbar_init();
+    tc::prefetch_tmap(&tk);
+    tc::prefetch_tmap(&tv);
   }
-  if (T) load_part(0);
-
-  const int pos = a.pos[b];
-  const int n = a.Tp ? (a.count ? min(max(a.count[b], 0), a.Tp) : a.Tp) : 0;
-  const int t0 = max(0, n - W);  // of more accepted tokens than the window, the last W
-  const int first = pos % W;
-  // Half a warp takes a token, a lane N columns and those D / 2 further.
-  const int unit = tid >> 4, units = nt >> 4, lane16 = tid & 15;
-  // accepted token t: its rotated key and its value
-  struct Entry {
-    float2 k1, k2, v1, v2;
-  };
-  const XT* kp = static_cast<const XT*>(a.kp.p) + b * a.kp.sb + hk * a.kp.sh;
-  const XT* vp = static_cast<const XT*>(a.vp.p) + b * a.vp.sb + hk * a.vp.sh;
-  const auto entry = [&](int t, int d) {
-    const XT *k = kp + t * a.kp.st + d, *v = vp + t * a.vp.st + d;
-    Entry e = {ldn<XT, N>(k), ldn<XT, N>(k + half), ldn<XT, N>(v), ldn<XT, N>(v + half)};
-    rotate(e.k1, e.k2, angle<N>(a.rot_p, b * a.rot_p.sb + (long long)t * D + d, half));
-    return e;
-  };
-  // to the ring, and to the copy of its rows row0 .. in shared memory
-  const auto put_entry = [&](const Entry& e, int t, int d, int row0, bool ring) {
-    const int slot = (first + t) % W, at = slot - row0;
-    if (T && at >= 0 && at < part) {
-      const int s1 = spot(part, at, d), s2 = spot(part, at, d + half);
-      put<N>(sK + s1, e.k1);
-      put<N>(sK + s2, e.k2);
-      put<N>(sV + s1, e.v1);
-      put<N>(sV + s2, e.v2);
-    }
-    if (ring) {
-      put<N>(kring + slot * D + d, e.k1);
-      put<N>(kring + slot * D + d + half, e.k2);
-      put<N>(vring + slot * D + d, e.v1);
-      put<N>(vring + slot * D + d + half, e.v2);
-    }
-  };
-  if (!T) {
-    for (int t = t0 + unit; t < n; t += units)
-      for (int d = lane16 * N; d < half; d += 16 * N) put_entry(entry(t, d), t, d, 0, true);
-    return;
-  }
-  // a token a unit loads now and waits in registers for the ring; others come later
-  const int mine = t0 + unit, dm = lane16 * N;
-  Entry early = {};
-  if (mine < n && dm < half) early = entry(mine, dm);
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");  // the ring and the workspace are written
+  asm volatile("fence.proxy.async;\n" ::: "memory");
+  load(0, 0);
+  __syncthreads();  // the barrier is initialised
 
   const int nr = (int)min((long long)pos + n, (long long)W);  // ring rows that hold a token
-  const int last = (first + n - 1 + W) % W;                   // slot of the newest (W >= 1)
+  const int last = (pos % W + n - 1 + W) % W;                 // slot of the newest (W >= 1)
   const float scale = rsqrtf((float)D) * kLog2e;
   const int krow = key_row(g), eight = 8 % T;
   const int rt = QT == 1 ? 0 : warp % QT;                     // this warp's row tile
@@ -280,66 +345,10 @@ swa_block_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__
   bool live = true;  // after a timeout nothing is written
 
   for (int r0 = 0; r0 < R; r0 += RQ) {
-    if (r0) {  // the merge of the rows before went over the keys: both again
+    if (r0) {  // the merge of the rows before went over the keys: again
       tc::fence_proxy_async_smem();
       __syncthreads();
-      load_part(0);
-    }
-    // zeros: keys T .. TN, query rows beyond R, columns D .. DP
-    for (int e = tid; e < (TN - T) * DP; e += nt) {
-      const int at = spot(TN, T + e / DP, e % DP);
-      sNK[at] = sNV[at] = 0.f;
-    }
-    for (int e = (R - r0) * LQ + tid; e < RQ * LQ; e += nt)
-      sQh[e] = sQl[e] = __float2bfloat16_rn(0.f);
-    if (D < DP) {
-      for (int e = tid; e < T * (DP - D); e += nt) {
-        const int at = spot(TN, e / (DP - D), D + e % (DP - D));
-        sNK[at] = sNV[at] = 0.f;
-      }
-      for (int e = tid; e < RQ * (DP - D); e += nt) {
-        const int at = e / (DP - D) * LQ + slot_of(D + e % (DP - D));
-        sQh[at] = sQl[at] = __float2bfloat16_rn(0.f);
-      }
-    }
-    {
-      // a token's rows two at a time: two query heads, or its key and value
-      const XT* qp = static_cast<const XT*>(a.q.p) + b * a.q.sb + hk * rep * a.q.sh;
-      const XT* kb = static_cast<const XT*>(a.k.p) + b * a.k.sb + hk * a.k.sh;
-      const XT* vb = static_cast<const XT*>(a.v.p) + b * a.v.sb + hk * a.v.sh;
-      const int groups = (rep + 1) / 2 + 1;
-      for (int i = unit; i < T * groups; i += units) {
-        const int grp = i / T, t = i - grp * T, h = 2 * grp;
-        const bool kv = grp + 1 == groups;
-        const XT* pa = kv ? kb + t * a.k.st : qp + h * a.q.sh + t * a.q.st;
-        const XT* pb = kv ? vb + t * a.v.st : pa + a.q.sh;
-        const int ra = h * T + t - r0, rb = ra + T;  // query rows of this pass
-        const bool two = kv || h + 1 < rep;
-        for (int d = lane16 * N; d < half; d += 16 * N) {
-          const Angle ang = angle<N>(a.rot, b * a.rot.sb + (long long)t * D + d, half);
-          float2 a1 = ldn<XT, N>(pa + d), a2 = ldn<XT, N>(pa + d + half), b1 = {}, b2 = {};
-          if (two) b1 = ldn<XT, N>(pb + d), b2 = ldn<XT, N>(pb + d + half);
-          rotate(a1, a2, ang);
-          if (kv) {
-            const int s1 = spot(TN, t, d), s2 = spot(TN, t, d + half);
-            put<N>(sNK + s1, a1);
-            put<N>(sNK + s2, a2);
-            put<N>(sNV + s1, b1);
-            put<N>(sNV + s2, b2);
-          } else {
-            rotate(b1, b2, ang);
-            const int c1 = slot_of(d), c2 = slot_of(d + half);
-            if (ra >= 0 && ra < RQ) {
-              put_split<N>(sQh, sQl, ra * LQ + c1, a1);
-              put_split<N>(sQh, sQl, ra * LQ + c2, a2);
-            }
-            if (two && rb >= 0 && rb < RQ) {
-              put_split<N>(sQh, sQl, rb * LQ + c1, b1);
-              put_split<N>(sQh, sQl, rb * LQ + c2, b2);
-            }
-          }
-        }
-      }
+      load(r0 / RQ, 0);
     }
     float m[2] = {-1e30f, -1e30f}, l[2] = {0.f, 0.f}, acc[4 * NG][4];
 #pragma unroll
@@ -355,24 +364,13 @@ swa_block_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__
       if (p) {
         tc::fence_proxy_async_smem();
         __syncthreads();  // the part before has been used
-        load_part(p);
+        load(0, p);
       }
-      if (!p && !r0) __syncthreads();  // the barrier is initialised
-      if (a.tma) {
+      if (a.tma || !p) {
         live = tc::mbar_wait(bar, phase, 96) && live;
         phase ^= 1;
-      } else {
-        __syncthreads();
       }
-      // the accepted tokens over what came, and (once) into the ring
-      const bool ring = !p && !r0 && live;
-      if (mine < n) {
-        if (dm < half) put_entry(early, mine, dm, p * part, ring);
-        for (int t = mine; t < n; t += units)
-          for (int d = t == mine ? dm + 16 * N : dm; d < half; d += 16 * N)
-            put_entry(entry(t, d), t, d, p * part, ring);
-      }
-      __syncthreads();
+      if (!a.tma) __syncthreads();
       const int held = min(max(nr - p * part, 0), part);  // rows of this part that hold a token
       const int ring_tiles = (held + 15) >> 4;
       const int tiles = ring_tiles + (p + 1 == parts ? TN >> 4 : 0);
@@ -483,7 +481,8 @@ swa_block_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__
       }
     }
     __syncthreads();
-    for (int e = tid >> 4; e < RQ; e += units) {  // a row a half warp, a lane a warp of its tile
+    const int lane16 = tid & 15;
+    for (int e = tid >> 4; e < RQ; e += nt >> 4) {  // a row a half warp, a lane a warp of its tile
       const int w = (lane16 * QT + (e >> 4)), at = w * 16 + (e & 15);
       const bool in = lane16 < kws;
       const float mw = in ? sMax[at] : -1e30f;
@@ -552,21 +551,31 @@ int ring_map(CUtensorMap* m, const float* p, const SwaBlockArgs& a, int heads) {
   return LZ_OK;
 }
 
-template <typename XT, int DP, int QT, int N>
-int launch_swa_block(SwaBlockArgs& a, int grid, cudaStream_t st) {
-  // the ring in shared memory, in parts of 64 KB of keys and values at most
-  a.part = std::min((a.W + 15) & ~15, 64 * 1024 / (DP * 8));
+// Ring rows in shared memory at a time: 64 KB of keys and values at most.
+int ring_part(int W, int DP) { return std::min((W + 15) & ~15, 64 * 1024 / (DP * 8)); }
+
+int launched(cudaError_t e, const char* what) {
+  if (e != cudaSuccess) {
+    set_error(std::string(what) + ": " + cudaGetErrorString(e));
+    return LZ_ERR_CUDA;
+  }
+  count_launches(1);
+  return check_launch(what);
+}
+
+template <int DP, int QT>
+int launch_attend(SwaBlockArgs& a, int B, cudaStream_t st) {
+  a.part = ring_part(a.W, DP);
   const int tiles = a.part / 16 + ((a.T + 15) >> 4);
   // as many warps as there are 16-key tiles for each row tile, in as few equal turns
   // as fit
   const int most_w = kWarps / QT, turns = ceil_div(tiles, most_w);
   const int warps = QT * std::max(ceil_div(tiles, turns), 4 / QT);
-  const size_t smem = swa_smem(DP, QT, a.part, a.T, warps).total;
   a.tma = a.D % 4 == 0 && aligned16(a.kr) && aligned16(a.vr);
   CUtensorMap tk = {}, tv = {};
-  if (a.tma && a.T) {
-    int rc = ring_map(&tk, a.kr, a, grid);
-    if (!rc) rc = ring_map(&tv, a.vr, a, grid);
+  if (a.tma) {
+    int rc = ring_map(&tk, a.kr, a, B * a.Hkv);
+    if (!rc) rc = ring_map(&tv, a.vr, a, B * a.Hkv);
     if (rc) return rc;
   }
   static bool done[64] = {false};
@@ -574,7 +583,7 @@ int launch_swa_block(SwaBlockArgs& a, int grid, cudaStream_t st) {
   cudaGetDevice(&dev);
   if (dev < 64 && !done[dev]) {
     const int most = swa_smem(DP, QT, 64 * 1024 / (DP * 8), kMaxBlock, kWarps).total;
-    cudaError_t e = cudaFuncSetAttribute(swa_block_kernel<XT, DP, QT, N>,
+    cudaError_t e = cudaFuncSetAttribute(swa_block_kernel<DP, QT>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e != cudaSuccess) {
       set_error(std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
@@ -582,24 +591,59 @@ int launch_swa_block(SwaBlockArgs& a, int grid, cudaStream_t st) {
     }
     done[dev] = true;
   }
-  swa_block_kernel<XT, DP, QT, N>
-      <<<dim3(grid / a.Hkv, a.Hkv), 32 * warps, smem, st>>>(tk, tv, a);
-  count_launches(1);
-  return check_launch("swa_block_kernel");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(B, a.Hkv);
+  cfg.blockDim = dim3(32 * warps);
+  cfg.dynamicSmemBytes = swa_smem(DP, QT, a.part, a.T, warps).total;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return launched(cudaLaunchKernelEx(&cfg, swa_block_kernel<DP, QT>, tk, tv, a),
+                  "swa_block_kernel");
 }
 
+template <typename XT, int DP, int QT>
+int launch_swa_block(SwaBlockArgs& a, bool pairs, int B, cudaStream_t st) {
+  const int rows = ((a.T + 15) & ~15) + a.Tp, per = DP / 2 / (pairs ? 2 : 1);
+  const dim3 grid(ceil_div(rows * per, 256), a.Hkv, B);
+  if (pairs)
+    swa_rotate_kernel<XT, DP, QT, 2><<<grid, 256, 0, st>>>(a);
+  else
+    swa_rotate_kernel<XT, DP, QT, 1><<<grid, 256, 0, st>>>(a);
+  int rc = launched(cudaSuccess, "swa_rotate_kernel");
+  if (!rc && a.T) rc = launch_attend<DP, QT>(a, B, st);
+  return rc;
+}
+
+int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+int row_tiles(int R) { return R <= 16 ? 1 : 2; }
+
 template <typename XT>
-int pick_swa_block(SwaBlockArgs& a, bool pairs, int grid, cudaStream_t st) {
-  const bool one = a.rep * a.T <= 16;
-#define LZ_SB(DP_)                                                  \
-  return !pairs ? launch_swa_block<XT, DP_, 1, 1>(a, grid, st)      \
-         : one  ? launch_swa_block<XT, DP_, 1, 2>(a, grid, st)      \
-                : launch_swa_block<XT, DP_, 2, 2>(a, grid, st)
-  if (a.D <= 32) LZ_SB(32);
-  if (a.D <= 64) LZ_SB(64);
-  if (a.D <= 128) LZ_SB(128);
-  LZ_SB(256);
+int pick_swa_block(SwaBlockArgs& a, bool pairs, int B, cudaStream_t st) {
+  const bool one = row_tiles(a.rep * a.T) == 1;
+#define LZ_SB(DP_)                                              \
+  return one ? launch_swa_block<XT, DP_, 1>(a, pairs, B, st)    \
+             : launch_swa_block<XT, DP_, 2>(a, pairs, B, st)
+  switch (padded(a.D)) {
+    case 32:
+      LZ_SB(32);
+    case 64:
+      LZ_SB(64);
+    case 128:
+      LZ_SB(128);
+    default:
+      LZ_SB(256);
+  }
 #undef LZ_SB
+}
+
+size_t swa_bytes(int B, int H, int Hkv, int T, int D) {
+  if (!T) return 0;
+  const int R = H / Hkv * T;
+  return (size_t)B * Hkv * swa_work(padded(D), row_tiles(R), R, T).total;
 }
 
 }  // namespace
@@ -607,14 +651,21 @@ int swa_block_timeout_flag(unsigned int* out) { return tc::read_timeout_flag_her
 int swa_block_timeout_clear() { return tc::clear_timeout_flag_here(); }
 }  // namespace lz
 
+extern "C" size_t lz_swa_decode_block_workspace_bytes(int B, int H, int Hkv, int T, int D) {
+  if (B < 1 || H < 1 || Hkv < 1 || H % Hkv || T < 0 || T > lz::kMaxBlock || D < 2 || D > 256)
+    return 0;
+  return lz::swa_bytes(B, H, Hkv, T, D);
+}
+
 extern "C" int lz_swa_decode_block(const void* q, const void* k, const void* v, int x_dtype,
                                    const long long* strides, const void* cos, const void* sin,
                                    int cs_dtype, long long cs_sb, const void* k_prev,
                                    const void* v_prev, const long long* strides_prev,
                                    const void* cos_prev, const void* sin_prev, long long cs_prev_sb,
                                    const int* count, float* k_ring, float* v_ring, const int* pos,
-                                   const float* meta, int n_meta, void* y, int B, int H, int Hkv,
-                                   int T, int T_prev, int window, int D, void* stream) {
+                                   const float* meta, int n_meta, void* y, void* workspace,
+                                   size_t workspace_bytes, int B, int H, int Hkv, int T,
+                                   int T_prev, int window, int D, void* stream) {
   using namespace lz;
   clear_error();
   LZ_REQUIRE(B >= 1 && H >= 1 && Hkv >= 1 && D >= 2 && window >= 1 && T >= 0 && T_prev >= 0,
@@ -627,8 +678,8 @@ extern "C" int lz_swa_decode_block(const void* q, const void* k, const void* v, 
              "a block holds at most 64 tokens");
   LZ_REQUIRE(D <= 256 && window <= kMaxWindow, LZ_ERR_UNSUPPORTED,
              "decode supports D <= 256 and windows up to 1024");
-  LZ_REQUIRE((long long)B * Hkv < (1ll << 31) && Hkv <= 65535 && (long long)H / Hkv * T < (1ll << 24),
-             LZ_ERR_UNSUPPORTED, "too many heads");
+  LZ_REQUIRE(B <= 65535 && Hkv <= 65535 && (long long)H / Hkv * T < (1ll << 20),
+             LZ_ERR_UNSUPPORTED, "too many sequences or heads");
   LZ_REQUIRE(n_meta >= 0 && n_meta <= 32 && (n_meta == 0 || meta), LZ_ERR_INVALID_ARGUMENT,
              "meta must hold n_meta (<= 32) values");
   LZ_REQUIRE((x_dtype == LZ_DTYPE_F32 || x_dtype == LZ_DTYPE_BF16) &&
@@ -641,7 +692,12 @@ extern "C" int lz_swa_decode_block(const void* q, const void* k, const void* v, 
              LZ_ERR_INVALID_ARGUMENT, "null pointer in the previous block");
   LZ_REQUIRE(!T || (reinterpret_cast<uintptr_t>(y) & 3) == 0, LZ_ERR_INVALID_ARGUMENT,
              "y must be 4-byte aligned");
+  LZ_REQUIRE(!T || (workspace && workspace_bytes >= swa_bytes(B, H, Hkv, T, D)), LZ_ERR_WORKSPACE,
+             "workspace too small, see lz_swa_decode_block_workspace_bytes");
+  LZ_REQUIRE(!T || aligned16(workspace), LZ_ERR_INVALID_ARGUMENT,
+             "workspace must be 16-byte aligned");
   SwaBlockArgs a = {};
+  a.ws = static_cast<unsigned char*>(workspace);
   if (T) {
     a.q = {q, strides[0], strides[1], strides[2]};
     a.k = {k, strides[3], strides[4], strides[5]};
@@ -683,6 +739,6 @@ extern "C" int lz_swa_decode_block(const void* q, const void* k, const void* v, 
             even(a.q, xs) && even(a.k, xs) && even(a.v, xs) && even(a.kp, xs) &&
             even(a.vp, xs) && even_r(a.rot) && even_r(a.rot_p);
   auto st = static_cast<cudaStream_t>(stream);
-  return x_dtype == LZ_DTYPE_F32 ? pick_swa_block<float>(a, pairs, B * Hkv, st)
-                                 : pick_swa_block<bf16>(a, pairs, B * Hkv, st);
+  return x_dtype == LZ_DTYPE_F32 ? pick_swa_block<float>(a, pairs, B, st)
+                                 : pick_swa_block<bf16>(a, pairs, B, st);
 }

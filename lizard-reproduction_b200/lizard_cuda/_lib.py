@@ -85,8 +85,9 @@ _SIGNATURES = {
                                                                      _vp] + [_c_int] * 5 + [_vp]),
     "lz_gla_decode_block": (_c_int, [_vp] * 4 + [_c_int] + [_vp] * 7 + [_c_int] * 8 + [_vp]),
     "lz_swa_decode_block": (_c_int, [_vp] * 3 + [_c_int] + [_vp] * 3 + [_c_int, _c_ll]
-                            + [_vp] * 5 + [_c_ll] + [_vp] * 5 + [_c_int, _vp] + [_c_int] * 7
-                            + [_vp]),
+                            + [_vp] * 5 + [_c_ll] + [_vp] * 5 + [_c_int, _vp, _vp, _c_size]
+                            + [_c_int] * 7 + [_vp]),
+    "lz_swa_decode_block_workspace_bytes": (_c_size, [_c_int] * 5),
     "lz_verify_drafts_workspace_bytes": (_c_size, [_c_int] * 3),
     "lz_verify_drafts": (_c_int, [_vp, _c_ll, _c_ll, _vp, _c_ll, _c_ll, _c_int, _vp, _c_int, _vp,
                                   _vp, _c_ll, _vp, ctypes.c_float, _vp, _vp, _vp, _vp, _c_size]

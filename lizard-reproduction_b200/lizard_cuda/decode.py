@@ -273,11 +273,14 @@ def swa_decode_block(q, k, v, cos, sin, meta, k_ring, v_ring, pos, pending=None)
     st = _lib.longlongs(9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
     meta32, pos = _lib.as_dtype(meta, torch.float32), pos.contiguous()
     p = _lib.ptr if Tp else (lambda t: None)
+    size = _lib.size_query("lz_swa_decode_block_workspace_bytes", B, H, Hkv, T, D)
+    ws = torch.empty(size, device=q.device, dtype=torch.uint8)
     rc = _lib.call(
         index, _lib.load().lz_swa_decode_block, q.data_ptr(), k.data_ptr(), v.data_ptr(),
         _DT[xdt], st, cos.data_ptr(), sin.data_ptr(), _DT[cdt], cs_sb, p(kp), p(vp), stp, p(cp),
         p(sp), cp_sb, _lib.ptr(count), k_ring.data_ptr(), v_ring.data_ptr(), pos.data_ptr(),
-        meta32.data_ptr() or None, meta32.numel(), y.data_ptr(), B, H, Hkv, T, Tp, W, D,
+        meta32.data_ptr() or None, meta32.numel(), y.data_ptr(), ws.data_ptr(), size, B, H, Hkv,
+        T, Tp, W, D,
         _lib.stream_of(q))
     if rc:
         _lib.check(rc, "swa decode block")
@@ -292,6 +295,44 @@ class LayerCache:
     k_ring: torch.Tensor  # fp32 [B, Hkv, W, D], rotated keys
     v_ring: torch.Tensor  # fp32 [B, Hkv, W, D]
     pos: torch.Tensor     # int32 [B], tokens seen
+    # the last block of drafted decoding, not folded in yet: (fk, v, log_gamma) of the
+    # GLA branch and (k, v, cos, sin) of the SWA branch
+    pending: tuple = None
+
+    def block(self, fq, fk, v, log_gamma, q, k, cos, sin, meta, accepted):
+        """Both branches' outputs for a block of new tokens, after the first
+        accepted[b] tokens (int32 [B]) of the block before have been folded in; the
+        block becomes the pending one."""
+        gla_p = swa_p = None
+        if self.pending is not None:
+            if accepted is None:
+                raise ValueError("a block is pending: accepted (int32 [B]) says how much of it "
+                                 "stands")
+            gla_p, swa_p = ((*p, accepted) for p in self.pending)
+        v16 = _lib.as_dtype(v, torch.bfloat16)
+        y_gla = gla_decode_block(fq, fk, v16, log_gamma, self.state, self.zstate, gla_p)
+        y_swa = swa_decode_block(q, k, v, cos, sin, meta, self.k_ring, self.v_ring, self.pos,
+                                 swa_p)
+        if self.pending is not None:
+            self.pos += accepted
+        self.pending = (fk, v16, log_gamma), (k, v, cos, sin)
+        return y_gla, y_swa
+
+    def settle(self, accepted):
+        """Fold the first accepted[b] tokens of the pending block in and forget the rest."""
+        if self.pending is None:
+            return
+        if accepted is None:
+            raise ValueError("accepted (int32 [B]) says how much of the pending block stands")
+        (fk, v, lg), (k, v_, cos, sin) = self.pending
+        H = lg.shape[1] if lg.dim() == 3 else fk.shape[1]
+        fq, q = fk.new_empty(fk.shape[0], H, 0, fk.shape[3]), k[:, :, :0]
+        gla_decode_block(fq, fk[:, :, :0], v[:, :, :0], lg[..., :0], self.state, self.zstate,
+                         (fk, v, lg, accepted))
+        swa_decode_block(q, q, v_[:, :, :0], cos[:, :0], sin[:, :0], cos.new_empty(0),
+                         self.k_ring, self.v_ring, self.pos, (k, v_, cos, sin, accepted))
+        self.pos += accepted
+        self.pending = None
 
 
 class LizardCache(dict):
@@ -299,4 +340,23 @@ class LizardCache(dict):
     attention layers are lizard_cuda LizardAttention: the first call with a
     layer's index missing runs the full forward over the prompt and stores the
     layer's state; later calls decode their tokens one at a time. Position ids
-    of the new tokens must be given to the model (position_ids=)."""
+    of the new tokens must be given to the model (position_ids=).
+
+    Drafted decoding: after draft(accepted) a call takes its tokens (up to 64) as
+    one block that can be taken back. It first folds in the first accepted[b]
+    tokens (int32 [B]) of the block before, and leaves its own to the next call;
+    settle(accepted) folds them in and returns to token-by-token decoding."""
+
+    drafting = False
+    accepted = None
+
+    def draft(self, accepted=None):
+        """The next call's tokens are a block; accepted tokens of the block before (all
+        rows 0 when there is none to keep)."""
+        self.drafting, self.accepted = True, accepted
+        return self
+
+    def settle(self, accepted):
+        for layer in self.values():
+            layer.settle(accepted)
+        self.drafting, self.accepted = False, None

@@ -106,15 +106,19 @@ class LizardAttention(nn.Module):
                 **kwargs):
         """(out, None) as the reference layer. With `lizard_cache` (a
         decode.LizardCache), a layer whose index is in the cache decodes its
-        tokens one at a time against the stored state; otherwise it runs the
+        tokens against the stored state, one at a time or (a drafting cache) as one
+        block that the next call keeps a prefix of; otherwise it runs the
         full forward and, given a cache, stores its state there. With
         `seq_comm` (a seqpar.DistExchange, or any object with rank, size and
         all_gather) hidden_states is this rank's slice of the sequence."""
         if seq_comm is not None and lizard_cache is not None:
             raise ValueError("a sequence-parallel forward does not fill a decode cache")
         if lizard_cache is not None and self.layer_idx in lizard_cache:
-            return self.decode(hidden_states, position_embeddings,
-                               lizard_cache[self.layer_idx]), None
+            layer_cache = lizard_cache[self.layer_idx]
+            if lizard_cache.drafting:
+                return self.decode_block(hidden_states, position_embeddings, layer_cache,
+                                         lizard_cache.accepted), None
+            return self.decode(hidden_states, position_embeddings, layer_cache), None
         x = hidden_states
         dtype = torch.promote_types(x.dtype, torch.float32)
         up = torch.is_grad_enabled()
@@ -190,6 +194,27 @@ class LizardAttention(nn.Module):
             y_gla, y_swa = y_gla[0].unsqueeze(2), y_swa[0].unsqueeze(2)
         else:
             y_gla, y_swa = torch.stack(y_gla, 2), torch.stack(y_swa, 2)
+        y = blend(y_gla, y_swa, self.param_as(self.alpha_blend, dtype), x.dtype)
+        return self.o_proj(y)
+
+
+    @torch.no_grad()
+    def decode_block(self, hidden_states, position_embeddings, cache, accepted):
+        """Output for a block of T <= 64 new tokens [B, T, hidden] that follow the tokens
+        in `cache` and the first accepted[b] (int32 [B]) of its pending block, which are
+        folded in; this block becomes the pending one. The values are decode's for the
+        same tokens, in one pass over the state and the ring."""
+        x = hidden_states
+        dtype = torch.promote_types(x.dtype, torch.float32)
+        q = self.heads_view(self.q_proj(x), self.heads)
+        k = self.heads_view(self.k_proj(x), self.kv_heads)
+        v = self.heads_view(self.v_proj(x), self.kv_heads)
+        lg = F.logsigmoid(self.W_gamma(x).to(dtype).squeeze(-1))
+        fq = fused_hedgehog(q, self.param_as(self.phi_q.weight, dtype))
+        fk = fused_hedgehog(k, self.param_as(self.phi_k.weight, dtype))
+        cos, sin = position_embeddings
+        meta = self.param_as(self.meta_tokens, dtype)
+        y_gla, y_swa = cache.block(fq, fk, v, lg, q, k, cos, sin, meta, accepted)
         y = blend(y_gla, y_swa, self.param_as(self.alpha_blend, dtype), x.dtype)
         return self.o_proj(y)
 

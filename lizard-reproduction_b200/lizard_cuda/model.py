@@ -17,11 +17,19 @@ greedy_generate(model, input_ids, steps) decodes with the recurrent cache
 step at O(1) cost per layer (the reference has no cache and would recompute
 the whole sequence for every new token); GraphedDecoder replays a captured
 decode step as one CUDA graph launch.
+
+speculative_generate(model, draft, input_ids, steps) gets several tokens out of a
+pass over the model's weights: a cheaper draft model proposes tokens, the model
+runs them as one block against its cache and keeps the prefix that its own
+probabilities accept. to_int8(model) makes such a draft of a copy of the model.
 """
 import torch
+import torch.nn as nn
 
 from .decode import LizardCache
+from .int8 import Int8Linear
 from .layer import LizardAttention, from_llama  # noqa: F401
+from .verify import verify_drafts
 from . import _lib
 
 OPTIONS = ("window", "num_meta", "feature_dim", "backend")
@@ -112,3 +120,82 @@ def greedy_generate(model, input_ids, steps, graph=False):
         tokens.append(logits[:, -1].argmax(-1, keepdim=True))
         pos = pos + 1
     return torch.cat(tokens, 1), cache
+
+
+INT8_LAYERS = ("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj",
+               "lm_head")
+
+
+@torch.no_grad()
+def to_int8(model, names=INT8_LAYERS):
+    """Replace the model's linear layers of these names by Int8Linear in place
+    (weights as 8-bit codes with a scale a channel, inputs quantised token by token)
+    and return the model: half the weight bytes of bf16, for inference on the GPU.
+    The small layers (feature maps, gate) keep their weights."""
+    for module in model.modules():
+        for name, child in module.named_children():
+            if name in names and isinstance(child, nn.Linear):
+                setattr(module, name, Int8Linear(child))
+    return model
+
+
+def _draw(logits, temperature, generator):
+    """One token a row of logits [B, V]: argmax at temperature 0, else by their probabilities."""
+    B, V = logits.shape
+    noise = torch.empty(B, V, device=logits.device).exponential_(generator=generator)
+    none = logits.new_empty(B, 0, V)
+    return verify_drafts(logits[:, None], none, torch.empty(B, 0, device=logits.device,
+                                                            dtype=torch.long),
+                         noise[:, :0], noise, temperature)[0]
+
+
+@torch.no_grad()
+def speculative_generate(model, draft, input_ids, steps, draft_len=4, temperature=0.0,
+                         generator=None):
+    """Continuation of input_ids [B, L] by `steps` tokens with drafted decoding: the
+    draft model proposes draft_len tokens a round, the model checks them in one
+    block and adds one of its own. At temperature 0 the tokens are the model's greedy
+    ones; otherwise they follow the model's probabilities at that temperature,
+    whatever the draft. Both models are Lizard models with the same vocabulary.
+    Returns the tokens [B, steps], the model's cache, settled on the tokens before
+    the last one it emitted (a row may run a few tokens past `steps`), and how many
+    rounds it took."""
+    dev, (B, L) = input_ids.device, input_ids.shape
+    K = draft_len
+    if not 1 <= K <= 63:
+        raise ValueError(f"draft_len must be 1 .. 63, got {draft_len}")
+    cache, draft_cache = LizardCache(), LizardCache()
+    logits = model(input_ids, lizard_cache=cache, use_cache=False, logits_to_keep=1).logits
+    draft(input_ids, lizard_cache=draft_cache, use_cache=False, logits_to_keep=1)
+    last = _draw(logits[:, -1], temperature, generator)
+    out = torch.zeros(B, steps + K + 1, device=dev, dtype=torch.long)
+    out[:, :1] = last
+    have = torch.ones(B, 1, device=dev, dtype=torch.long)
+    pos = torch.full((B, 1), L, device=dev, dtype=torch.long)  # of `last`
+    none = torch.zeros(B, device=dev, dtype=torch.int32)
+    stand, step, rounds = none, torch.arange(K + 1, device=dev), 0
+    while int(have.min()) < steps:
+        block, proposals = last, []
+        for i in range(K):
+            proposals.append(draft(block, position_ids=pos + step[:i + 1], use_cache=False,
+                                   lizard_cache=draft_cache.draft(stand if i == 0 else none),
+                                   logits_to_keep=1).logits[:, -1].to(logits.dtype))
+            block = torch.cat([block, _draw(proposals[-1], temperature, generator)], 1)
+        # the draft's own pass over the whole block, so that its cache can keep any prefix
+        draft(block, position_ids=pos + step, lizard_cache=draft_cache.draft(none),
+              use_cache=False, logits_to_keep=1)
+        logits = model(block, position_ids=pos + step, lizard_cache=cache.draft(stand),
+                       use_cache=False).logits
+        uniforms = torch.rand(B, K, device=dev, generator=generator)
+        noise = torch.empty(B, logits.shape[-1], device=dev).exponential_(generator=generator)
+        tokens, accepted = verify_drafts(logits, torch.stack(proposals, 1), block[:, 1:], uniforms,
+                                         noise, temperature)
+        # rows that are done write their further tokens into the spare columns
+        at = torch.minimum(have + step, torch.full_like(have, steps + K))
+        new = step <= accepted[:, None]
+        out.scatter_(1, at, torch.where(new, tokens, out.gather(1, at)))
+        last = tokens.gather(1, accepted[:, None].long())
+        stand = accepted + 1  # the block's first token stands in any case
+        have, pos, rounds = have + stand[:, None], pos + stand[:, None], rounds + 1
+    cache.settle(stand)
+    return out[:, :steps], cache, rounds
