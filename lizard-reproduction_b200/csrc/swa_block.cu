@@ -280,8 +280,7 @@ swa_block_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__
   float* sNK = reinterpret_cast<float*>(sm + o.nk);
   float* sNV = reinterpret_cast<float*>(sm + o.nv);
   float* sO = reinterpret_cast<float*>(sm);             // [warp][16][LO], after the last key
-  bf16* sQh = reinterpret_cast<bf16*>(sm + o.q);        // [RQ][LQ]
-  bf16* sQl = sQh + RQ * LQ;
+  bf16* sQh = reinterpret_cast<bf16*>(sm + o.q);        // [hi | lo][RQ][LQ]
   float* sMax = reinterpret_cast<float*>(sm + o.stat);  // [warp][16]
   float* sSum = sMax + nw * 16;
   float* sCof = sSum + nw * 16;
@@ -331,17 +330,25 @@ swa_block_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__
     tc::prefetch_tmap(&tk);
     tc::prefetch_tmap(&tv);
   }
+  // the sinks of lane16 and lane16 + 16, in the exponent's base
+  const int lane16 = tid & 15;
+  const float sink0 = lane16 < a.n_meta ? a.meta[lane16] * kLog2e : -INFINITY;
+  const float sink1 = lane16 + 16 < a.n_meta ? a.meta[lane16 + 16] * kLog2e : -INFINITY;
   asm volatile("griddepcontrol.wait;\n" ::: "memory");  // the ring and the workspace are written
-  asm volatile("fence.proxy.async;\n" ::: "memory");
+  if (tid == 0) asm volatile("fence.proxy.async;\n" ::: "memory");
   load(0, 0);
   __syncthreads();  // the barrier is initialised
 
   const int nr = (int)min((long long)pos + n, (long long)W);  // ring rows that hold a token
   const int last = (pos % W + n - 1 + W) % W;                 // slot of the newest (W >= 1)
   const float scale = rsqrtf((float)D) * kLog2e;
-  const int krow = key_row(g), eight = 8 % T;
+  const int krow = key_row(g), vrow0 = key_row(2 * j), vrow1 = key_row(2 * j + 1);
+  const int eight = 8 % T;
   const int rt = QT == 1 ? 0 : warp % QT;                     // this warp's row tile
   const int kw = QT == 1 ? warp : warp / QT, kws = nw / QT;   // and its turn among the keys
+  // ldmatrix rows of this lane's queries, hi and lo
+  const uint32_t aqh = smem_u32(sQh) + (rt * 16 + (lane & 15)) * (LQ * 2) + (lane >> 4) * 16;
+  const uint32_t aql = aqh + RQ * LQ * 2;
   bool live = true;  // after a timeout nothing is written
 
   for (int r0 = 0; r0 < R; r0 += RQ) {
@@ -377,55 +384,69 @@ swa_block_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__
       for (int tl = kw; tl < tiles; tl += kws) {
         const bool own = tl >= ring_tiles;
         const int rows = own ? TN : part, row0 = (own ? tl - ring_tiles : tl) * 16;
-        const float* kt = own ? sNK : sK;
+        const int lim = own ? T : held;  // rows beyond hold nothing (perhaps not numbers)
+        // this lane's places: key row krow, value rows of keys 2j and 2j + 1 (8 rows on
+        // and 16 columns on keep the swizzle's row and flip one bit of its chunk)
+        const float* kg = (own ? sNK : sK) + (row0 + krow) * 32;
+        const float *k0 = kg + ((j ^ krow) << 2), *k1 = kg + (((4 + j) ^ krow) << 2);
         const float* vt = own ? sNV : sV;
-        // scores of 16 keys
-        float sc[2][4];
+        const float* v0 = vt + (row0 + vrow0) * 32 + ((g ^ vrow0) << 2);
+        const float* v1 = vt + (row0 + vrow1) * 32 + ((g ^ vrow1) << 2);
+        // scores of 16 keys: hi hi, and the cross products in sums of their own (the
+        // chain of dependent products is what a warp waits for here)
+        float sc[2][4], sx[2][4];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) sc[i][c] = 0.f;
-        const float* kg = kt + (row0 + krow) * 32;
+          for (int c = 0; c < 4; ++c) sc[i][c] = sx[i][c] = 0.f;
 #pragma unroll
         for (int ks = 0; ks < NS; ++ks) {
           uint32_t qh[4], ql[4];
-          lda_rm(qh, sQh, LQ, rt * 16, ks * 16);
-          lda_rm(ql, sQl, LQ, rt * 16, ks * 16);
+          ldsm_x4(qh, aqh + ks * 32);
+          ldsm_x4(ql, aql + ks * 32);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float4 x = *reinterpret_cast<const float4*>(
-                kg + ((ks >> 1) * rows + 8 * i) * 32 + ((((ks & 1) * 4 + j) ^ krow) << 2));
+            const float4 x = *reinterpret_cast<const float4*>((ks & 1 ? k1 : k0) + 256 * i);
             uint32_t kh[2], kl[2];
             split2(x.x, x.y, kh[0], kl[0]);
             split2(x.z, x.w, kh[1], kl[1]);
             mma16816(sc[i], qh, kh[0], kh[1]);
-            mma16816(sc[i], qh, kl[0], kl[1]);
-            mma16816(sc[i], ql, kh[0], kh[1]);
+            mma16816(sx[i], qh, kl[0], kl[1]);
+            mma16816(sx[i], ql, kh[0], kh[1]);
           }
+          if (ks & 1) k0 += rows * 32, k1 += rows * 32;
         }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) sc[i][c] += sx[i][c];
         // position - base of this thread's keys 8 i + 2 j + c; a ring slot holds the
         // last position before base that falls on it
         int rel[4];
+        bool clear = true;  // every row of the tile sees every key
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int k = row0 + (i >> 1) * 8 + key_row(2 * j + (i & 1));
+          const int k = row0 + (i >> 1) * 8 + (i & 1 ? vrow1 : vrow0);
           const int back = last - (p * part + k);
-          rel[i] = own ? (k < T ? k : 1 << 30)
-                       : (k < held ? -1 - (back < 0 ? back + W : back) : 1 << 30);
+          rel[i] = own ? k : -1 - (back < 0 ? back + W : back);
+          if (k >= lim) rel[i] = 1 << 30;
+          clear = clear && rel[i] < 0 && rel[i] >= T - W;
+        }
+        if (!__all_sync(0xffffffffu, clear)) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (rel[i] > tq[h] || rel[i] <= tq[h] - W) sc[i >> 1][2 * h + (i & 1)] = -INFINITY;
         }
         uint32_t ph[4], pl[4];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int t = tq[h];
-          float mx = m[h];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float& x = sc[i >> 1][2 * h + (i & 1)];
-            x = rel[i] <= t && rel[i] > t - W ? x * scale : -INFINITY;
-            mx = fmaxf(mx, x);
-          }
+          float mx = fmaxf(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]),
+                           fmaxf(sc[1][2 * h], sc[1][2 * h + 1]));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          mx = fmaxf(mx * scale, m[h]);
           if (tl != kw || p) {  // not the first keys: rescale
             const float f = tc::ex2(m[h] - mx);
             l[h] *= f;
@@ -438,22 +459,25 @@ swa_block_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__
           m[h] = mx;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float x0 = tc::ex2(sc[i][2 * h] - mx), x1 = tc::ex2(sc[i][2 * h + 1] - mx);
+            const float x0 = tc::ex2(fmaf(sc[i][2 * h], scale, -mx));
+            const float x1 = tc::ex2(fmaf(sc[i][2 * h + 1], scale, -mx));
             l[h] += x0 + x1;
             split2(x0, x1, ph[2 * i + h], pl[2 * i + h]);
           }
         }
         // values: rows of keys 2j, 2j + 1, 2j + 8, 2j + 9, columns 4 g .. 4 g + 3 of each 32
-        const int va = row0 + key_row(2 * j), vb = row0 + key_row(2 * j + 1);
-        const int lim = own ? T : held;  // rows beyond hold nothing (perhaps not numbers)
 #pragma unroll
         for (int q = 0; q < NG; ++q) {
           float4 x[4];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int r = (u & 1 ? vb : va) + (u >> 1) * 8;
-            x[u] = *reinterpret_cast<const float4*>(vt + (q * rows + r) * 32 + ((g ^ (r & 7)) << 2));
-            if (r >= lim) x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int u = 0; u < 4; ++u)
+            x[u] = *reinterpret_cast<const float4*>((u & 1 ? v1 : v0) + 256 * (u >> 1));
+          v0 += rows * 32, v1 += rows * 32;
+          if (row0 + 16 > lim) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              if (row0 + (u & 1 ? vrow1 : vrow0) + (u >> 1) * 8 >= lim)
+                x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -481,18 +505,15 @@ swa_block_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__
       }
     }
     __syncthreads();
-    const int lane16 = tid & 15;
     for (int e = tid >> 4; e < RQ; e += nt >> 4) {  // a row a half warp, a lane a warp of its tile
       const int w = (lane16 * QT + (e >> 4)), at = w * 16 + (e & 15);
       const bool in = lane16 < kws;
       const float mw = in ? sMax[at] : -1e30f;
-      float top = mw;
-      for (int i = lane16; i < a.n_meta; i += 16) top = fmaxf(top, a.meta[i] * kLog2e);
+      float top = fmaxf(mw, fmaxf(sink0, sink1));
 #pragma unroll
       for (int x = 1; x < 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
       const float f = tc::ex2(mw - top);
-      float sum = in ? f * sSum[at] : 0.f;
-      for (int i = lane16; i < a.n_meta; i += 16) sum += tc::ex2(a.meta[i] * kLog2e - top);
+      float sum = (in ? f * sSum[at] : 0.f) + tc::ex2(sink0 - top) + tc::ex2(sink1 - top);
 #pragma unroll
       for (int x = 1; x < 16; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
       if (in) sCof[at] = f / sum;
