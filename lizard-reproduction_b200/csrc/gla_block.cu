@@ -189,13 +189,7 @@ gla_block_kernel(const __grid_constant__ CUtensorMap ts, const GlaBlockArgs a) {
 #pragma unroll
     for (int h = 0; h < HALVES; ++h) tc::tma_load_3d(sm + h * tile, &ts, d0 + 32 * h, 0, sidx, bar);
   }
-  const bf16* fq = a.fq + (size_t)(b * a.H + s * rep) * T * F;
-  if (T) {
-    stage_rows(sK, LD, FP, F, a.fk + (size_t)kvh * T * F, T, F, TK, NT);
-    stage_rows(sQ, LD, FP, F, fq, min(R, kQRows), F, kQRows, NT);
-    stage_rows(sV, LV, DN, D, a.v + (size_t)kvh * T * D + d0, T, D - d0, TK, NT);
-    cp_async_commit();
-  }
+  // small loads: they arrive while the rest is staged
   const size_t grow = a.gph ? (size_t)b * a.H + s : (size_t)b;
   // lane r of every warp holds the gates of tokens r and r + 32
   const float lg0 = lane < T ? a.lg[grow * T + lane] : 0.f;
@@ -227,6 +221,13 @@ gla_block_kernel(const __grid_constant__ CUtensorMap ts, const GlaBlockArgs a) {
     }
   };
   fetch(0);
+  const bf16* fq = a.fq + (size_t)(b * a.H + s * rep) * T * F;
+  if (T) {
+    stage_rows(sK, LD, FP, F, a.fk + (size_t)kvh * T * F, T, F, TK, NT);
+    stage_rows(sQ, LD, FP, F, fq, min(R, kQRows), F, kQRows, NT);
+    stage_rows(sV, LV, DN, D, a.v + (size_t)kvh * T * D + d0, T, D - d0, TK, NT);
+    cp_async_commit();
+  }
   // decays: M of the block (a warp a token), w of the pending tokens (every warp)
   for (int t = warp; t < T; t += NT / 32) {
     float e0 = lane <= t ? lg0 : 0.f, e1 = lane + 32 <= t ? lg1 : 0.f;
