@@ -527,8 +527,8 @@ int lz_gla_decode_block(const void* fq, const void* fk, const void* v,
  * count[b] and on, to the ring and to the block's earlier tokens, with the
  * sink logits. pos[b] counts the tokens the rings hold before the call; the
  * caller advances it by count[b]. q, k, v (k_prev, v_prev) are read in place:
- * strides = {batch, head, token} in elements for q, k, v in turn (9 values;
- * strides_prev 6), host memory, last dimension contiguous; cos, sin [T, D] per
+ * strides = {batch, head, token, column} in elements for q, k, v in turn (12
+ * values; strides_prev 8), host memory, the column's 1; cos, sin [T, D] per
  * batch row, cs_sb elements apart (0: one table for all). Rings fp32
  * [B*Hkv, window, D], D even up to 256, window up to 1024. The workspace (16-byte
  * aligned, lz_swa_decode_block_workspace_bytes; 0 for T = 0) holds the rotated block. */

@@ -721,12 +721,16 @@ extern "C" int lz_swa_decode_block(const void* q, const void* k, const void* v, 
   a.ws = static_cast<unsigned char*>(workspace);
   if (T) {
     a.q = {q, strides[0], strides[1], strides[2]};
-    a.k = {k, strides[3], strides[4], strides[5]};
-    a.v = {v, strides[6], strides[7], strides[8]};
+    a.k = {k, strides[4], strides[5], strides[6]};
+    a.v = {v, strides[8], strides[9], strides[10]};
+    LZ_REQUIRE(strides[3] == 1 && strides[7] == 1 && strides[11] == 1, LZ_ERR_INVALID_ARGUMENT,
+               "the last dimension must be contiguous");
   }
   if (T_prev) {
     a.kp = {k_prev, strides_prev[0], strides_prev[1], strides_prev[2]};
-    a.vp = {v_prev, strides_prev[3], strides_prev[4], strides_prev[5]};
+    a.vp = {v_prev, strides_prev[4], strides_prev[5], strides_prev[6]};
+    LZ_REQUIRE(strides_prev[3] == 1 && strides_prev[7] == 1, LZ_ERR_INVALID_ARGUMENT,
+               "the last dimension must be contiguous");
   }
   const int cb = cs_dtype == LZ_DTYPE_BF16;
   a.rot = {cos, sin, cs_sb, cb};

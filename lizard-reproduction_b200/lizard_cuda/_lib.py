@@ -6,7 +6,6 @@ every call raises.
 """
 import contextlib
 import ctypes
-import functools
 import threading
 from pathlib import Path
 
@@ -200,16 +199,14 @@ def ptr(t):
     return None if t is None else t.data_ptr()
 
 
-@functools.lru_cache(None)
-def longlongs(n):
-    """The ctypes array type of n 64-bit integers (host arguments of strides)."""
-    return ctypes.c_longlong * n
+def raw_stream(index):
+    """The current stream of device `index` as an address (without building a Stream
+    object, which costs more than a small launch)."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def stream_of(t):
-    """The current stream of t's device as an address (without building a Stream object,
-    which costs more than a small launch)."""
-    return torch._C._cuda_getCurrentRawStream(t.get_device())
+    return raw_stream(t.get_device())
 
 
 def call(index, fn, *args):
@@ -218,18 +215,6 @@ def call(index, fn, *args):
         return fn(*args)
     with torch.cuda.device(index):
         return fn(*args)
-
-
-def same_device(first, *rest):
-    """Whether every tensor is on the CUDA device of the first (require_cuda names the one
-    that is not)."""
-    i = first.get_device()
-    if i < 0:
-        return False
-    for t in rest:
-        if t.get_device() != i:
-            return False
-    return True
 
 
 def as_dtype(t, dtype):

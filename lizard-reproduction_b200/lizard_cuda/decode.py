@@ -14,6 +14,7 @@ With a gate shared by the heads (log_gamma [B, L], the layer's case) and
 grouped keys / values, the H / Hkv query heads of a group read the same state,
 so the cache keeps Hkv states per batch row.
 """
+import struct
 from dataclasses import dataclass
 
 import torch
@@ -152,13 +153,14 @@ def gla_decode_block(fq, fk, v, log_gamma, state, zstate, pending=None):
     which first advances state and zstate (fp32 [B, Hs, F, D] and [B, Hs, F], in
     place) by the first count[b] (int32 [B], None = all) of its tokens.
     T = 0 (empty fq, fk, v, log_gamma) only advances the state."""
-    given = (fq, fk, v, log_gamma, state, zstate)
-    if not _lib.same_device(*given):
-        _lib.require_cuda(*given)
+    index = fq.get_device()
+    if not (index == fk.get_device() == v.get_device() == log_gamma.get_device()
+            == state.get_device() == zstate.get_device() >= 0):
+        _lib.require_cuda(fq, fk, v, log_gamma, state, zstate)
     if fq.dim() != 4 or fk.dim() != 4 or v.dim() != 4 or state.dim() != 4:
         raise ValueError("fq, fk, v must be [B, heads, T, dim] and state [B, Hs, F, D]")
     B, H, T, F = fq.shape
-    Hkv, D, Hs, index = fk.shape[1], v.shape[3], state.shape[1], fq.get_device()
+    Hkv, D, Hs = fk.shape[1], v.shape[3], state.shape[1]
     if fk.shape != (B, Hkv, T, F) or v.shape != (B, Hkv, T, D):
         raise ValueError(f"fk and v must be [B, Hkv, T, F] and [B, Hkv, T, D] matching fq "
                          f"{tuple(fq.shape)}, got {tuple(fk.shape)}, {tuple(v.shape)}")
@@ -171,11 +173,10 @@ def gla_decode_block(fq, fk, v, log_gamma, state, zstate, pending=None):
     per_head = 1 if log_gamma.dim() == 3 else 0
     if log_gamma.shape != ((B, H, T) if per_head else (B, T)):
         raise ValueError(f"log_gamma must be [B, T] or [B, H, T], got {tuple(log_gamma.shape)}")
-    fkp = vp = lgp = count = None
-    Tp = 0
+    Tp = p_fk = p_v = p_lg = p_count = 0
     if pending is not None:
         fkp, vp, lgp, count = pending
-        if not _lib.same_device(fq, fkp, vp, lgp):
+        if not index == fkp.get_device() == vp.get_device() == lgp.get_device():
             _lib.require_cuda(fq, fkp, vp, lgp)
         Tp = fkp.shape[2]
         if fkp.shape != (B, Hkv, Tp, F) or vp.shape != (B, Hkv, Tp, D):
@@ -184,19 +185,21 @@ def gla_decode_block(fq, fk, v, log_gamma, state, zstate, pending=None):
         if lgp.shape != ((B, H, Tp) if per_head else (B, Tp)):
             raise ValueError(f"pending log_gamma must have log_gamma's layout, got "
                              f"{tuple(lgp.shape)}")
-        count = _pending_count(count, B, index)
         fkp, vp = _lib.as_dtype(fkp, torch.bfloat16), _lib.as_dtype(vp, torch.bfloat16)
         lgp = _lib.as_dtype(lgp, torch.float32)
-    y = torch.empty((B, H, T, D), device=fq.device, dtype=torch.bfloat16)
+        p_fk, p_v, p_lg = fkp.data_ptr(), vp.data_ptr(), lgp.data_ptr()
+        if count is not None:
+            count = _pending_count(count, B, index)
+            p_count = count.data_ptr()
+    y = fq.new_empty((B, H, T, D), dtype=torch.bfloat16)
     if B == 0 or T == 0 and Tp == 0:
         return y
-    fq, fk, v = (_lib.as_dtype(t, torch.bfloat16) for t in (fq, fk, v))
-    lg = _lib.as_dtype(log_gamma, torch.float32)
+    fq, fk = _lib.as_dtype(fq, torch.bfloat16), _lib.as_dtype(fk, torch.bfloat16)
+    v, lg = _lib.as_dtype(v, torch.bfloat16), _lib.as_dtype(log_gamma, torch.float32)
     rc = _lib.call(
         index, _lib.load().lz_gla_decode_block, fq.data_ptr(), fk.data_ptr(), v.data_ptr(),
-        lg.data_ptr(), per_head, _lib.ptr(fkp), _lib.ptr(vp), _lib.ptr(lgp), _lib.ptr(count),
-        state.data_ptr(), zstate.data_ptr(), y.data_ptr(), B, H, Hkv, Hs, T, Tp, F, D,
-        _lib.stream_of(fq))
+        lg.data_ptr(), per_head, p_fk, p_v, p_lg, p_count, state.data_ptr(), zstate.data_ptr(),
+        y.data_ptr(), B, H, Hkv, Hs, T, Tp, F, D, _lib.raw_stream(index))
     if rc:
         _lib.check(rc, "gla decode block")
     return y
@@ -220,6 +223,9 @@ def _rows(t, dtype):
     return t if t.stride(3) == 1 else t.contiguous()
 
 
+_strides3, _strides2 = struct.Struct("12q").pack, struct.Struct("8q").pack
+
+
 def swa_decode_block(q, k, v, cos, sin, meta, k_ring, v_ring, pos, pending=None):
     """A block of T <= 64 new tokens against the rings, for drafted decoding:
     q [B, H, T, D], k, v [B, Hkv, T, D] (unrotated; strided views with a
@@ -231,57 +237,60 @@ def swa_decode_block(q, k, v, cos, sin, meta, k_ring, v_ring, pos, pending=None)
     [B], None = all) of its tokens to slots (pos[b] + t) % W. pos counts the
     tokens the rings hold before the call, without the pending ones; the caller
     then advances it by count. T = 0 only advances the rings."""
-    given = (q, k, v, cos, sin, meta, k_ring, v_ring, pos)
-    if not _lib.same_device(*given):
-        _lib.require_cuda(*given)
+    index = q.get_device()
+    if not (index == k.get_device() == v.get_device() == cos.get_device() == sin.get_device()
+            == meta.get_device() == k_ring.get_device() == v_ring.get_device()
+            == pos.get_device() >= 0):
+        _lib.require_cuda(q, k, v, cos, sin, meta, k_ring, v_ring, pos)
     if q.dim() != 4 or k.dim() != 4 or k_ring.dim() != 4:
         raise ValueError("q, k, v must be [B, heads, T, D] and the rings [B, Hkv, W, D]")
     B, H, T, D = q.shape
-    Hkv, W, index = k.shape[1], k_ring.shape[2], q.get_device()
+    Hkv, W = k.shape[1], k_ring.shape[2]
     if k.shape != (B, Hkv, T, D) or v.shape != k.shape:
         raise ValueError(f"k and v must be [B, Hkv, T, D] matching q {tuple(q.shape)}, got "
                          f"{tuple(k.shape)}, {tuple(v.shape)}")
-    for ring in (k_ring, v_ring):
-        if (ring.shape != (B, Hkv, W, D) or ring.dtype is not torch.float32
-                or not ring.is_contiguous()):
-            raise ValueError(f"the rings must be contiguous fp32 [B, Hkv, W, D], got "
-                             f"{ring.dtype} {tuple(ring.shape)}")
+    if (k_ring.shape != (B, Hkv, W, D) or v_ring.shape != k_ring.shape
+            or k_ring.dtype is not torch.float32 or v_ring.dtype is not torch.float32
+            or not k_ring.is_contiguous() or not v_ring.is_contiguous()):
+        raise ValueError(f"the rings must be contiguous fp32 [B, Hkv, W, D], got {k_ring.dtype} "
+                         f"{tuple(k_ring.shape)}, {v_ring.dtype} {tuple(v_ring.shape)}")
     if pos.dtype is not torch.int32 or pos.shape != (B,):
         raise ValueError("pos must be int32 [B]")
     xdt = q.dtype if q.dtype in _DT else torch.float32
     cdt = cos.dtype if cos.dtype is sin.dtype and cos.dtype in _DT else torch.float32
-    kp = vp = cp = sp = count = stp = None
-    Tp = cp_sb = 0
+    Tp = cp_sb = p_k = p_v = p_c = p_s = p_count = 0
+    stp = None
     if pending is not None:
         kp, vp, cp, sp, count = pending
-        if not _lib.same_device(q, kp, vp, cp, sp):
+        if not (index == kp.get_device() == vp.get_device() == cp.get_device()
+                == sp.get_device()):
             _lib.require_cuda(q, kp, vp, cp, sp)
         Tp = kp.shape[2]
         if kp.shape != (B, Hkv, Tp, D) or vp.shape != kp.shape:
             raise ValueError(f"pending k and v must be [B, Hkv, T, D], got {tuple(kp.shape)}, "
                              f"{tuple(vp.shape)}")
-        count = _pending_count(count, B, index)
         if Tp:
             cp, sp, cp_sb = _tables(cp, sp, cdt, B, Tp, D)
             kp, vp = _rows(kp, xdt), _rows(vp, xdt)
-            stp = _lib.longlongs(6)(*kp.stride()[:3], *vp.stride()[:3])
-    y = torch.empty((B, H, T, D), device=q.device, dtype=torch.bfloat16)
+            stp = _strides2(*kp.stride(), *vp.stride())
+            p_k, p_v, p_c, p_s = kp.data_ptr(), vp.data_ptr(), cp.data_ptr(), sp.data_ptr()
+        if count is not None:
+            count = _pending_count(count, B, index)
+            p_count = count.data_ptr()
+    y = q.new_empty((B, H, T, D), dtype=torch.bfloat16)
     if B == 0 or T == 0 and Tp == 0:
         return y
     cos, sin, cs_sb = _tables(cos, sin, cdt, B, T, D)
     q, k, v = _rows(q, xdt), _rows(k, xdt), _rows(v, xdt)
-    st = _lib.longlongs(9)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
-    meta32, pos = _lib.as_dtype(meta, torch.float32), pos.contiguous()
-    p = _lib.ptr if Tp else (lambda t: None)
+    meta, pos = _lib.as_dtype(meta, torch.float32), pos.contiguous()
     size = _lib.size_query("lz_swa_decode_block_workspace_bytes", B, H, Hkv, T, D)
-    ws = torch.empty(size, device=q.device, dtype=torch.uint8)
+    ws = pos.new_empty((size + 3) // 4)
     rc = _lib.call(
         index, _lib.load().lz_swa_decode_block, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-        _DT[xdt], st, cos.data_ptr(), sin.data_ptr(), _DT[cdt], cs_sb, p(kp), p(vp), stp, p(cp),
-        p(sp), cp_sb, _lib.ptr(count), k_ring.data_ptr(), v_ring.data_ptr(), pos.data_ptr(),
-        meta32.data_ptr() or None, meta32.numel(), y.data_ptr(), ws.data_ptr(), size, B, H, Hkv,
-        T, Tp, W, D,
-        _lib.stream_of(q))
+        _DT[xdt], _strides3(*q.stride(), *k.stride(), *v.stride()), cos.data_ptr(),
+        sin.data_ptr(), _DT[cdt], cs_sb, p_k, p_v, stp, p_c, p_s, cp_sb, p_count,
+        k_ring.data_ptr(), v_ring.data_ptr(), pos.data_ptr(), meta.data_ptr(), meta.numel(),
+        y.data_ptr(), ws.data_ptr(), size, B, H, Hkv, T, Tp, W, D, _lib.raw_stream(index))
     if rc:
         _lib.check(rc, "swa decode block")
     return y

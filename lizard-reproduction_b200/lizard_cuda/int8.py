@@ -79,9 +79,10 @@ def _aligned(t):
 def int8_matmul(a, a_scale, b, b_scale, bias=None, dtype=torch.bfloat16):
     """y [..., N] = (a b^T) * a_scale * b_scale + bias for codes a int8 [..., K],
     b int8 [N, K] and scales fp32 [...] and [N], in `dtype` (bf16 or fp32)."""
-    given = (a, a_scale, b, b_scale) if bias is None else (a, a_scale, b, b_scale, bias)
-    if not _lib.same_device(*given):
-        _lib.require_cuda(*given)
+    index = a.get_device()
+    if not (index == a_scale.get_device() == b.get_device() == b_scale.get_device()
+            == (index if bias is None else bias.get_device()) >= 0):
+        _lib.require_cuda(a, a_scale, b, b_scale, *(() if bias is None else (bias,)))
     _no_grad(a_scale, b_scale, bias)
     if a.dim() < 1 or a.dtype is not torch.int8:
         raise ValueError(f"a must be int8 [..., K], got {a.dtype} {tuple(a.shape)}")
@@ -90,7 +91,7 @@ def int8_matmul(a, a_scale, b, b_scale, bias=None, dtype=torch.bfloat16):
         raise ValueError(f"a's scale must be fp32 {tuple(lead)}, got {a_scale.dtype} "
                          f"{tuple(a_scale.shape)}")
     _check(K, N, b, b_scale, bias, dtype)
-    y = torch.empty((*lead, N), device=a.device, dtype=dtype)
+    y = a.new_empty((*lead, N), dtype=dtype)
     ar = _rows(a)
     M = ar.shape[0]
     if M:
@@ -99,13 +100,12 @@ def int8_matmul(a, a_scale, b, b_scale, bias=None, dtype=torch.bfloat16):
         bias = None if bias is None else bias.contiguous()
         ws = None
         if not (_aligned(ar) and _aligned(br)):
-            ws = torch.empty(_lib.size_query("lz_int8_workspace_bytes", M, N, K), device=a.device,
-                             dtype=torch.uint8)
+            ws = a.new_empty(_lib.size_query("lz_int8_workspace_bytes", M, N, K))
         rc = _lib.call(
-            a.get_device(), _lib.load().lz_int8_matmul, ar.data_ptr(), ar.stride(0),
+            index, _lib.load().lz_int8_matmul, ar.data_ptr(), ar.stride(0),
             sa.data_ptr(), br.data_ptr(), br.stride(0), sb.data_ptr(), _lib.ptr(bias),
             0 if bias is None else _DT[bias.dtype], y.data_ptr(), _DT[dtype], _lib.ptr(ws),
-            0 if ws is None else ws.numel(), M, N, K, _lib.stream_of(a))
+            0 if ws is None else ws.numel(), M, N, K, _lib.raw_stream(index))
         if rc:
             _lib.check(rc, "int8 matmul")
     return y
@@ -115,9 +115,10 @@ def int8_linear(x, weight, weight_scale, bias=None, dtype=None):
     """y [..., N] = x W^T + bias with x [..., K] (fp32 or bf16) quantised row by
     row and the weight given as codes int8 [N, K] with a scale fp32 [N] for each
     channel (int8_quantize of an nn.Linear weight), in `dtype` (x's by default)."""
-    given = (x, weight, weight_scale) if bias is None else (x, weight, weight_scale, bias)
-    if not _lib.same_device(*given):
-        _lib.require_cuda(*given)
+    index = x.get_device()
+    if not (index == weight.get_device() == weight_scale.get_device()
+            == (index if bias is None else bias.get_device()) >= 0):
+        _lib.require_cuda(x, weight, weight_scale, *(() if bias is None else (bias,)))
     _no_grad(x, weight_scale, bias)
     if x.dim() < 1:
         raise ValueError(f"x must be [..., K], got {tuple(x.shape)}")
@@ -127,7 +128,7 @@ def int8_linear(x, weight, weight_scale, bias=None, dtype=None):
     if dtype is None:
         dtype = x.dtype
     _check(K, N, weight, weight_scale, bias, dtype)
-    y = torch.empty((*lead, N), device=x.device, dtype=dtype)
+    y = x.new_empty((*lead, N), dtype=dtype)
     xr = _rows(x)
     M = xr.shape[0]
     if M:
@@ -135,12 +136,12 @@ def int8_linear(x, weight, weight_scale, bias=None, dtype=None):
         bias = None if bias is None else bias.contiguous()
         size = (_lib.size_query("lz_int8_linear_workspace_bytes", M, K) if _aligned(w)
                 else _lib.size_query("lz_int8_workspace_bytes", M, N, K))
-        work = torch.empty(size, device=x.device, dtype=torch.uint8)
+        work = w.new_empty(size)
         rc = _lib.call(
-            x.get_device(), _lib.load().lz_int8_linear, xr.data_ptr(), _DT[xr.dtype],
+            index, _lib.load().lz_int8_linear, xr.data_ptr(), _DT[xr.dtype],
             xr.stride(0), w.data_ptr(), w.stride(0), ws.data_ptr(), _lib.ptr(bias),
             0 if bias is None else _DT[bias.dtype], y.data_ptr(), _DT[dtype], work.data_ptr(),
-            size, M, N, K, _lib.stream_of(x))
+            size, M, N, K, _lib.raw_stream(index))
         if rc:
             _lib.check(rc, "int8 linear")
     return y

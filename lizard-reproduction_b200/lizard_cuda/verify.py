@@ -29,9 +29,10 @@ def verify_drafts(target_logits, draft_logits, draft_tokens, uniforms, noise, te
     drafted tokens of each sequence (0..K) when they differ. tokens holds the
     accepted tokens, the next one, and -1 beyond; the next one is -1 only where
     the target's row is masked (-inf or NaN) throughout."""
-    given = (target_logits, draft_logits, draft_tokens, uniforms, noise)
-    if not _lib.same_device(*given):
-        _lib.require_cuda(*given)
+    index = target_logits.get_device()
+    if not (index == draft_logits.get_device() == draft_tokens.get_device()
+            == uniforms.get_device() == noise.get_device() >= 0):
+        _lib.require_cuda(target_logits, draft_logits, draft_tokens, uniforms, noise)
     if target_logits.dim() != 3 or target_logits.shape[1] < 1:
         raise ValueError(f"target_logits must be [B, K + 1, V], got {tuple(target_logits.shape)}")
     B, K1, V = target_logits.shape
@@ -59,9 +60,8 @@ def verify_drafts(target_logits, draft_logits, draft_tokens, uniforms, noise, te
             raise ValueError(f"lengths must be int32 [{B}], got {lengths.dtype} "
                              f"{tuple(lengths.shape)}")
         lengths = lengths.contiguous()
-    dev = target_logits.device
-    out = torch.empty((B, K1), device=dev, dtype=draft_tokens.dtype)
-    accepted = torch.empty((B,), device=dev, dtype=torch.int32)
+    out = draft_tokens.new_empty((B, K1))
+    accepted = draft_tokens.new_empty(B, dtype=torch.int32)
     if B == 0:
         return out, accepted
     xdt = target_logits.dtype if target_logits.dtype in _DT else torch.float32
@@ -69,13 +69,13 @@ def verify_drafts(target_logits, draft_logits, draft_tokens, uniforms, noise, te
     e = _logits(noise, torch.float32)
     tok, u = draft_tokens.contiguous(), _lib.as_dtype(uniforms, torch.float32)
     size = _lib.size_query("lz_verify_drafts_workspace_bytes", B, K, V)
-    ws = torch.empty(size, device=dev, dtype=torch.uint8)
+    ws = noise.new_empty(size // 4, dtype=torch.float32)  # whole 16-byte records
     (tb, tr, _), (db, dr, _) = t.stride(), d.stride()
     rc = _lib.call(
-        t.get_device(), _lib.load().lz_verify_drafts, t.data_ptr(), tb, tr, d.data_ptr(), db, dr,
+        index, _lib.load().lz_verify_drafts, t.data_ptr(), tb, tr, d.data_ptr(), db, dr,
         _DT[xdt], tok.data_ptr(), tok.dtype is torch.int64, u.data_ptr(), e.data_ptr(),
         e.stride(0), _lib.ptr(temp), temp_all, _lib.ptr(lengths), out.data_ptr(),
-        accepted.data_ptr(), ws.data_ptr(), size, B, K, V, _lib.stream_of(t))
+        accepted.data_ptr(), ws.data_ptr(), size, B, K, V, _lib.raw_stream(index))
     if rc:
         _lib.check(rc, "verify drafts")
     return out, accepted

@@ -45,7 +45,9 @@ def test_gla_decode_block_validates(lib):
 
 def test_swa_decode_block_validates(lib):
     p = _fake(16)
-    st, stp = (ctypes.c_longlong * 9)(), (ctypes.c_longlong * 6)()
+    st = (ctypes.c_longlong * 12)(*[0, 0, 0, 1] * 3)
+    stp = (ctypes.c_longlong * 8)(*[0, 0, 0, 1] * 2)
+    bad = (ctypes.c_longlong * 12)(*[0, 0, 0, 1, 0, 0, 0, 2, 0, 0, 0, 1])
 
     def call(B=2, H=8, Hkv=2, T=4, Tp=4, W=64, D=64, x=0, cs=0, n_meta=4, meta=p[13], strides=st,
              q=p[0], kp=p[5], ws=p[15], n=1 << 30):
@@ -61,6 +63,7 @@ def test_swa_decode_block_validates(lib):
     assert call(n_meta=33) == 1 and call(meta=None) == 1 and b"n_meta" in _msg(lib)
     assert call(x=2) == 1 and call(cs=7) == 1 and b"dtypes" in _msg(lib)
     assert call(q=None) == 1 and call(strides=None) == 1
+    assert call(strides=bad) == 1 and b"contiguous" in _msg(lib)
     assert call(kp=None) == 1 and b"previous block" in _msg(lib)
     need = lib.lz_swa_decode_block_workspace_bytes(2, 8, 2, 4, 64)
     assert need >= 4 * (16 * 64 * 4 + 2 * 16 * 64 * 4)
