@@ -177,10 +177,91 @@ __device__ __forceinline__ int piece_vectors(int nv, int np) {
   return (per + kU * 32 - 1) / (kU * 32) * (kU * 32);
 }
 
-// Statistics of the pieces of the rows, a warp each: a warp's lanes read 16 bytes
-// apiece, kU times in flight.
+// A warp's piece of a row: vectors v0 .. v1 of 16 bytes, and for the row's first
+// piece the elements before and after all vectors, a lane each.
 template <typename T>
-__global__ void __launch_bounds__(kT, 5) verify_stats_kernel(const VerifyArgs a) {
+struct Span {
+  const T* x;
+  int head, v0, v1, edge, edge_at;
+  __device__ __forceinline__ const uint4* vectors() const {
+    return reinterpret_cast<const uint4*>(x + head);
+  }
+};
+
+// The rare ways through a piece are functions of their own, so that their registers
+// do not weigh on the usual one.
+// Greedy: the largest logit and its lowest index.
+template <typename T>
+__device__ __noinline__ Piece greedy_piece(const Span<T> sp) {
+  constexpr int VE = 16 / sizeof(T);
+  const int lane = threadIdx.x & 31;
+  const uint4* xv = sp.vectors();
+  float m = -INFINITY;
+  int at = -1;   // index of m for an element taken one by one,
+  int vec = -1;  // or the first vector that holds m
+  if (lane < sp.edge && ld(sp.x + sp.edge_at) > m) m = ld(sp.x + sp.edge_at), at = sp.edge_at;
+  float vm = -INFINITY;
+  for (int i = sp.v0 + lane; i < sp.v1; i += kU * 32) {
+    uint4 w[kU];
+    load(w, xv, i, sp.v1, T());
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const float t1 = top(w[u], T());
+      if (t1 > vm) vm = t1, vec = i + u * 32;
+    }
+  }
+  unsigned long long best = 0;  // (ordered bits of the logit, ~index)
+  const auto offer = [&](float v, int i) {
+    const unsigned int u = __float_as_uint(v + 0.f);  // -0 counts as 0
+    const unsigned int o = u & 0x80000000u ? ~u : u | 0x80000000u;
+    best = max(best, (unsigned long long)o << 32 | (unsigned int)~i);
+  };
+  if (at >= 0) offer(m, at);
+  if (vec >= 0) {
+    float f[VE];
+    unpack(xv[vec], f);
+#pragma unroll
+    for (int e = VE - 1; e >= 0; --e)
+      if (f[e] == vm) at = sp.head + vec * VE + e;
+    offer(vm, at);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+  if (!best) return Piece{-INFINITY, 0.f, -1, 0};
+  const unsigned int o = (unsigned int)(best >> 32);
+  return Piece{__uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o), 0.f,
+               (int)~(unsigned int)best, 0};
+}
+// A piece with NaN or huge values: every logit cleaned.
+template <typename T>
+__device__ __noinline__ Stat cleaned_piece(const Span<T> sp, float c) {
+  constexpr int VE = 16 / sizeof(T);
+  const int lane = threadIdx.x & 31;
+  const uint4* xv = sp.vectors();
+  Stat st = {-INFINITY, 0.f};
+  const auto add = [&](float v) {
+    v = clean(v);
+    if (v > st.m) {
+      if (st.m > -INFINITY) st.s *= exp2f((st.m - v) * c);
+      st.m = v;
+    }
+    if (v > -INFINITY) st.s += exp2f((v - st.m) * c);
+  };
+  if (lane < sp.edge) add(ld(sp.x + sp.edge_at));
+  for (int i = sp.v0 + lane; i < sp.v1; i += 32) {
+    float f[VE];
+    unpack(xv[i], f);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) add(f[e]);
+  }
+  return warp_join(st, c);
+}
+
+// Statistics of the pieces of the rows, a warp each: a warp's lanes read 16 bytes
+// apiece, kU times in flight. (Loading the next vectors ahead of the sums costs
+// more in resident warps than it hides: 47 us against 41 for 960 rows of 128256.)
+template <typename T>
+__global__ void __launch_bounds__(kT, 6) verify_stats_kernel(const VerifyArgs a) {
   constexpr int VE = 16 / sizeof(T);
   const int lane = threadIdx.x & 31, piece = blockIdx.x * (kT / 32) + (threadIdx.x >> 5);
   const int nrow = 2 * a.K + 1, b = blockIdx.y / nrow, r = blockIdx.y - b * nrow;
@@ -191,131 +272,73 @@ __global__ void __launch_bounds__(kT, 5) verify_stats_kernel(const VerifyArgs a)
   const bool greedy = !(t >= kGreedy);
   const int n = drafted(a, b);
   if (r <= a.K ? r > n : (greedy || r - a.K - 1 >= n)) return;
-  const T* x = r <= a.K ? static_cast<const T*>(a.target) + b * a.t_sb + r * a.t_sr
-                        : static_cast<const T*>(a.draft) + b * a.d_sb + (r - a.K - 1) * a.d_sr;
+  Span<T> sp;
+  sp.x = r <= a.K ? static_cast<const T*>(a.target) + b * a.t_sb + r * a.t_sr
+                  : static_cast<const T*>(a.draft) + b * a.d_sb + (r - a.K - 1) * a.d_sr;
   // head up to a 16-byte boundary, whole vectors, tail; head and tail go to piece 0
-  const int head = min(a.V, (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
-  const int nv = (a.V - head) / VE, tail0 = head + nv * VE;
-  const uint4* xv = reinterpret_cast<const uint4*>(x + head);
-  const int per = piece_vectors(nv, a.np), v0 = min(nv, per * piece), v1 = min(nv, v0 + per);
+  sp.head = min(a.V, (int)(((16 - (reinterpret_cast<uintptr_t>(sp.x) & 15)) & 15) / sizeof(T)));
+  const int nv = (a.V - sp.head) / VE, tail0 = sp.head + nv * VE;
+  const int per = piece_vectors(nv, a.np);
+  sp.v0 = min(nv, per * piece);
+  sp.v1 = min(nv, sp.v0 + per);
   // up to 2 (VE - 1) elements taken one by one, a lane each
-  const int edge = piece == 0 ? head + a.V - tail0 : 0;
-  const int edge_at = lane < head ? lane : tail0 + lane - head;
+  sp.edge = piece == 0 ? sp.head + a.V - tail0 : 0;
+  sp.edge_at = lane < sp.head ? lane : tail0 + lane - sp.head;
   Piece* out = a.pieces + (size_t)blockIdx.y * a.np + piece;
-
   if (greedy) {
-    float m = -INFINITY;
-    int at = -1;   // index of m for an element taken one by one,
-    int vec = -1;  // or the first vector that holds m
-    if (lane < edge && ld(x + edge_at) > m) m = ld(x + edge_at), at = edge_at;
-    float vm = -INFINITY;
-    for (int i = v0 + lane; i < v1; i += kU * 32) {
-      uint4 w[kU];
-      load(w, xv, i, v1, T());
-#pragma unroll
-      for (int u = 0; u < kU; ++u) {
-        const float t1 = top(w[u], T());
-        if (t1 > vm) vm = t1, vec = i + u * 32;
-      }
-    }
-    unsigned long long best = 0;  // (ordered bits of the logit, ~index)
-    const auto offer = [&](float v, int i) {
-      const unsigned int u = __float_as_uint(v + 0.f);  // -0 counts as 0
-      const unsigned int o = u & 0x80000000u ? ~u : u | 0x80000000u;
-      best = max(best, (unsigned long long)o << 32 | (unsigned int)~i);
-    };
-    if (at >= 0) offer(m, at);
-    if (vec >= 0) {
-      float f[VE];
-      unpack(xv[vec], f);
-#pragma unroll
-      for (int e = VE - 1; e >= 0; --e)
-        if (f[e] == vm) at = head + vec * VE + e;
-      offer(vm, at);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-    if (lane == 0) {
-      const unsigned int o = (unsigned int)(best >> 32);
-      *out = best ? Piece{__uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o), 0.f,
-                          (int)~(unsigned int)best, 0}
-                  : Piece{-INFINITY, 0.f, -1, 0};
-    }
+    const Piece p = greedy_piece(sp);
+    if (lane == 0) *out = p;
     return;
   }
-
+  const uint4* xv = sp.vectors();
   const float c = kLog2e / t;
   Stat st = {-INFINITY, 0.f};
-  {
-    float mc = 0.f;  // m c, rounded; its rounding error is taken out of the sum at the end
-    float2 sum[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
-    const auto rebase = [&](float m) {
-      const float omc = mc;
-      mc = m * c;
-      if (st.m > -INFINITY) {
-        const float f = tc::ex2(omc - mc);
+  float mc = 0.f;  // m c, rounded; its rounding error is taken out of the sum at the end
+  float2 sum[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
+  const auto rebase = [&](float m) {
+    const float omc = mc;
+    mc = m * c;
+    if (st.m > -INFINITY) {
+      const float f = tc::ex2(omc - mc);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum[i].x *= f, sum[i].y *= f;
-      }
-      st.m = m;
-    };
-    const auto take = [&](const uint4(&w)[kU]) {
-      const float vm = top(w, T());
-      if (vm > st.m) rebase(vm);
-      if (st.m == -INFINITY) return;
-      const float2 cc = make_float2(c, c), nm = make_float2(-mc, -mc);
-#pragma unroll
-      for (int u = 0; u < kU; ++u) {
-        float f[VE];
-        unpack(w[u], f);
-#pragma unroll
-        for (int e = 0; e < VE; e += 2) {
-          const float2 g = fma2(make_float2(f[e], f[e + 1]), cc, nm);
-          sum[(e >> 1) & 3] = add2(sum[(e >> 1) & 3], make_float2(tc::ex2(g.x), tc::ex2(g.y)));
-        }
-      }
-    };
-    if (lane < edge) {
-      const float v = ld(x + edge_at);
-      if (v > st.m) rebase(v);
-      if (st.m > -INFINITY) sum[0].x = tc::ex2(fmaf(v, c, -mc));
+      for (int i = 0; i < 4; ++i) sum[i].x *= f, sum[i].y *= f;
     }
-    for (int i = v0 + lane; i < v1; i += kU * 32) {
-      uint4 w[kU];
-      if (i - lane + kU * 32 <= v1) {
-#pragma unroll
-        for (int u = 0; u < kU; ++u) w[u] = __ldg(xv + i + u * 32);
-      } else {
-        load(w, xv, i, v1, T());
-      }
-      take(w);
-    }
-    sum[0] = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
-    st.s = sum[0].x + sum[0].y;
-    // sum of 2^(x c - fl(m c)) -> sum of 2^((x - m) c)
-    if (st.m > -INFINITY) st.s *= exp2f(-fmaf(st.m, c, -mc));
-    st = warp_join(st, c);
+    st.m = m;
+  };
+  if (lane < sp.edge) {
+    const float v = ld(sp.x + sp.edge_at);
+    if (v > st.m) rebase(v);
+    if (st.m > -INFINITY) sum[0].x = tc::ex2(fmaf(v, c, -mc));
   }
-  if (!(st.s < INFINITY && st.m < INFINITY)) {
-    // NaN or huge values: once more, every logit cleaned
-    st = {-INFINITY, 0.f};
-    const auto add = [&](float v) {
-      v = clean(v);
-      if (v > st.m) {
-        if (st.m > -INFINITY) st.s *= exp2f((st.m - v) * c);
-        st.m = v;
-      }
-      if (v > -INFINITY) st.s += exp2f((v - st.m) * c);
-    };
-    if (lane < edge) add(ld(x + edge_at));
-    for (int i = v0 + lane; i < v1; i += 32) {
+  for (int i = sp.v0 + lane; i < sp.v1; i += kU * 32) {
+    uint4 w[kU];
+    if (i - lane + kU * 32 <= sp.v1) {
+#pragma unroll
+      for (int u = 0; u < kU; ++u) w[u] = __ldg(xv + i + u * 32);
+    } else {
+      load(w, xv, i, sp.v1, T());
+    }
+    const float vm = top(w, T());
+    if (vm > st.m) rebase(vm);
+    if (st.m == -INFINITY) continue;
+    const float2 cc = make_float2(c, c), nm = make_float2(-mc, -mc);
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
       float f[VE];
-      unpack(xv[i], f);
+      unpack(w[u], f);
 #pragma unroll
-      for (int e = 0; e < VE; ++e) add(f[e]);
+      for (int e = 0; e < VE; e += 2) {
+        const float2 g = fma2(make_float2(f[e], f[e + 1]), cc, nm);
+        sum[(e >> 1) & 3] = add2(sum[(e >> 1) & 3], make_float2(tc::ex2(g.x), tc::ex2(g.y)));
+      }
     }
-    st = warp_join(st, c);
   }
+  sum[0] = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+  st.s = sum[0].x + sum[0].y;
+  // sum of 2^(x c - fl(m c)) -> sum of 2^((x - m) c)
+  if (st.m > -INFINITY) st.s *= exp2f(-fmaf(st.m, c, -mc));
+  st = warp_join(st, c);
+  if (!(st.s < INFINITY && st.m < INFINITY)) st = cleaned_piece(sp, c);
   if (lane == 0) *out = {st.m, st.s, -1, 0};
 }
 
