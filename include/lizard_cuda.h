@@ -596,9 +596,10 @@ int lz_int8_matmul(const void* a, long long a_ld, const float* a_scale,
 int lz_int8_set_path(int path);
 
 /* lz_int8_quantize of x and lz_int8_matmul with the weight codes w [N, K] in
- * one call. Workspace: lz_int8_linear_workspace_bytes(M, K) when rows of w start
- * on 16-byte boundaries, else lz_int8_workspace_bytes(M, N, K). */
-size_t lz_int8_linear_workspace_bytes(int M, int K);
+ * one call (for a few tokens, in one kernel). Workspace:
+ * lz_int8_linear_workspace_bytes when rows of w start on 16-byte boundaries (0 for
+ * a few tokens), else lz_int8_workspace_bytes. */
+size_t lz_int8_linear_workspace_bytes(int M, int N, int K);
 int lz_int8_linear(const void* x, int x_dtype, long long x_ld, const void* w, long long w_ld,
                    const float* w_scale, const void* bias, int bias_dtype, void* y, int y_dtype,
                    void* workspace, size_t workspace_bytes, int M, int N, int K, void* stream);

@@ -241,6 +241,9 @@ struct Out {  // y and what scales it
   const void* bias;  // [N] fp32 or bf16, or null
   void* y;           // [M, N] contiguous, fp32 or bf16
   int bias_bf16, y_bf16, M, N, K;
+  const void* x;  // x itself, rows ldx elements apart, where the product quantises it
+  long long ldx;
+  int x_bf16;
 };
 __device__ __forceinline__ float bias_at(const Out& o, int n) {
   if (!o.bias) return 0.f;
@@ -253,39 +256,96 @@ __device__ __forceinline__ float scaled(int acc, float sa, float sb, float bias)
 
 // -------------------------------------------------------------------- narrow
 constexpr int kNStaging = 8192;  // bytes of y on their way out: 32 tokens x 128 channels (bf16)
-template <int BN>
+constexpr int kFuseK = 4096;  // the largest K whose tokens a CTA quantises by itself
+template <int BN, bool FUSE>
 struct Narrow {
   static constexpr int kStages = BN <= 32 ? 5 : BN == 64 ? 4 : 3;
   static constexpr int kA = 128 * 128, kB = BN * 128;
+  static constexpr int kStage = kA + (FUSE ? 0 : kB);
   static constexpr int kCols = BN < 32 ? 32 : BN;  // TMEM columns of an accumulator
   // operand stages (the partials of a split reuse them), staging, token scales,
-  // barriers, TMEM address; two CTAs fit an SM
-  static constexpr size_t kSmem =
-      1024 + (size_t)kStages * (kA + kB) + kNStaging + 2 * BN * 4 + 256;
-  static_assert((size_t)kStages * (kA + kB) >= (size_t)BN * 128 * 4, "partials fit");
-  static_assert(kSmem <= 115712, "two CTAs an SM");
+  // barriers, TMEM address; with FUSE the codes of `steps` steps of K besides
+  static constexpr size_t smem(int steps) {
+    return 1024 + (size_t)kStages * kStage + kNStaging + (FUSE ? (size_t)steps * kB : 0) +
+           2 * BN * 4 + 256;
+  }
+  static_assert((size_t)kStages * kStage >= (size_t)BN * 128 * 4, "partials fit");
+  static_assert(FUSE || smem(0) <= 115712, "two CTAs an SM");
 };
+
+// The tokens of a small call, quantised by the CTA that multiplies them: rows M of x,
+// codes of columns k0 .. k1 to the swizzled K-major tiles at `codes` ([step][BN]
+// rows of 128 bytes), scales to sa. By 128 threads, a warp a row, 8 vectors of 16
+// bytes a lane kept (the rest is read twice: registers for all of it would leave one
+// CTA an SM, and clusters of eight then no longer all fit at once). The same
+// arithmetic as i8_quantize_kernel.
+template <typename T, int BN>
+__device__ __forceinline__ void quantize_here(const T* x, long long ldx, int M, int K, int k0,
+                                              int k1, unsigned char* codes, float* sa) {
+  using V = Vec<T>;
+  constexpr int KEEP = 8;
+  const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) & 3;
+  const auto at = [&](int m, int k) {
+    const int c = k - k0;
+    return codes + (c >> 7) * (BN * 128) + m * 128 + ((((c >> 4) & 7) ^ (m & 7)) << 4) + (c & 15);
+  };
+  for (int m = w; m < M; m += 4) {
+    const T* row = x + m * ldx;
+    const int nv = (reinterpret_cast<uintptr_t>(row) & 15) == 0 ? K / V::N : 0;
+    const uint4* rv = reinterpret_cast<const uint4*>(row);
+    uint4 keep[KEEP];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i)
+      keep[i] = lane + 32 * i < nv ? __ldg(rv + lane + 32 * i) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) top = max(top, V::top(keep[i]));
+    for (int i = lane + 32 * KEEP; i < nv; i += 32) top = max(top, V::top(__ldg(rv + i)));
+    for (int k = nv * V::N + lane; k < K; k += 32)
+      top = max(top, __float_as_uint(V::value(row + k)) & 0x7fffffffu);
+    top = __reduce_max_sync(0xffffffffu, top);
+    const float t = __uint_as_float(top);
+    const bool live = t >= 4e-37f && t < INFINITY;
+    const float inv = live ? 127.f / t : 0.f;
+    if (lane == 0) sa[m] = live ? t / 127.f : (t < 1.f ? 0.f : __uint_as_float(0x7fc00000u));
+    if (!live) {
+      for (int k = k0 + lane; k < k1; k += 32) *at(m, k) = 0;
+      continue;
+    }
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) {
+      const int k = (lane + 32 * i) * V::N;
+      if (lane + 32 * i < nv && k >= k0 && k < k1)
+        store_codes(reinterpret_cast<int8_t*>(at(m, k)), keep[i], inv, T());
+    }
+    for (int i = lane + 32 * KEEP; i < nv; i += 32) {
+      const int k = i * V::N;
+      if (k >= k0 && k < k1)
+        store_codes(reinterpret_cast<int8_t*>(at(m, k)), __ldg(rv + i), inv, T());
+    }
+    for (int k = nv * V::N + lane; k < K; k += 32)
+      if (k >= k0 && k < k1)
+        *at(m, k) = (unsigned char)(code_of(V::value(row + k), inv) & 0xffu);
+  }
+}
 
 // Warps: 0 TMA, 1 MMA (and TMEM), 2..5 epilogue. split == 1: a CTA walks the (weight
 // tile, token tile) pairs blockIdx.x, + gridDim.x, ..., weight tiles fastest. split
-// > 1: clusters of `split` CTAs, one tile each, K dealt over the cluster.
-template <int BN>
+// > 1: clusters of `split` CTAs, one tile each, K dealt over the cluster. FUSE: x
+// itself comes in o.x, and the epilogue warps quantise it while the weights load: one
+// launch instead of two, for the few tokens of a decode step (M <= 4, K <= kFuseK).
+template <int BN, bool FUSE>
 __global__ void __launch_bounds__(192)
 i8_narrow_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx,
                  const __grid_constant__ CUtensorMap ty, const Out o, const int split,
                  const int ytma) {
-  using P = Narrow<BN>;
+  using P = Narrow<BN, FUSE>;
   constexpr int S = P::kStages;
   extern __shared__ unsigned char raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-  unsigned char* staging = sm + (size_t)S * (P::kA + P::kB);
-  float* sSa = reinterpret_cast<float*>(staging + kNStaging);  // [2][BN] token scales
-  uint64_t* full = reinterpret_cast<uint64_t*>(sSa + 2 * BN);
-  uint64_t* empty = full + S;
-  uint64_t* acc_full = empty + S;      // [2]
-  uint64_t* acc_empty = acc_full + 2;  // [2]
-  uint32_t* tptr = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  unsigned char* staging = sm + (size_t)S * P::kStage;
+  unsigned char* codes = staging + kNStaging;  // FUSE: [nk][BN] rows of 128 bytes
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = split > 1 ? blockIdx.x % split : 0;
   const int wt = (o.N + 127) >> 7, tiles = wt * ((o.M + BN - 1) / BN);
@@ -293,7 +353,15 @@ i8_narrow_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__
   const int KT = (o.K + 127) >> 7;
   const int kt0 = split > 1 ? KT * rank / split : 0;
   const int nk = (split > 1 ? KT * (rank + 1) / split : KT) - kt0;
+  float* sSa = reinterpret_cast<float*>(codes + (FUSE ? nk * P::kB : 0));  // [2][BN] token scales
+  uint64_t* full = reinterpret_cast<uint64_t*>(sSa + 2 * BN);
+  uint64_t* empty = full + S;
+  uint64_t* acc_full = empty + S;      // [2]
+  uint64_t* acc_empty = acc_full + 2;  // [2]
+  uint64_t* xready = acc_empty + 2;    // FUSE: the four quantising warps
+  uint32_t* tptr = reinterpret_cast<uint32_t*>(xready + 1);
   if (tid == 0) {
+    tc::mbar_init(xready, 4);
     for (int s = 0; s < S; ++s) tc::mbar_init(full + s, 1), tc::mbar_init(empty + s, 1);
     for (int i = 0; i < 2; ++i) tc::mbar_init(acc_full + i, 1), tc::mbar_init(acc_empty + i, 4);
     tc::fence_mbar_init();
@@ -310,13 +378,27 @@ i8_narrow_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__
   tc::tc_fence_after();
   const uint32_t tmem = *tptr;
 
+  if constexpr (FUSE) {
+    if (warp >= 2) {
+      const int k0 = kt0 * 128, k1 = min(o.K, (kt0 + nk) * 128);
+      if (o.x_bf16)
+        quantize_here<bf16, BN>(static_cast<const bf16*>(o.x), o.ldx, o.M, o.K, k0, k1, codes, sSa);
+      else
+        quantize_here<float, BN>(static_cast<const float*>(o.x), o.ldx, o.M, o.K, k0, k1, codes,
+                                 sSa);
+      tc::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(xready);
+      tc::named_bar_sync(2, 128);  // the scales are there
+    }
+  }
   if (warp == 0 && lane == 0) {
     // the weights of the first stages do not depend on the launch before (the
     // quantisation of x): they load while it ends
     const int pre = min(nk, S), n0 = first % wt * 128;
     for (int i = 0; i < pre; ++i) {
-      tc::mbar_expect_tx(full + i, P::kA + P::kB);
-      tma_load_2d(sm + (size_t)i * (P::kA + P::kB), &tw, (kt0 + i) * 128, n0, full + i);
+      tc::mbar_expect_tx(full + i, P::kStage);
+      tma_load_2d(sm + (size_t)i * P::kStage, &tw, (kt0 + i) * 128, n0, full + i);
     }
     grid_dependency_wait();
     uint32_t it = 0;
@@ -324,18 +406,19 @@ i8_narrow_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__
       const int n = t % wt * 128, m = t / wt * BN;
       for (int k = 0; k < nk; ++k, ++it) {
         const int s = it % S;
-        unsigned char* st = sm + (size_t)s * (P::kA + P::kB);
+        unsigned char* st = sm + (size_t)s * P::kStage;
         if (it >= (uint32_t)pre) {
           if (it >= S) tc::mbar_wait(empty + s, (it / S - 1) & 1, 120);
-          tc::mbar_expect_tx(full + s, P::kA + P::kB);
+          tc::mbar_expect_tx(full + s, P::kStage);
           tma_load_2d(st, &tw, (kt0 + k) * 128, n, full + s);
         }
-        tma_load_2d(st + P::kA, &tx, (kt0 + k) * 128, m, full + s);
+        if constexpr (!FUSE) tma_load_2d(st + P::kA, &tx, (kt0 + k) * 128, m, full + s);
       }
     }
   } else if (warp == 1 && lane == 0) {
     constexpr uint32_t idesc = idesc_i8(128, BN);
     uint32_t it = 0, at = 0;
+    if constexpr (FUSE) tc::mbar_wait(xready, 0, 125);
     for (int t = first; t < tiles; t += stride, ++at) {
       const int buf = at & 1;
       if (at >= 2) tc::mbar_wait(acc_empty + buf, (at / 2 - 1) & 1, 123);
@@ -344,8 +427,10 @@ i8_narrow_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__
         const int s = it % S;
         tc::mbar_wait(full + s, (it / S) & 1, 121);
         tc::tc_fence_after();
-        const uint32_t a0 = smem_u32(sm + (size_t)s * (P::kA + P::kB));
-        const uint64_t ad = tc::sdesc(a0, 0, 1024), bd = tc::sdesc(a0 + P::kA, 0, 1024);
+        const uint32_t a0 = smem_u32(sm + (size_t)s * P::kStage);
+        const uint64_t ad = tc::sdesc(a0, 0, 1024);
+        const uint64_t bd =
+            tc::sdesc(FUSE ? smem_u32(codes + k * P::kB) : a0 + P::kA, 0, 1024);
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           mma_i8(tmem + buf * P::kCols, ad + 2 * q, bd + 2 * q, idesc, (k | q) != 0);
@@ -361,8 +446,9 @@ i8_narrow_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__
     for (int t = first; t < tiles; t += stride, ++at) {
       const int buf = at & 1, n0 = t % wt * 128, m0 = t / wt * BN, n = n0 + ch;
       const float sb = n < o.N ? o.sb[n] : 0.f, bias = n < o.N ? bias_at(o, n) : 0.f;
-      float* sa = sSa + buf * BN;
-      for (int i = tid - 64; i < BN; i += 128) sa[i] = m0 + i < o.M ? o.sa[m0 + i] : 0.f;
+      float* sa = FUSE ? sSa : sSa + buf * BN;
+      if constexpr (!FUSE)
+        for (int i = tid - 64; i < BN; i += 128) sa[i] = m0 + i < o.M ? o.sa[m0 + i] : 0.f;
       tc::mbar_wait(acc_full + buf, (at / 2) & 1, 122);
       tc::tc_fence_after();
       const int mt = min(BN, o.M - m0);
@@ -451,7 +537,7 @@ i8_narrow_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__
         sum.z += p.z;
         sum.w += p.w;
       }
-      const float sa = o.sa[m0 + c];
+      const float sa = FUSE ? sSa[c] : o.sa[m0 + c];
       const int v[4] = {sum.x, sum.y, sum.z, sum.w};
       const size_t at = (size_t)(m0 + c) * o.N + n0 + q;
       float y[4];
@@ -749,7 +835,7 @@ int k_split(long long tiles, int KT) {
   return split;
 }
 
-template <int BN>
+template <int BN, bool FUSE = false>
 int launch_narrow(const Operand& x, const Operand& w, const Out& o, bool after_quantize,
                   cudaStream_t st) {
   const int es = o.y_bf16 ? 2 : 4;
@@ -758,22 +844,25 @@ int launch_narrow(const Operand& x, const Operand& w, const Out& o, bool after_q
   const int split = k_split((long long)wt * mt, KT);
   CUtensorMap tw, tx, ty;
   int rc = encode(&tw, "the weight", CU_TENSOR_MAP_DATA_TYPE_UINT8, w.p, o.K, o.N, w.ld, 128, 128);
-  if (!rc) rc = encode(&tx, "x", CU_TENSOR_MAP_DATA_TYPE_UINT8, x.p, o.K, o.M, x.ld, 128, BN);
+  if (!rc && !FUSE)
+    rc = encode(&tx, "x", CU_TENSOR_MAP_DATA_TYPE_UINT8, x.p, o.K, o.M, x.ld, 128, BN);
   if (!rc && ytma && split == 1)
     rc = encode(&ty, "y", o.y_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
                 o.y, o.N, o.M, (long long)o.N * es, 128, std::min(BN, kNStaging / (128 * es)),
                 CU_TENSOR_MAP_SWIZZLE_NONE);
   else
-    ty = tx;
+    ty = tw;
+  if (FUSE) tx = tw;
   if (rc) return rc;
   static bool done[64] = {false};
-  rc = allow_smem(i8_narrow_kernel<BN>, Narrow<BN>::kSmem, done);
+  using P = Narrow<BN, FUSE>;
+  rc = allow_smem(i8_narrow_kernel<BN, FUSE>, P::smem(FUSE ? kFuseK / 128 : 0), done);
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = split > 1 ? dim3(wt * mt * split)
                           : dim3((unsigned)std::min<long long>((long long)wt * mt, 296));
   cfg.blockDim = dim3(192);
-  cfg.dynamicSmemBytes = Narrow<BN>::kSmem;
+  cfg.dynamicSmemBytes = P::smem(FUSE ? ceil_div(KT, split) : 0);
   cfg.stream = st;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -783,7 +872,7 @@ int launch_narrow(const Operand& x, const Operand& w, const Out& o, bool after_q
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = after_quantize ? 2 : 1;
-  return launched(cudaLaunchKernelEx(&cfg, i8_narrow_kernel<BN>, tw, tx, ty, o, split, ytma),
+  return launched(cudaLaunchKernelEx(&cfg, i8_narrow_kernel<BN, FUSE>, tw, tx, ty, o, split, ytma),
                   "i8_narrow_kernel");
 }
 
@@ -869,6 +958,15 @@ int product(const Operand& x, const Operand& w, const Out& o, bool after_quantiz
   return launch_narrow<128>(x, w, o, after_quantize, st);
 }
 
+// Whether the product quantises x by itself: every CTA then reads all of x, a warp a
+// row, so for up to four tokens of up to 4096 values, and while an SM has one weight
+// tile at most (the codes' room leaves one CTA an SM, which with more tiles loads the
+// weights more slowly: 50 us against 46 at K = 2048, N = 128256). One token, K = N =
+// 2048: 6.1 us against 6.0 on the device, a launch less for the host.
+bool fuse_quantize(int M, int N, int K) {
+  return M <= 4 && K <= kFuseK && N <= 148 * 128;
+}
+
 long long row16(int K) { return ((long long)K + 15) / 16 * 16; }
 
 // Rows of codes as the kernels take them: as they are, or repacked into *ws.
@@ -936,8 +1034,8 @@ extern "C" size_t lz_int8_workspace_bytes(int M, int N, int K) {
          lz::align_up((size_t)N * r, 256);
 }
 
-extern "C" size_t lz_int8_linear_workspace_bytes(int M, int K) {
-  if (M < 1 || K < 1) return 0;
+extern "C" size_t lz_int8_linear_workspace_bytes(int M, int N, int K) {
+  if (M < 1 || N < 1 || K < 1 || lz::fuse_quantize(M, N, K)) return 0;
   return lz::align_up((size_t)M * (size_t)lz::row16(K), 256) + lz::align_up((size_t)M * 4, 256);
 }
 
@@ -964,7 +1062,7 @@ extern "C" int lz_int8_matmul(const void* a, long long a_ld, const float* a_scal
   if (!rc) rc = as_operand(&w, b, b_ld, N, K, &ws, st);
   if (rc) return rc;
   const Out o = {a_scale, b_scale, bias, y, bias_dtype == LZ_DTYPE_BF16, y_dtype == LZ_DTYPE_BF16,
-                 M, N, K};
+                 M, N, K, nullptr, 0, 0};
   return product(x, w, o, false, st);
 }
 
@@ -981,12 +1079,18 @@ extern "C" int lz_int8_linear(const void* x, int x_dtype, long long x_ld, const 
              "x must be LZ_DTYPE_F32 or LZ_DTYPE_BF16");
   LZ_REQUIRE(N == 1 || w_ld >= K, LZ_ERR_INVALID_ARGUMENT, "rows of codes overlap");
   const bool fits = aligned16(w) && (N == 1 || w_ld % 16 == 0);
-  LZ_REQUIRE(workspace && aligned16(workspace) &&
-                 workspace_bytes >= (fits ? lz_int8_linear_workspace_bytes(M, K)
-                                          : lz_int8_workspace_bytes(M, N, K)),
+  const size_t need =
+      fits ? lz_int8_linear_workspace_bytes(M, N, K) : lz_int8_workspace_bytes(M, N, K);
+  LZ_REQUIRE(!need || (workspace && aligned16(workspace) && workspace_bytes >= need),
              LZ_ERR_WORKSPACE, "workspace too small, see lz_int8_linear_workspace_bytes");
   auto st = static_cast<cudaStream_t>(stream);
   unsigned char* ws = static_cast<unsigned char*>(workspace);
+  if (fits && fuse_quantize(M, N, K)) {
+    const Operand wo = {static_cast<const int8_t*>(w), N == 1 ? row16(K) : w_ld, N};
+    const Out o = {nullptr, w_scale, bias, y, bias_dtype == LZ_DTYPE_BF16,
+                   y_dtype == LZ_DTYPE_BF16, M, N, K, x, x_ld, x_dtype == LZ_DTYPE_BF16};
+    return launch_narrow<16, true>({nullptr, 0, M}, wo, o, false, st);
+  }
   int8_t* codes = reinterpret_cast<int8_t*>(ws);
   ws += align_up((size_t)M * row16(K), 256);
   float* sa = reinterpret_cast<float*>(ws);
@@ -997,6 +1101,6 @@ extern "C" int lz_int8_linear(const void* x, int x_dtype, long long x_ld, const 
   if (rc) return rc;
   const Operand xo = {codes, row16(K), M};
   const Out o = {sa, w_scale, bias, y, bias_dtype == LZ_DTYPE_BF16, y_dtype == LZ_DTYPE_BF16,
-                 M, N, K};
+                 M, N, K, nullptr, 0, 0};
   return product(xo, wo, o, true, st);
 }

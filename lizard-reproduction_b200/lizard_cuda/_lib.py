@@ -94,7 +94,7 @@ _SIGNATURES = {
     "lz_int8_quantize": (_c_int, [_vp, _c_int, _c_ll, _vp, _c_ll, _vp, _c_int, _c_int, _vp]),
     "lz_int8_set_path": (_c_int, [_c_int]),
     "lz_int8_workspace_bytes": (_c_size, [_c_int] * 3),
-    "lz_int8_linear_workspace_bytes": (_c_size, [_c_int] * 2),
+    "lz_int8_linear_workspace_bytes": (_c_size, [_c_int] * 3),
     "lz_int8_matmul": (_c_int, [_vp, _c_ll, _vp, _vp, _c_ll, _vp, _vp, _c_int, _vp, _c_int, _vp,
                                 _c_size] + [_c_int] * 3 + [_vp]),
     "lz_int8_linear": (_c_int, [_vp, _c_int, _c_ll, _vp, _c_ll, _vp, _vp, _c_int, _vp, _c_int,

@@ -134,13 +134,13 @@ def int8_linear(x, weight, weight_scale, bias=None, dtype=None):
     if M:
         w, ws = _rows(weight), weight_scale.contiguous()
         bias = None if bias is None else bias.contiguous()
-        size = (_lib.size_query("lz_int8_linear_workspace_bytes", M, K) if _aligned(w)
+        size = (_lib.size_query("lz_int8_linear_workspace_bytes", M, N, K) if _aligned(w)
                 else _lib.size_query("lz_int8_workspace_bytes", M, N, K))
-        work = w.new_empty(size)
+        work = w.new_empty(size) if size else None
         rc = _lib.call(
             index, _lib.load().lz_int8_linear, xr.data_ptr(), _DT[xr.dtype],
             xr.stride(0), w.data_ptr(), w.stride(0), ws.data_ptr(), _lib.ptr(bias),
-            0 if bias is None else _DT[bias.dtype], y.data_ptr(), _DT[dtype], work.data_ptr(),
+            0 if bias is None else _DT[bias.dtype], y.data_ptr(), _DT[dtype], _lib.ptr(work),
             size, M, N, K, _lib.raw_stream(index))
         if rc:
             _lib.check(rc, "int8 linear")

@@ -111,8 +111,9 @@ def test_int8_entries_validate(lib):
     assert mm(b=None) == 1
     need = lib.lz_int8_workspace_bytes(4, 8, 33)
     assert need >= (4 + 8) * 48 and mm(K=33, ld=33, ws=p[6], n=need - 1) == 4
-    assert lib.lz_int8_linear_workspace_bytes(4, 33) >= 4 * 48 + 16
-    rc = lib.lz_int8_linear(p[0], 0, 32, p[1], 32, p[2], None, 0, p[3], 0, None, 0, 4, 8, 32, None)
+    assert lib.lz_int8_linear_workspace_bytes(20, 8, 33) >= 20 * 48 + 80
+    assert lib.lz_int8_linear_workspace_bytes(4, 8, 33) == 0  # a few tokens need none
+    rc = lib.lz_int8_linear(p[0], 0, 32, p[1], 32, p[2], None, 0, p[3], 0, None, 0, 20, 8, 32, None)
     assert rc == 4 and b"workspace" in _msg(lib)
     rc = lib.lz_int8_linear(p[0], 9, 32, p[1], 32, p[2], None, 0, p[3], 0, p[4], 1 << 20, 4, 8, 32,
                             None)

@@ -130,7 +130,10 @@ def test_both_kernels_at_any_size(M, K, N, path):
         assert _lib.load().lz_int8_set_path(old) == path
 
 
-@pytest.mark.parametrize("M,K,N", [(1, 130, 77), (40, 1001, 300), (800, 250, 301)])
+@pytest.mark.parametrize("M,K,N", [(1, 130, 77), (40, 1001, 300), (800, 250, 301),
+                                   # quantised by the product itself, and just not
+                                   (1, 4096, 2048), (4, 4096, 140), (5, 2048, 300),
+                                   (4, 999, 129), (3, 64, 20000), (2, 4097, 64), (2, 2500, 64)])
 def test_linear_bit_for_bit_and_in_any_layout(M, K, N):
     from lizard_cuda import int8_linear, int8_matmul, int8_quantize
     g = torch.Generator(device=DEV).manual_seed(M + K)
