@@ -161,6 +161,19 @@ def test_masks_that_leave_nothing():
         assert acc[5] == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_masks_of_the_types_lowest_value(dtype):
+    """Forbidden tokens at finfo.min rather than -inf; a piece of the row, and a whole
+    row, of nothing else."""
+    low = torch.finfo(dtype).min
+    args = list(inputs(5, 2, 40000, dtype, 17))
+    args[0][:, :, 100:30000] = low
+    args[1][:, :, 100:30000] = low
+    args[0][3, 0] = low  # uniform over the vocabulary, as softmax has it
+    check(args)
+    check(args, temperature=0.3)
+
+
 def test_tokens_outside_the_vocabulary_are_refused():
     args = list(inputs(4, 3, 100, torch.float32, 9))
     args[3].zero_()  # accepts whatever has a probability
