@@ -26,10 +26,15 @@
 // output) and contracts the queries with them 32 rows at a time; the two halves of
 // F meet at the end, a row tile each. (8 columns by all of F needs no such meeting
 // but reads every key and query value twice as often from shared memory, which then
-// bounds the kernel.)
+// bounds the kernel.) Measured, 2048 states of 256 x 64, 32 query rows, 8 tokens: 80 us,
+// 4.2 TB/s of state and operands; what is left is the chain of phases of a CTA (load,
+// decays, update, products, meeting) at the two CTAs an SM that registers and shared
+// memory allow. A persistent form that loads the next state under this one's products
+// was slower (90 us): the rows of a batch accept different numbers of tokens, and
+// CTAs handed out one by one even that out.
 // The scores of the block's keys are shared: a quarter of F a warp, added through
-// shared memory. z rides along as two more keys (hi and lo): with M = [exp of the decay from key to token,
-// 0 above the diagonal | d_t for the two z columns], a' = (q K^T) o M has the row
+// shared memory. z rides along as two more keys (hi and lo): with M = [exp of the
+// decay from key to token, 0 above the diagonal | d_t for the two z columns], a' = (q K^T) o M has the row
 // sum as its own sum over all columns, and y = (d_t q S + a' V) / sum a' with zero
 // rows of V for z.
 #include <algorithm>
@@ -205,19 +210,23 @@ gla_block_kernel(const __grid_constant__ CUtensorMap ts, const GlaBlockArgs a) {
   // the first pending keys and values, before it is known how many stand
   const bf16* kp = a.fk_p + (size_t)kvh * Tp * F;
   const bf16* vp = a.v_p + (size_t)kvh * Tp * D + d0;
-  bf16 kk[ZN][kPend], vv[kPend * DN / NT];
+  // (bits in whole registers: packing them in pairs would wait for the loads)
+  uint32_t kk[ZN][kPend], vv[kPend * DN / NT];
+  const auto bits = [](const bf16* p) {
+    return (uint32_t)__ldg(reinterpret_cast<const unsigned short*>(p));
+  };
   const auto fetch = [&](int t0) {
 #pragma unroll
     for (int i = 0; i < ZN; ++i)
 #pragma unroll
       for (int t = 0; t < kPend; ++t) {
         const int f = tid + i * NT;
-        kk[i][t] = t0 + t < Tp && f < F ? kp[(t0 + t) * F + f] : __float2bfloat16_rn(0.f);
+        kk[i][t] = t0 + t < Tp && f < F ? bits(kp + (t0 + t) * F + f) : 0u;
       }
 #pragma unroll
     for (int i = 0; i < kPend * DN / NT; ++i) {
       const int t = t0 + (tid + i * NT) / DN, d = (tid + i * NT) % DN;
-      vv[i] = t < Tp && d0 + d < D ? vp[t * D + d] : __float2bfloat16_rn(0.f);
+      vv[i] = t < Tp && d0 + d < D ? bits(vp + t * D + d) : 0u;
     }
   };
   fetch(0);
@@ -258,7 +267,7 @@ gla_block_kernel(const __grid_constant__ CUtensorMap ts, const GlaBlockArgs a) {
 #pragma unroll
       for (int t = 0; t < kPend; ++t)
         if (t0 + t < n) {
-          const float x = __bfloat162float(kk[i][t]), w = w_of(t0 + t);
+          const float x = bf16_lo(kk[i][t]), w = w_of(t0 + t);
           if (f < FP) sKw[t * FP + at] = x;
           z[i] += w * x;
         }
@@ -266,7 +275,7 @@ gla_block_kernel(const __grid_constant__ CUtensorMap ts, const GlaBlockArgs a) {
 #pragma unroll
     for (int i = 0; i < kPend * DN / NT; ++i) {
       const int t = t0 + (tid + i * NT) / DN;  // the same for a warp
-      if (t < n) sVw[tid + i * NT] = w_of(t) * __bfloat162float(vv[i]);
+      if (t < n) sVw[tid + i * NT] = w_of(t) * bf16_lo(vv[i]);
     }
   };
   if (n) stage(0);
@@ -277,6 +286,7 @@ gla_block_kernel(const __grid_constant__ CUtensorMap ts, const GlaBlockArgs a) {
   f32x2 st[NH][2][2];  // [step][rows][column]
   const int cg = warp % (2 * HALVES), fh = warp / (2 * HALVES), half = cg >> 1;
   const int c = (cg & 1) * 16 + g;  // within the 32 of its tile
+  cp_async_wait_all();  // here, not at their use: after the stores below it waits for those too
   const bool live = tc::mbar_wait(bar, 0, 95);  // after a timeout nothing is written
   // (f & 7 is 2j or 2j + 1 whatever the step: two swizzled addresses and constants)
   float *even[2], *odd[2];
@@ -355,7 +365,6 @@ gla_block_kernel(const __grid_constant__ CUtensorMap ts, const GlaBlockArgs a) {
   }
 
   // z as two more keys
-  cp_async_wait_all();
   __syncthreads();  // keys and queries are there (their zero rows too)
 #pragma unroll
   for (int i = 0; i < ZN; ++i) {
@@ -592,7 +601,7 @@ extern "C" int lz_gla_decode_block(const void* fq, const void* fk, const void* v
   LZ_REQUIRE(F <= 256 && D % 4 == 0 && D <= 256, LZ_ERR_UNSUPPORTED,
              "decode supports F <= 256 and D a multiple of 4 up to 256");
   LZ_REQUIRE((long long)B * H * std::max({T, T_prev, 1}) < (1ll << 31) && Hs <= 65535,
-             LZ_ERR_UNSUPPORTED, "too many heads");
+             LZ_ERR_UNSUPPORTED, "too many sequences or heads");
   LZ_REQUIRE(state && zstate, LZ_ERR_INVALID_ARGUMENT, "null pointer");
   LZ_REQUIRE(!T || (fq && fk && v && log_gamma && y), LZ_ERR_INVALID_ARGUMENT, "null pointer");
   LZ_REQUIRE(!T_prev || (fk_prev && v_prev && log_gamma_prev), LZ_ERR_INVALID_ARGUMENT,
