@@ -158,6 +158,25 @@ def test_linear_bit_for_bit_and_in_any_layout(M, K, N):
     assert int8_linear(x3[:0], codes, scale).shape == (0, 2, N)
 
 
+@pytest.mark.parametrize("M,K,N,dtype", [(4100, 2048, 1500, torch.bfloat16),
+                                         (5000, 2056, 1289, torch.bfloat16),
+                                         (4096, 2052, 1300, torch.float32),
+                                         (20000, 4096, 256, torch.bfloat16)])
+def test_many_long_rows(M, K, N, dtype):
+    from lizard_cuda import int8_linear, int8_quantize
+    g = torch.Generator(device=DEV).manual_seed(M)
+    codes, scale = int8_quantize(torch.randn(N, K, generator=g, device=DEV))
+    wide = torch.randn(M, K + 32, generator=g, device=DEV).to(dtype)
+    x = wide[:, :K]  # rows further apart than they are long
+    x[7] = 0
+    x[M - 1, 3] = math.nan
+    xq, xs = _quantize(x)
+    want = _product(xq, xs, codes, scale, None, dtype)
+    for _ in range(3):
+        assert _same(int8_linear(x, codes, scale), want)
+    assert _same(int8_linear(x.contiguous(), codes, scale), want)
+
+
 @pytest.mark.parametrize("M", [3, 600])
 def test_the_largest_sums_stay_exact(M):
     from lizard_cuda import int8_matmul
