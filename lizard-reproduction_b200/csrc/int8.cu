@@ -21,8 +21,8 @@
 //     shares a 256 x 256 tile: each loads half of either operand, so a byte in
 //     shared memory feeds twice the math; two accumulators of 256 TMEM columns
 //     let the epilogue of a tile run under the next one's products. Measured, M =
-//     32768, K = 8192, N = 2048: 336 us, 3.27 POP/s (twice the measured bf16 peak of
-//     1638 TFLOP/s), and 118 us for the quantisation before it. A form that quantised
+//     32768, K = 8192, N = 2048: 321 us, 3.43 POP/s (twice the measured bf16 peak of
+//     1638 TFLOP/s is 3.28), and 115 us for the quantisation before it. A form that quantised
 //     in four more warps of this kernel, rows dealt over all CTAs in the order of the
 //     tiles, took 484 us against 442 for the two launches: the rows are long waits for
 //     few warps, and their traffic slows the operands'.

@@ -166,9 +166,11 @@ __host__ __device__ inline SwaWork swa_work(int DP, int QT, int R, int T) {
   return w;
 }
 
-// The first kernel. blockIdx = (block of 256 threads over the (token, columns) of a
-// pair of heads, head, batch row); tokens 0 .. TN are the block's, the rest the
-// pending ones. N: columns a thread takes (2 where alignment allows).
+// The first kernel. blockIdx = (256 threads over (token, columns), key/value head,
+// batch row); tokens 0 .. T are the block's, the rest the pending ones. Rows beyond
+// the last token or query stay as they are: the second kernel masks such keys, zeroes
+// such values and writes no such output. N: columns a thread takes (2 where alignment
+// allows).
 template <typename XT, int DP, int QT, int N>
 __global__ void __launch_bounds__(256) swa_rotate_kernel(const SwaBlockArgs a) {
   constexpr int LQ = DP + 8, RQ = 16 * QT, PER = DP / 2 / N;  // threads a token
@@ -176,13 +178,13 @@ __global__ void __launch_bounds__(256) swa_rotate_kernel(const SwaBlockArgs a) {
   const int i = blockIdx.x * 256 + threadIdx.x, row = i / PER, d = i % PER * N;
   const int b = blockIdx.z, hk = blockIdx.y, T = a.T, D = a.D, half = D / 2;
   const int TN = (T + 15) & ~15, rep = a.rep, R = rep * T;
-  if (row < TN) {
+  if (row < T) {
     const SwaWork o = swa_work(DP, QT, R, T);
     unsigned char* ws = a.ws + (size_t)(b * a.Hkv + hk) * o.total;
     float* wk = reinterpret_cast<float*>(ws + o.k);
     float* wv = reinterpret_cast<float*>(ws + o.v);
     const int t = row;
-    const bool in = t < T && d < half;
+    const bool in = d < half;
     const XT* kp = static_cast<const XT*>(a.k.p) + b * a.k.sb + hk * a.k.sh + t * a.k.st + d;
     const XT* vp = static_cast<const XT*>(a.v.p) + b * a.v.sb + hk * a.v.sh + t * a.v.st + d;
     const XT* qp = static_cast<const XT*>(a.q.p) + b * a.q.sb + hk * rep * a.q.sh + t * a.q.st + d;
@@ -200,31 +202,21 @@ __global__ void __launch_bounds__(256) swa_rotate_kernel(const SwaBlockArgs a) {
     put<N>(wk + spot(TN, t, e2), x2);
     put<N>(wv + spot(TN, t, e1), v1);
     put<N>(wv + spot(TN, t, e2), v2);
-    if (t < T) {
-      const int c1 = slot_of(e1), c2 = slot_of(e2);
+    const int c1 = slot_of(e1), c2 = slot_of(e2);
 #pragma unroll 4
-      for (int h = 0; h < rep; ++h) {
-        float2 q1 = {}, q2 = {};
-        if (in) {
-          q1 = ldn<XT, N>(qp + h * a.q.sh), q2 = ldn<XT, N>(qp + h * a.q.sh + half);
-          rotate(q1, q2, ang);
-        }
-        const int r = h * T + t;
-        bf16* hi = reinterpret_cast<bf16*>(ws) + (r / RQ) * (2 * RQ * LQ) + (r % RQ) * LQ;
-        put_split<N>(hi, hi + RQ * LQ, c1, q1);
-        put_split<N>(hi, hi + RQ * LQ, c2, q2);
+    for (int h = 0; h < rep; ++h) {
+      float2 q1 = {}, q2 = {};
+      if (in) {
+        q1 = ldn<XT, N>(qp + h * a.q.sh), q2 = ldn<XT, N>(qp + h * a.q.sh + half);
+        rotate(q1, q2, ang);
       }
-    }
-    // rows of the last pass beyond R: zeros, dealt to the block's rows
-    const int pads = (R + RQ - 1) / RQ * RQ - R;
-    for (int p = t; p < pads; p += TN) {
-      const int r = R + p;
+      const int r = h * T + t;
       bf16* hi = reinterpret_cast<bf16*>(ws) + (r / RQ) * (2 * RQ * LQ) + (r % RQ) * LQ;
-      put_split<N>(hi, hi + RQ * LQ, slot_of(e1), make_float2(0.f, 0.f));
-      put_split<N>(hi, hi + RQ * LQ, slot_of(e2), make_float2(0.f, 0.f));
+      put_split<N>(hi, hi + RQ * LQ, c1, q1);
+      put_split<N>(hi, hi + RQ * LQ, c2, q2);
     }
-  } else if (row < TN + a.Tp && d < half) {
-    const int t = row - TN, W = a.W;
+  } else if (row < T + a.Tp && d < half) {
+    const int t = row - T, W = a.W;
     const int n = a.count ? min(max(a.count[b], 0), a.Tp) : a.Tp;
     if (t >= n || t < n - W) return;  // of more accepted tokens than the window, the last W
     const XT* kp = static_cast<const XT*>(a.kp.p) + b * a.kp.sb + hk * a.kp.sh + t * a.kp.st + d;
@@ -628,7 +620,7 @@ int launch_attend(SwaBlockArgs& a, int B, cudaStream_t st) {
 
 template <typename XT, int DP, int QT>
 int launch_swa_block(SwaBlockArgs& a, bool pairs, int B, cudaStream_t st) {
-  const int rows = ((a.T + 15) & ~15) + a.Tp, per = DP / 2 / (pairs ? 2 : 1);
+  const int rows = a.T + a.Tp, per = DP / 2 / (pairs ? 2 : 1);
   const dim3 grid(ceil_div(rows * per, 256), a.Hkv, B);
   if (pairs)
     swa_rotate_kernel<XT, DP, QT, 2><<<grid, 256, 0, st>>>(a);
