@@ -17,7 +17,10 @@
 // test and races over its own piece of the one row that decides, and the
 // sequence's last block to finish writes the result. Keys of the race are
 // (score, ~index) in 64 bits under atomicMax, so no order of blocks can change
-// the answer.
+// the answer. Measured, 64 sequences of 7 drafts over 128256, bf16: 63 us, 45 of them
+// the statistics (246 MB, 5.5 TB/s); kernel 2 reads 64 MB in the other 18, behind the
+// join and before the last block's finish. (Prefetching its noise to L2 under kernel 1
+// took 66 us, two steps of its loads in flight 65: registers for resident warps.)
 #include <algorithm>
 
 #include "common.cuh"
@@ -144,8 +147,9 @@ struct Stat {
 __device__ __forceinline__ Stat join(Stat a, Stat b, float c) {
   const float m = fmaxf(a.m, b.m);
   if (m == -INFINITY) return {m, 0.f};
-  // a side with nothing left has m = -inf and s = 0
-  return {m, a.s * exp2f((a.m - m) * c) + b.s * exp2f((b.m - m) * c)};
+  // a side with nothing left has m = -inf and s = 0 (and c is 0 at an infinite temperature)
+  return {m, (a.s > 0.f ? a.s * exp2f((a.m - m) * c) : 0.f) +
+                 (b.s > 0.f ? b.s * exp2f((b.m - m) * c) : 0.f)};
 }
 
 // The same over a warp: the maximum first, then one rescale and a plain sum.
@@ -509,11 +513,11 @@ __global__ void __launch_bounds__(kT) verify_draw_kernel(const VerifyArgs a) {
       return need;
     };
     unsigned long long best = 0;
-    const auto evaluate = [&](int w0, unsigned int need) {
+    const auto evaluate = [&](int w0, unsigned int need) {  // may name tokens past the end
       const bool whole = vec && w0 + 256 <= j1;
       for (; need; need &= need - 1) {
         const int j = token(w0, whole, __ffs(need) - 1);
-        best = max(best, race_key(weight(j, true), ex[j], j));
+        if (j < j1) best = max(best, race_key(weight(j, true), ex[j], j));
       }
     };
     // the largest upper bounds of a lane: of one step, and of all its other steps

@@ -161,6 +161,34 @@ def test_masks_that_leave_nothing():
         assert acc[5] == 0
 
 
+@pytest.mark.parametrize("nothing", [-math.inf, math.nan])
+@pytest.mark.parametrize("V", [97, 300, 1000])
+def test_a_draft_without_probabilities_stays_inside_the_vocabulary(V, nothing):
+    """Draft rows masked throughout, in rows that go on past the vocabulary with large
+    logits and small noise: nothing past the end is looked at."""
+    from lizard_cuda import verify_drafts
+    B, K = 16, 2
+    args = list(inputs(B, K, V, torch.float32, 18))
+    args[1][:] = nothing
+    args[2][:] = -1
+    wide = [torch.full((B, n, V + 300), 60.0, device=DEV) for n in (K + 1, K)]
+    noise = torch.full((B, V + 300), 1e-9, device=DEV)
+    for w, a in zip(wide, args):
+        w[..., :V] = a
+    noise[:, :V] = args[4]
+    want, wacc = reference(*args)
+    out, acc = verify_drafts(wide[0][..., :V], wide[1][..., :V], *args[2:4], noise[:, :V])
+    assert not wacc.any() and torch.equal(acc.cpu(), wacc)
+    assert torch.equal(out.cpu(), want)
+
+
+def test_an_infinite_temperature_is_uniform_over_what_is_allowed():
+    args = list(inputs(6, 2, 9001, torch.float32, 19, masked=0.3))
+    args[0][:, :, 2000:7000] = -math.inf  # pieces of a row with nothing in them
+    args[1][:, :, 2000:7000] = -math.inf
+    check(args, temperature=torch.full((6,), math.inf, device=DEV))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_masks_of_the_types_lowest_value(dtype):
     """Forbidden tokens at finfo.min rather than -inf; a piece of the row, and a whole
