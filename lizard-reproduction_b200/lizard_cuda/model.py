@@ -159,7 +159,8 @@ def speculative_generate(model, draft, input_ids, steps, draft_len=4, temperatur
     whatever the draft. Both models are Lizard models with the same vocabulary.
     Returns the tokens [B, steps], the model's cache, settled on the tokens before
     the last one it emitted (a row may run a few tokens past `steps`), and how many
-    rounds it took."""
+    rounds it took. A row whose logits are NaN or masked throughout gets the token -1
+    there and goes on as after token 0."""
     dev, (B, L) = input_ids.device, input_ids.shape
     K = draft_len
     if not 1 <= K <= 63:
@@ -177,14 +178,15 @@ def speculative_generate(model, draft, input_ids, steps, draft_len=4, temperatur
     while int(have.min()) < steps:
         block, proposals = last, []
         for i in range(K):
-            proposals.append(draft(block, position_ids=pos + step[:i + 1], use_cache=False,
+            proposals.append(draft(block.clamp_min(0), position_ids=pos + step[:i + 1], use_cache=False,
                                    lizard_cache=draft_cache.draft(stand if i == 0 else none),
                                    logits_to_keep=1).logits[:, -1].to(logits.dtype))
             block = torch.cat([block, _draw(proposals[-1], temperature, generator)], 1)
         # the draft's own pass over the whole block, so that its cache can keep any prefix
-        draft(block, position_ids=pos + step, lizard_cache=draft_cache.draft(none),
+        fed = block.clamp_min(0)
+        draft(fed, position_ids=pos + step, lizard_cache=draft_cache.draft(none),
               use_cache=False, logits_to_keep=1)
-        logits = model(block, position_ids=pos + step, lizard_cache=cache.draft(stand),
+        logits = model(fed, position_ids=pos + step, lizard_cache=cache.draft(stand),
                        use_cache=False).logits
         uniforms = torch.rand(B, K, device=dev, generator=generator)
         noise = torch.empty(B, logits.shape[-1], device=dev).exponential_(generator=generator)

@@ -151,6 +151,29 @@ def test_speculative_sampling_follows_the_model():
     assert rows.shape[0] > 100 and chi < 45, chi
 
 
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+def test_speculative_with_a_draft_of_nan(temperature):
+    """A draft whose logits are NaN proposes nothing that stands: every round gives the
+    model's own token."""
+    from lizard_cuda.model import speculative_generate
+    model = _model()
+    draft = copy.deepcopy(model)
+    with torch.no_grad():
+        draft.lm_head.weight.fill_(float("nan"))
+    ids = torch.randint(0, 97, (2, 20), generator=torch.Generator().manual_seed(3)).to(DEV)
+    steps = 6
+    toks, cache, rounds = speculative_generate(
+        model, draft, ids, steps, draft_len=3, temperature=temperature,
+        generator=torch.Generator(device=DEV).manual_seed(7))
+    assert rounds == steps - 1 and int(toks.min()) >= 0
+    assert (cache[0].pos == 20 + steps - 1).all()
+    if temperature == 0:
+        with torch.no_grad():
+            full = model(torch.cat([ids, toks], 1), use_cache=False).logits[:, 19:-1].float()
+        got = full.gather(-1, toks[..., None])[..., 0]
+        assert (full.amax(-1) - got <= 2e-2 * full.abs().amax()).all()
+
+
 def test_speculative_refusals():
     from lizard_cuda.model import speculative_generate
     model = _model()
