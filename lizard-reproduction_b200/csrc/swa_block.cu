@@ -25,6 +25,11 @@
 // converted is written back to shared memory. (A warp on two row tiles converts a
 // key once instead of twice, but its registers leave 16 warps an SM for 20, and
 // the nine 16-key tiles of a window of 128 and its block do not divide over eight.)
+// Measured, 128 sequences of 8 key / value heads of 64, window 128, 32 query heads, 8
+// tokens: 48 us (85 MB, 1.8 TB/s), 45 of them this kernel: a fifth of its instructions are
+// the conversions, and 1024 CTAs leave the fullest SM 8 for a mean of 6.9. The ring in
+// smaller parts (16, 32, 64 KB) or fewer warps a CTA (4 .. 8), so that more CTAs fit
+// an SM, took 47 to 55 us: a long window is cut at 64 KB.
 //
 // Fragments. Within a step of 16 columns thread j takes d = 4j .. 4j+3 (the
 // queries are stored in that order), so a key is one 16-byte read; column tile i
@@ -223,7 +228,7 @@ __global__ void __launch_bounds__(256) swa_rotate_kernel(const SwaBlockArgs a) {
     const XT* vp = static_cast<const XT*>(a.vp.p) + b * a.vp.sb + hk * a.vp.sh + t * a.vp.st + d;
     float2 x1 = ldn<XT, N>(kp), x2 = ldn<XT, N>(kp + half);
     rotate(x1, x2, angle<N>(a.rot_p, b * a.rot_p.sb + (long long)t * D + d, half));
-    const int slot = (a.pos[b] % W + t) % W;
+    const int slot = (max(a.pos[b], 0) % W + t) % W;
     const size_t at = ((size_t)(b * a.Hkv + hk) * W + slot) * D + d;
     put<N>(a.kr + at, x1);
     put<N>(a.kr + at + half, x2);
@@ -314,7 +319,7 @@ swa_block_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__
         sV[spot(part, r, d)] = in ? vring[(size_t)slot * D + d] : 0.f;
       }
   };
-  const int pos = a.pos[b];
+  const int pos = max(a.pos[b], 0);
   const int n = a.Tp ? (a.count ? min(max(a.count[b], 0), a.Tp) : a.Tp) : 0;
   if (tid == 0) {
     tc::mbar_init(bar, 1);

@@ -132,9 +132,6 @@ def swa_decode(q, k, v, cos, sin, meta, k_ring, v_ring, pos):
     return y
 
 
-MAX_BLOCK = 64  # tokens a block
-
-
 def _pending_count(count, B, index):
     if count is None:
         return None
