@@ -26,17 +26,17 @@
 // output) and contracts the queries with them 32 rows at a time; the two halves of
 // F meet at the end, a row tile each. (8 columns by all of F needs no such meeting
 // but reads every key and query value twice as often from shared memory, which then
-// bounds the kernel.) Measured, 2048 states of 256 x 64, 32 query rows, 8 tokens: 80 us,
-// 4.2 TB/s of state and operands; what is left is the chain of phases of a CTA (load,
+// bounds the kernel.) Measured, 2048 states of 256 x 64, 32 query rows, 8 tokens: 81 us,
+// 4.1 TB/s of state and operands; what is left is the chain of phases of a CTA (load,
 // decays, update, products, meeting) at the two CTAs an SM that registers and shared
 // memory allow. A persistent form that loads the next state under this one's products
 // was slower (90 us): the rows of a batch accept different numbers of tokens, and
 // CTAs handed out one by one even that out.
 // The scores of the block's keys are shared: a quarter of F a warp, added through
 // shared memory. z rides along as two more keys (hi and lo): with M = [exp of the
-// decay from key to token, 0 above the diagonal | d_t for the two z columns], a' = (q K^T) o M has the row
-// sum as its own sum over all columns, and y = (d_t q S + a' V) / sum a' with zero
-// rows of V for z.
+// decay from key to token, 0 above the diagonal | d_t for the two z columns], a' =
+// (q K^T) o M has the row sum as its own sum over all columns, and y = (d_t q S + a' V) /
+// sum a' with zero rows of V for z.
 #include <algorithm>
 #include <type_traits>
 
@@ -155,6 +155,69 @@ __host__ __device__ inline BlockSmem block_smem(int KS, int HALVES, int T) {
   s.bar = (n + 7) & ~7, n = s.bar + 8;
   s.total = n + 1024;
   return s;
+}
+
+// One output by itself, from tokens 0 .. t only: y = (d q S + sum_{s <= t} a_s v_s) /
+// (d q z + sum a_s). The tensor cores give masked tokens a weight of zero, and 0 * inf
+// and 0 * NaN are NaN: where that may have happened (the output is NaN), a thread
+// comes here. q: the row's queries; S: the state's swizzled column tile and the column
+// in it; K: keys, then z hi and lo; V: this column of the values; M: the row's decays.
+__device__ __forceinline__ float alone(const bf16* q, const float* S, int col, const bf16* K,
+                                       int LD, const bf16* V, int LV, const float* M, int t, int T,
+                                       int F) {
+  float num = 0.f, den = 0.f;
+#pragma unroll 1
+  for (int f = 0; f < F; ++f) {
+    const float x = __bfloat162float(q[f]);
+    num = fmaf(x, S[f * 32 + ((((col >> 2) ^ (f & 7)) << 2) | (col & 3))], num);
+    den = fmaf(x, __bfloat162float(K[T * LD + f]) + __bfloat162float(K[(T + 1) * LD + f]), den);
+  }
+  num *= M[T], den *= M[T];
+#pragma unroll 1
+  for (int s = 0; s <= t && num == num && den == den; ++s) {
+    float a = 0.f;
+#pragma unroll 1
+    for (int f = 0; f < F; ++f)
+      a = fmaf(__bfloat162float(q[f]), __bfloat162float(K[s * LD + f]), a);
+    a *= M[s];
+    num = fmaf(a, __bfloat162float(V[s * LV]), num);
+    den += a;
+  }
+  return num / (den < kTiny ? kTiny : den);
+}
+
+__device__ __forceinline__ int special(int which) {
+  int v;
+  if (which == 0) asm volatile("mov.u32 %0, %%tid.x;\n" : "=r"(v));
+  if (which == 1) asm volatile("mov.u32 %0, %%ctaid.x;\n" : "=r"(v));
+  if (which == 2) asm volatile("mov.u32 %0, %%ctaid.y;\n" : "=r"(v));
+  if (which == 3) asm volatile("mov.u32 %0, %%ctaid.z;\n" : "=r"(v));
+  return v;
+}
+// A thread's outputs of rows r0 .. that are NaN, one by one. Everything is derived anew
+// (the volatile reads see to it), so that nothing of this is kept in registers before;
+// as a call it would cost every launch 15 %, here 1 %.
+template <int KS, int HALVES>
+__device__ __forceinline__ void redo(const GlaBlockArgs& a, const unsigned char* sm, int r0) {
+  constexpr int FP = 64 * KS, LD = FP + 8, DN = 32 * HALVES, LV = DN + 8;
+  const int T = a.T, TK = (T + 2 + 15) & ~15, R = a.rep * T;
+  const BlockSmem o = block_smem(KS, HALVES, T);
+  const int tid = special(0), lane = tid & 31, warp = tid >> 5;
+  const int cg = warp % (2 * HALVES), fh = warp / (2 * HALVES), d0 = special(3) * DN;
+  const size_t row0 = ((size_t)special(1) * a.H + special(2) * a.rep) * T;
+#pragma unroll 1
+  for (int e = 0; e < 8; ++e) {
+    const int row = r0 + fh * 16 + (lane >> 2) + (e >> 1 & 1) * 8, t = row % T;
+    const int dd = cg * 16 + (e >> 2) * 8 + 2 * (lane & 3) + (e & 1);
+    if (row >= R || d0 + dd >= a.D) continue;
+    bf16* yr = a.y + (row0 + row) * a.D + d0 + dd;
+    if (__hisnan(*yr))
+      *yr = __float2bfloat16_rn(alone(
+          a.fq + (row0 + row) * a.F, reinterpret_cast<const float*>(sm + (dd >> 5) * FP * 128),
+          dd & 31, reinterpret_cast<const bf16*>(sm + o.k), LD,
+          reinterpret_cast<const bf16*>(sm + o.v) + dd, LV,
+          reinterpret_cast<const float*>(sm + o.m) + t * TK, t, T, a.F));
+  }
 }
 
 // KS: F <= 64 KS. HALVES: 32-column groups of a CTA, four warps each.
@@ -500,6 +563,7 @@ gla_block_kernel(const __grid_constant__ CUtensorMap ts, const GlaBlockArgs a) {
                                                    fh ? x[0][i][2] : x[1][i][2],
                                                    fh ? x[0][i][3] : x[1][i][3]);
     __syncthreads();
+    float probe = 0.f;  // NaN once an output is not finite
     const int other = fh ? warp - 2 * HALVES : warp + 2 * HALVES, row = r0 + fh * 16 + g;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -516,10 +580,12 @@ gla_block_kernel(const __grid_constant__ CUtensorMap ts, const GlaBlockArgs a) {
           for (int e = 0; e < 2; ++e) {
             const float mine = fh ? x[1][i][2 * h + e] : x[0][i][2 * h + e];
             y[e] = (f.x * (mine + q[2 * h + e]) + out[i][2 * h + e]) * f.y;
+            probe = fmaf(y[e], 0.f, probe);
           }
           *reinterpret_cast<uint32_t*>(yr + 8 * h * D) = pack_bf16(y[0], y[1]);
         }
     }
+    if (probe != 0.f) redo<KS, HALVES>(a, sm, r0);
   }
   if (tid == 0) tc::bulk_wait_read0();  // the state has left shared memory
 }

@@ -258,6 +258,43 @@ __host__ __device__ inline SwaSmem swa_smem(int DP, int QT, int part, int T, int
   return s;
 }
 
+// Four outputs by themselves, from the keys that their row sees only. The tensor cores
+// give masked values a weight of zero, and 0 * inf and 0 * NaN are NaN: where that may
+// have happened (an output is NaN), a thread comes here. q: the row's queries, hi, with
+// lo after `lo`; kr, vr: the ring, `nr` of its W rows in use, the newest in slot `last`;
+// nk, nv: the block's keys and values in swizzled tiles of TN rows.
+__device__ __noinline__ float4 alone(const bf16* q, int lo, const float* kr, const float* vr,
+                                     int nr, int last, int W, const float* nk, const float* nv,
+                                     int TN, int t, int D, int d, const float* meta, int n_meta) {
+  const float scale = rsqrtf((float)D) * kLog2e;
+  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < n_meta; ++i) m = fmaxf(m, meta[i] * kLog2e);
+  for (int i = 0; i < n_meta; ++i) l += tc::ex2(meta[i] * kLog2e - m);
+  for (int i = 0; i < nr + t + 1 && l == l; ++i) {
+    const bool own = i >= nr;
+    const int back = last - i, k = own ? i - nr : i;
+    const int rel = own ? k : -1 - (back < 0 ? back + W : back);
+    if (rel <= t - W) continue;
+    float s = 0.f;
+    for (int e = 0; e < D; ++e) {
+      const int at = slot_of(e);
+      s = fmaf(__bfloat162float(q[at]) + __bfloat162float(q[lo + at]),
+               own ? nk[spot(TN, k, e)] : kr[(size_t)k * D + e], s);
+    }
+    s *= scale;
+    if (s == -INFINITY) continue;
+    const float mx = fmaxf(m, s), f = m > -INFINITY ? tc::ex2(m - mx) : 0.f, x = tc::ex2(s - mx);
+    m = mx;
+    l = l * f + x;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int at = d + c < D ? d + c : d;
+      o[c] = o[c] * f + x * (own ? nv[spot(TN, k, at)] : vr[(size_t)k * D + at]);
+    }
+  }
+  return make_float4(o[0] / l, o[1] / l, o[2] / l, o[3] / l);
+}
+
 // DP: D padded to whole 32s. QT: 16-row tiles of queries at once, one a warp.
 template <int DP, int QT>
 __global__ void __launch_bounds__(32 * kWarps, DP <= 64 ? 2 : 1)
@@ -541,6 +578,11 @@ swa_block_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__
         x.z += v.z;
         x.w += v.w;
       }
+      const float any = x.x + x.y + x.z + x.w;
+      if (any != any)
+        x = alone(reinterpret_cast<const bf16*>(ws + wo.q + (r0 / RQ) * kQBytes) + r * LQ, RQ * LQ,
+                  kring, vring, nr, last, W, reinterpret_cast<const float*>(ws + wo.k),
+                  reinterpret_cast<const float*>(ws + wo.v), TN, row % T, D, d, a.meta, a.n_meta);
       bf16* yr = a.y + ((size_t)(b * a.H + hk * rep) * T + row) * D + d;  // D is even
       *reinterpret_cast<uint32_t*>(yr) = pack_bf16(x.x, x.y);
       if (d + 2 < D) *reinterpret_cast<uint32_t*>(yr + 2) = pack_bf16(x.z, x.w);

@@ -150,6 +150,32 @@ def test_gla_block_with_closed_gates_and_an_empty_state():
     assert torch.equal(y, torch.zeros_like(y))
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("F,D,T,per_head", [(256, 64, 5, False), (93, 84, 13, True),
+                                            (32, 32, 40, False)])
+def test_gla_block_tokens_that_are_not_numbers(F, D, T, per_head, bad):
+    """A token with such a key or value leaves the tokens before it alone; pending ones
+    that do not stand leave no trace."""
+    from lizard_cuda.decode import gla_decode_block
+    fq, (fk, v, lg), (fkp, vp, lgp), count, S, z = _gla_inputs(3, 6, 3, F, D, T, 4, per_head, F)
+    count.fill_(2)
+    fkp[:, :, 2], vp[:, :, 3], lgp[..., 2] = bad, bad, math.nan
+    t = T // 2
+    fk[0, :, t, F // 3] = bad
+    v[1, :, t, :] = bad
+    v[2, 1, T - 1, 7] = bad
+    adv = _gla_walk(S.double(), z.double(), fkp, vp, lgp.nan_to_num(0), None, count)
+    ref = _gla_walk(adv[2], adv[3], fk, v, lg, fq)
+    y = gla_decode_block(fq, fk, v, lg, S, z, pending=(fkp, vp, lgp, count))
+    # (the walk's magnitudes of the state count every pending token)
+    assert S.isfinite().all() and z.isfinite().all()
+    want = ref[0].isfinite()
+    assert want[0, :, :t].all() and not want[0, :, t:].any() and not want[1, :, t:].any()
+    assert torch.equal(want, y.isfinite())
+    assert _rounds_to(y.masked_fill(~want, 0), ref[0].masked_fill(~want, 0),
+                      2.0 ** -14 * ref[1].masked_fill(~want, 0))
+
+
 def test_gla_block_agrees_with_gla_decode_and_repeats():
     from lizard_cuda.decode import gla_decode, gla_decode_block
     fq, (fk, v, lg), pend, count, S, z = _gla_inputs(2, 8, 2, 256, 64, 8, 8, False, 4)
@@ -201,7 +227,8 @@ def _swa_inputs(B, H, Hkv, W, D, T, Tp, dtype, pos, n_meta=4, seed=0, tables=tor
 
 
 def _check_swa(y, q, blk, pend, meta, kr0, vr0, pos, kr, vr):
-    """64-bit reference: write the accepted tokens, then attend token by token."""
+    """64-bit reference: write the accepted tokens, then attend token by token. Where a
+    value that the token sees is not a number, the output is not one either."""
     k, v, cos, sin = blk
     kp, vp, cp, sp, count = pend
     B, H, T, D = q.shape
@@ -226,10 +253,12 @@ def _check_swa(y, q, blk, pend, meta, kr0, vr0, pos, kr, vr):
             mag = torch.einsum("hnd,hd->hn", keys.abs(), qb[b, :, t].abs()).amax(-1) / D ** 0.5
             p = torch.softmax(torch.cat([x, meta.double().expand(H, -1)], -1), -1)[:, :n]
             ref = torch.einsum("hn,hnd->hd", p, vals)
-            top = vals.abs().amax((1, 2))
+            assert torch.equal(ref.isfinite(), y[b, :, t].isfinite()), (b, t)
+            ref, got = ref.nan_to_num(0, 0, 0), y[b, :, t].nan_to_num(0, 0, 0)
+            top = vals.nan_to_num(0, 0, 0).abs().amax((1, 2))
             # split products miss 3 2^-18 of the score's magnitude, twice in a quotient
             tol = (top * (mag * 6 * 2.0 ** -18 + 2.0 ** -14))[:, None]
-            assert _rounds_to(y[b, :, t], ref, tol), (b, t)
+            assert _rounds_to(got, ref, tol), (b, t)
 
 
 @pytest.mark.parametrize("B,H,Hkv,W,D,T,Tp,dtype,pos", [
@@ -249,6 +278,24 @@ def test_swa_block_matches_single_steps_in_64_bits(B, H, Hkv, W, D, T, Tp, dtype
     kr0, vr0 = kr.clone(), vr.clone()
     y = swa_decode_block(q, *blk, meta, kr, vr, pos, pending=pend)
     assert torch.isfinite(y).all()
+    _check_swa(y, q, blk, pend, meta, kr0, vr0, pos, kr, vr)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("W,T,D", [(64, 5, 64), (8, 11, 32), (37, 20, 62)])
+def test_swa_block_masked_values_that_are_not_numbers(W, T, D, bad):
+    """Values at masked places: of later tokens of the block, and of ring tokens that have
+    left the window of all or of some of the block's tokens."""
+    from lizard_cuda.decode import swa_decode_block
+    q, blk, pend, meta, kr, vr, pos = _swa_inputs(4, 4, 2, W, D, T, 2, torch.bfloat16,
+                                                  [3 * W, 3 * W, W + 5, 2], seed=W)
+    pend[4].zero_()
+    blk[1][0, :, T - 1, 3] = bad               # the last token of the block
+    blk[1][3, 1, T // 2] = bad
+    vr[1, :, 0] = bad                          # the oldest: no token of the block sees it
+    vr[2, 1, (5 + 2) % W, 5:9] = bad           # seen by the first two
+    kr0, vr0 = kr.clone(), vr.clone()
+    y = swa_decode_block(q, *blk, meta, kr, vr, pos, pending=pend)
     _check_swa(y, q, blk, pend, meta, kr0, vr0, pos, kr, vr)
 
 
