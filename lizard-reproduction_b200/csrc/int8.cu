@@ -28,6 +28,7 @@
 //     few warps, and their traffic slows the operands'.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 #include "tc.cuh"
@@ -72,22 +73,27 @@ __device__ __forceinline__ uint32_t code_of(float x, float inv) {
 __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
-__device__ __forceinline__ void store_codes(int8_t* p, const uint4& w, float inv, float) {
-  *reinterpret_cast<uint32_t*>(p) =
-      pack4(code_of(__uint_as_float(w.x), inv), code_of(__uint_as_float(w.y), inv),
-            code_of(__uint_as_float(w.z), inv), code_of(__uint_as_float(w.w), inv));
+// The codes of 16 bytes of x, the first in the lowest byte.
+__device__ __forceinline__ uint32_t codes_of(const uint4& w, float inv, float) {
+  return pack4(code_of(__uint_as_float(w.x), inv), code_of(__uint_as_float(w.y), inv),
+               code_of(__uint_as_float(w.z), inv), code_of(__uint_as_float(w.w), inv));
 }
-__device__ __forceinline__ void store_codes(int8_t* p, const uint4& w, float inv, bf16) {
-  *reinterpret_cast<uint2*>(p) =
-      make_uint2(pack4(code_of(bf16_lo(w.x), inv), code_of(bf16_hi(w.x), inv),
-                       code_of(bf16_lo(w.y), inv), code_of(bf16_hi(w.y), inv)),
-                 pack4(code_of(bf16_lo(w.z), inv), code_of(bf16_hi(w.z), inv),
-                       code_of(bf16_lo(w.w), inv), code_of(bf16_hi(w.w), inv)));
+__device__ __forceinline__ unsigned long long codes_of(const uint4& w, float inv, bf16) {
+  return pack4(code_of(bf16_lo(w.x), inv), code_of(bf16_hi(w.x), inv),
+               code_of(bf16_lo(w.y), inv), code_of(bf16_hi(w.y), inv)) |
+         (unsigned long long)pack4(code_of(bf16_lo(w.z), inv), code_of(bf16_hi(w.z), inv),
+                                   code_of(bf16_lo(w.w), inv), code_of(bf16_hi(w.w), inv)) << 32;
+}
+template <typename T>
+__device__ __forceinline__ void store_codes(int8_t* p, const uint4& w, float inv, T) {
+  const auto c = codes_of(w, inv, T());
+  *reinterpret_cast<std::remove_const_t<decltype(c)>*>(p) = c;
 }
 
 // ROW threads a row (a warp for short rows, the CTA for long ones): the row is read
-// once into registers, KEEP 16-byte vectors a thread (the part beyond, and rows that
-// do not start on 16 bytes, twice). The largest |x| is taken on the bits, where
+// once into registers, KEEP 16-byte vectors a thread (the part beyond twice). A row
+// that does not start on 16 bytes has a head of a few values before its vectors; codes
+// still leave in whole words, put together from two neighbours' vectors. The largest |x| is taken on the bits, where
 // infinities and NaN are larger than every number: such a row gets the scale NaN, and
 // so NaN outputs. Bound by memory: 32768 rows of 8192 bf16 in 117 us, 6.9 TB/s.
 template <typename T, int ROW, int KEEP>
@@ -102,9 +108,10 @@ i8_quantize_kernel(const T* __restrict__ x, long long ldx, int8_t* __restrict__ 
   if (m >= M) return;  // whole warps
   const T* row = x + m * ldx;
   int8_t* out = codes + m * ldc;
-  const bool vec = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
-  const int nv = vec ? K / V::N : 0;
-  const uint4* rv = reinterpret_cast<const uint4*>(row);
+  const int head =
+      min(K, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15) & 15) / sizeof(T)));
+  const int nv = (K - head) / V::N;
+  const uint4* rv = reinterpret_cast<const uint4*>(row + head);
   uint4 keep[KEEP];
   uint32_t top = 0;
 #pragma unroll
@@ -112,10 +119,11 @@ i8_quantize_kernel(const T* __restrict__ x, long long ldx, int8_t* __restrict__ 
     const int at = tid + i * ROW;
     keep[i] = at < nv ? __ldg(rv + at) : make_uint4(0, 0, 0, 0);
   }
+  if (tid < head) top = __float_as_uint(V::value(row + tid)) & 0x7fffffffu;
 #pragma unroll
   for (int i = 0; i < KEEP; ++i) top = max(top, V::top(keep[i]));
   for (int at = tid + KEEP * ROW; at < nv; at += ROW) top = max(top, V::top(rv[at]));
-  for (int k = nv * V::N + tid; k < K; k += ROW)
+  for (int k = head + nv * V::N + tid; k < K; k += ROW)
     top = max(top, __float_as_uint(V::value(row + k)) & 0x7fffffffu);
   top = __reduce_max_sync(0xffffffffu, top);
   if constexpr (ROW == kQT) {
@@ -133,13 +141,39 @@ i8_quantize_kernel(const T* __restrict__ x, long long ldx, int8_t* __restrict__ 
     for (int k = tid; k < ldc; k += ROW) out[k] = 0;
     return;
   }
+  if (head == 0) {
 #pragma unroll
-  for (int i = 0; i < KEEP; ++i) {
-    const int at = tid + i * ROW;
-    if (at < nv) store_codes(out + at * V::N, keep[i], inv, T());
+    for (int i = 0; i < KEEP; ++i) {
+      const int at = tid + i * ROW;
+      if (at < nv) store_codes(out + at * V::N, keep[i], inv, T());
+    }
+    for (int at = tid + KEEP * ROW; at < nv; at += ROW)
+      store_codes(out + at * V::N, rv[at], inv, T());
+  } else {
+    // word `at` holds the last `head` codes of vector at - 1 and the first of vector at
+    const auto word = [&](int at, const uint4& w) {
+      auto cur = codes_of(w, inv, T());
+      auto before = __shfl_up_sync(0xffffffffu, cur, 1);
+      if ((tid & 31) == 0 && at < nv) {
+        before = 0;
+        if (at)
+          before = codes_of(rv[at - 1], inv, T());
+        else
+          for (int k = 0; k < head; ++k)
+            before |= (decltype(cur))(code_of(V::value(row + k), inv) & 0xffu)
+                      << 8 * (V::N - head + k);
+      }
+      if (at < nv)
+        *reinterpret_cast<decltype(cur)*>(out + at * V::N) =
+            cur << 8 * head | before >> 8 * (V::N - head);
+    };
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) word(tid + i * ROW, keep[i]);
+    for (int at0 = (tid & ~31) + KEEP * ROW; at0 < nv; at0 += ROW) {
+      const int at = at0 + (tid & 31);
+      word(at, at < nv ? rv[at] : make_uint4(0, 0, 0, 0));
+    }
   }
-  for (int at = tid + KEEP * ROW; at < nv; at += ROW)
-    store_codes(out + at * V::N, rv[at], inv, T());
   for (int k = nv * V::N + tid; k < K; k += ROW)
     out[k] = (int8_t)(code_of(V::value(row + k), inv) & 0xffu);
   for (int k = K + tid; k < ldc; k += ROW) out[k] = 0;
@@ -334,6 +368,19 @@ __device__ __forceinline__ void quantize_here(const T* x, long long ldx, int M, 
   }
 }
 
+// `rows` values 128 apart in shared memory to a column of y, eight on their way at once.
+template <typename T>
+__device__ __forceinline__ void copy_column(T* y, int N, const T* from, int rows) {
+  for (int r0 = 0; r0 < rows; r0 += 8) {
+    T v[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) v[r] = from[min(r0 + r, rows - 1) * 128];
+#pragma unroll
+    for (int r = 0; r < 8; ++r, y += N)
+      if (r0 + r < rows) *y = v[r];
+  }
+}
+
 // Warps: 0 TMA, 1 MMA (and TMEM), 2..5 epilogue. split == 1: a CTA walks the (weight
 // tile, token tile) pairs blockIdx.x, + gridDim.x, ..., weight tiles fastest. split
 // > 1: clusters of `split` CTAs, one tile each, K dealt over the cluster. FUSE: x
@@ -494,14 +541,13 @@ i8_narrow_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__
           tc::named_bar_sync(1, 128);
           if (n < o.N) {
             const int rows = min(chunk, mt - c0);
+            const size_t at = (size_t)(m0 + c0) * o.N + n;
             if (o.y_bf16)
-              for (int r = 0; r < rows; ++r)
-                static_cast<bf16*>(o.y)[(size_t)(m0 + c0 + r) * o.N + n] =
-                    reinterpret_cast<const bf16*>(staging)[r * 128 + ch];
+              copy_column(static_cast<bf16*>(o.y) + at, o.N,
+                          reinterpret_cast<const bf16*>(staging) + ch, rows);
             else
-              for (int r = 0; r < rows; ++r)
-                static_cast<float*>(o.y)[(size_t)(m0 + c0 + r) * o.N + n] =
-                    reinterpret_cast<const float*>(staging)[r * 128 + ch];
+              copy_column(static_cast<float*>(o.y) + at, o.N,
+                          reinterpret_cast<const float*>(staging) + ch, rows);
           }
         }
       }
@@ -582,7 +628,73 @@ constexpr int kWS = 5;                       // operand stages
 constexpr int kWHalf = 128 * 128;            // bytes of one operand's half of a stage
 constexpr int kWStage = 2 * kWHalf;          // a CTA's bytes of a stage
 constexpr int kWStaging = 8 * 32 * 128;      // 32 rows x 128 bytes of y for each epilogue warp
-constexpr size_t kWSmem = 1024 + (size_t)kWS * kWStage + kWStaging + 2 * 256 * 4 + 256;
+constexpr size_t kWSmem = 1024 + (size_t)kWS * kWStage + kWStaging + 4 * 256 * 4 + 256;
+
+__device__ __forceinline__ void store2(void* p, uint32_t w) {
+  *static_cast<unsigned short*>(p) = (unsigned short)w;
+}
+// A warp's staging (32 rows of 128 swizzled bytes: columns cs .. of rows row0 ..) to a y
+// whose rows TMA cannot store: a row at a time, 4 bytes a lane; in rows of bf16 that
+// start off 4 bytes (N odd), a lane stores its upper value and its neighbour's lower one.
+// (2939 tokens, K = 73, bf16: N = 92615 368 us, value by value 726; N = 92616, by TMA, 234.)
+__device__ __forceinline__ void store_rows(const Out& o, const unsigned char* buf, int row0,
+                                           int cs) {
+  const int lane = threadIdx.x & 31, rows = min(32, o.M - row0), left = o.N - cs;
+  const auto word = [&](int r) {
+    return *reinterpret_cast<const uint32_t*>(buf + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) +
+                                              (lane & 3) * 4);
+  };
+  const int es = o.y_bf16 ? 2 : 4;
+  const int mine = left - lane * (4 / es);  // columns from this lane's on
+  const size_t pitch = (size_t)o.N * es;
+  unsigned char* y = static_cast<unsigned char*>(o.y) + ((size_t)row0 * o.N + cs) * es;
+  // rows first, first + step, ..., on a multiple of 4 bytes or 2 off one
+  const auto some = [&](int first, int step, bool off) {
+    unsigned char* to = y + first * pitch + 4 * lane;
+    const size_t by = step * pitch;
+    for (int r0 = first; r0 < rows; r0 += 8 * step, to += 8 * by) {
+      uint32_t w[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) w[r] = word(min(r0 + r * step, 31));
+      if (!off) {
+        if (4 <= mine * es) {
+#pragma unroll
+          for (int r = 0; r < 8; ++r)
+            if (r0 + r * step < rows) *reinterpret_cast<uint32_t*>(to + r * by) = w[r];
+        } else if (mine == 1) {
+#pragma unroll
+          for (int r = 0; r < 8; ++r)
+            if (r0 + r * step < rows) store2(to + r * by, w[r]);
+        }
+        continue;
+      }
+      if (lane == 0 && mine > 0) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          if (r0 + r * step < rows) store2(to + r * by, w[r]);
+      }
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        w[r] = __funnelshift_r(w[r], __shfl_down_sync(0xffffffffu, w[r], 1), 16);
+      if (lane < 31 && mine >= 3) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          if (r0 + r * step < rows) *reinterpret_cast<uint32_t*>(to + r * by + 2) = w[r];
+      } else if (mine >= 2) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          if (r0 + r * step < rows) store2(to + r * by + 2, w[r]);
+      }
+    }
+  };
+  const int odd = reinterpret_cast<uintptr_t>(y) >> 1 & 1;  // the first row's
+  if (pitch % 4 == 0) {
+    some(0, 1, odd);
+  } else {
+    some(odd, 2, false);
+    some(1 - odd, 2, true);
+  }
+}
 
 // Warps: 0 TMA, 1 MMA (and TMEM), 2..9 epilogue (two a lane quadrant, 128 columns each).
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1)
@@ -592,9 +704,8 @@ i8_wide_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ C
   unsigned char* sm = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* staging = sm + (size_t)kWS * kWStage;
-  float* sSb = reinterpret_cast<float*>(staging + kWStaging);  // [256] channel scales
-  float* sBias = sSb + 256;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sBias + 256);  // in the leader: both CTAs' bytes
+  float* scales = reinterpret_cast<float*>(staging + kWStaging);  // [2][scale, bias][256]
+  uint64_t* full = reinterpret_cast<uint64_t*>(scales + 4 * 256);  // in the leader: both CTAs' bytes
   uint64_t* empty = full + kWS;
   uint64_t* acc_full = empty + kWS;    // [2]
   uint64_t* acc_empty = acc_full + 2;  // [2], in the leader: the sixteen epilogue warps
@@ -680,18 +791,28 @@ i8_wide_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ C
     const int per = o.y_bf16 ? 64 : 32;  // columns a 128-byte row of the staging holds
     grid_dependency_wait();
     uint32_t at = 0;
+    // a tile's scales, loaded while the one before is written
+    float next_sa = 0.f, next_sb = 0.f, next_bias = 0.f;
+    const auto fetch = [&](int t) {
+      int m, n;
+      place(t, m, n);
+      m = m * 256 + rank * 128 + quad * 32 + lane;
+      n = n * 256 + etid;
+      next_sa = m < o.M ? o.sa[m] : 0.f;
+      next_sb = n < o.N ? o.sb[n] : 0.f;
+      next_bias = n < o.N ? bias_at(o, n) : 0.f;
+    };
+    if (cl < tiles) fetch(cl);
     for (int t = cl; t < tiles; t += ncl, ++at) {
       int mt, nt;
       place(t, mt, nt);
       const int buf = at & 1, n0 = nt * 256, row0 = mt * 256 + rank * 128 + quad * 32;
-      tc::named_bar_sync(1, 256);  // the scales of the tile before have been used
-      if (n0 + etid < o.N) {
-        sSb[etid] = o.sb[n0 + etid];
-        sBias[etid] = bias_at(o, n0 + etid);
-      }
-      const int row = row0 + lane;
-      const float sa = row < o.M ? o.sa[row] : 0.f;
-      tc::named_bar_sync(1, 256);
+      float *sSb = scales + buf * 512, *sBias = sSb + 256;
+      sSb[etid] = next_sb;
+      sBias[etid] = next_bias;
+      const float sa = next_sa;
+      tc::named_bar_sync(1, 256);  // (every warp is done with the tile before the last)
+      if (t + ncl < tiles) fetch(t + ncl);
       tc::mbar_wait(acc_full + buf, (at / 2) & 1, 133);
       tc::tc_fence_after();
       const uint32_t ta = tmem + buf * 256 + col0 + ((uint32_t)(quad * 32) << 16);
@@ -753,16 +874,7 @@ i8_wide_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ C
           }
         } else {
           __syncwarp();
-          for (int r = 0; r < 32 && row0 + r < o.M; ++r)
-            for (int c = lane; c < per && cs + c < o.N; c += 32) {
-              const size_t to = (size_t)(row0 + r) * o.N + cs + c;
-              if (o.y_bf16)
-                static_cast<bf16*>(o.y)[to] = *reinterpret_cast<const bf16*>(
-                    buf_y + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
-              else
-                static_cast<float*>(o.y)[to] = *reinterpret_cast<const float*>(
-                    buf_y + r * 128 + (((c >> 2) ^ (r & 7)) << 4) + (c & 3) * 4);
-            }
+          store_rows(o, buf_y, row0, cs);
           __syncwarp();
         }
       }

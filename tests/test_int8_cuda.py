@@ -69,6 +69,23 @@ def test_quantize_bit_for_bit(M, K, dtype):
     assert torch.equal(codes[1], want) and torch.equal(scale[0], wscale)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("K", [1, 5, 8, 31, 255, 1023, 2047, 2055, 4133, 9001])
+def test_quantize_rows_that_start_anywhere(K, dtype):
+    """Rows at every offset from 16 bytes (an odd row length runs through them), short
+    rows and such that a warp, and a block, keeps in part only; padding codes are zero."""
+    from lizard_cuda import int8_quantize
+    g = torch.Generator(device=DEV).manual_seed(K)
+    for off in (0, 1, 6):
+        flat = torch.randn(off + 19 * (K + 2 - K % 2 + 1), generator=g, device=DEV).to(dtype)
+        x = flat[off:].view(19, -1)[:, :K]
+        codes, scale = int8_quantize(x)
+        want, wscale = _quantize(x)
+        assert torch.equal(codes, want) and torch.equal(scale, wscale)
+        whole = codes.as_strided((19, codes.stride(0)), codes.stride())
+        assert not whole[:, K:].any()
+
+
 def test_quantize_rows_without_a_scale():
     from lizard_cuda import int8_linear, int8_quantize
     x = torch.randn(8, 100, device=DEV)
@@ -112,7 +129,8 @@ def test_matmul_bit_for_bit(M, K, N, dtype):
 @pytest.mark.parametrize("path", [1, 2])
 @pytest.mark.parametrize("M,K,N", [(1, 200, 300), (20, 16, 1), (100, 700, 2000), (300, 129, 257),
                                    (1000, 4096, 136), (260, 384, 5000), (3000, 65, 700),
-                                   (129, 300, 40000)])
+                                   (129, 300, 40000), (290, 73, 4097), (65, 140, 323),
+                                   (257, 100, 130)])
 def test_both_kernels_at_any_size(M, K, N, path):
     """Few and many tokens, tiles more and fewer than the machine holds, K in one step
     or split, y that TMA can and cannot write: both kernels give the same bits."""
