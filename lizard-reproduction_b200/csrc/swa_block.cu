@@ -319,8 +319,8 @@ swa_block_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__
   float* sSum = sMax + nw * 16;
   float* sCof = sSum + nw * 16;
   uint64_t* bar = reinterpret_cast<uint64_t*>(sm + o.bar);
-  const int b = blockIdx.x, hk = blockIdx.y, bk = b * a.Hkv + hk;
-  const int rep = a.rep, R = rep * T;
+  const int pass = blockIdx.x, b = blockIdx.y, hk = blockIdx.z, bk = b * a.Hkv + hk;
+  const int rep = a.rep, R = rep * T, r0 = pass * RQ;
   const float* kring = a.kr + (size_t)bk * W * D;
   const float* vring = a.vr + (size_t)bk * W * D;
   const int parts = (W + part - 1) / part;
@@ -329,9 +329,9 @@ swa_block_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__
   constexpr int kQBytes = 2 * RQ * LQ * 2;
   uint32_t phase = 0;
 
-  // ring rows [p part, (p + 1) part) into sK / sV; with the first part, the queries of
-  // pass `pass` and the new keys and values
-  const auto load = [&](int pass, int p) {
+  // ring rows [p part, (p + 1) part) into sK / sV; with the first part, the queries and
+  // the new keys and values
+  const auto load = [&](int p) {
     if (tid == 0 && (a.tma || !p)) {
       const int nb = TN * DP * 4;
       tc::mbar_expect_tx(bar, (a.tma ? 2 * part * DP * 4 : 0) + (p ? 0 : kQBytes + 2 * nb));
@@ -370,7 +370,7 @@ swa_block_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__
   const float sink1 = lane16 + 16 < a.n_meta ? a.meta[lane16 + 16] * kLog2e : -INFINITY;
   asm volatile("griddepcontrol.wait;\n" ::: "memory");  // the ring and the workspace are written
   if (tid == 0) asm volatile("fence.proxy.async;\n" ::: "memory");
-  load(0, 0);
+  load(0);
   __syncthreads();  // the barrier is initialised
 
   const int nr = (int)min((long long)pos + n, (long long)W);  // ring rows that hold a token
@@ -385,208 +385,201 @@ swa_block_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__
   const uint32_t aql = aqh + RQ * LQ * 2;
   bool live = true;  // after a timeout nothing is written
 
-  for (int r0 = 0; r0 < R; r0 += RQ) {
-    if (r0) {  // the merge of the rows before went over the keys: again
-      tc::fence_proxy_async_smem();
-      __syncthreads();
-      load(r0 / RQ, 0);
-    }
-    float m[2] = {-1e30f, -1e30f}, l[2] = {0.f, 0.f}, acc[4 * NG][4];
+  float m[2] = {-1e30f, -1e30f}, l[2] = {0.f, 0.f}, acc[4 * NG][4];
 #pragma unroll
-    for (int i = 0; i < 4 * NG; ++i)
+  for (int i = 0; i < 4 * NG; ++i)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) acc[i][c] = 0.f;
-    int tq[2];  // the tokens of this thread's rows
-    tq[0] = (r0 + rt * 16 + g) % T;
-    tq[1] = tq[0] + eight;
-    if (tq[1] >= T) tq[1] -= T;
+    for (int c = 0; c < 4; ++c) acc[i][c] = 0.f;
+  int tq[2];  // the tokens of this thread's rows
+  tq[0] = (r0 + rt * 16 + g) % T;
+  tq[1] = tq[0] + eight;
+  if (tq[1] >= T) tq[1] -= T;
 
-    for (int p = 0; p < parts; ++p) {
-      if (p) {
-        tc::fence_proxy_async_smem();
-        __syncthreads();  // the part before has been used
-        load(0, p);
+  for (int p = 0; p < parts; ++p) {
+    if (p) {
+      tc::fence_proxy_async_smem();
+      __syncthreads();  // the part before has been used
+      load(p);
+    }
+    if (a.tma || !p) {
+      live = tc::mbar_wait(bar, phase, 96) && live;
+      phase ^= 1;
+    }
+    if (!a.tma) __syncthreads();
+    const int held = min(max(nr - p * part, 0), part);  // rows of this part that hold a token
+    const int ring_tiles = (held + 15) >> 4;
+    const int tiles = ring_tiles + (p + 1 == parts ? TN >> 4 : 0);
+    for (int tl = kw; tl < tiles; tl += kws) {
+      const bool own = tl >= ring_tiles;
+      const int rows = own ? TN : part, row0 = (own ? tl - ring_tiles : tl) * 16;
+      const int lim = own ? T : held;  // rows beyond hold nothing (perhaps not numbers)
+      // this lane's places: key row krow, value rows of keys 2j and 2j + 1 (8 rows on
+      // and 16 columns on keep the swizzle's row and flip one bit of its chunk)
+      const float* kg = (own ? sNK : sK) + (row0 + krow) * 32;
+      const float *k0 = kg + ((j ^ krow) << 2), *k1 = kg + (((4 + j) ^ krow) << 2);
+      const float* vt = own ? sNV : sV;
+      const float* v0 = vt + (row0 + vrow0) * 32 + ((g ^ vrow0) << 2);
+      const float* v1 = vt + (row0 + vrow1) * 32 + ((g ^ vrow1) << 2);
+      // scores of 16 keys: hi hi, and the cross products in sums of their own (the
+      // chain of dependent products is what a warp waits for here)
+      float sc[2][4], sx[2][4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sc[i][c] = sx[i][c] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < NS; ++ks) {
+        uint32_t qh[4], ql[4];
+        ldsm_x4(qh, aqh + ks * 32);
+        ldsm_x4(ql, aql + ks * 32);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float4 x = *reinterpret_cast<const float4*>((ks & 1 ? k1 : k0) + 256 * i);
+          uint32_t kh[2], kl[2];
+          split2(x.x, x.y, kh[0], kl[0]);
+          split2(x.z, x.w, kh[1], kl[1]);
+          mma16816(sc[i], qh, kh[0], kh[1]);
+          mma16816(sx[i], qh, kl[0], kl[1]);
+          mma16816(sx[i], ql, kh[0], kh[1]);
+        }
+        if (ks & 1) k0 += rows * 32, k1 += rows * 32;
       }
-      if (a.tma || !p) {
-        live = tc::mbar_wait(bar, phase, 96) && live;
-        phase ^= 1;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sc[i][c] += sx[i][c];
+      // position - base of this thread's keys 8 i + 2 j + c; a ring slot holds the
+      // last position before base that falls on it
+      int rel[4];
+      bool clear = true;  // every row of the tile sees every key
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = row0 + (i >> 1) * 8 + (i & 1 ? vrow1 : vrow0);
+        const int back = last - (p * part + k);
+        rel[i] = own ? k : -1 - (back < 0 ? back + W : back);
+        if (k >= lim) rel[i] = 1 << 30;
+        clear = clear && rel[i] < 0 && rel[i] >= T - W;
       }
-      if (!a.tma) __syncthreads();
-      const int held = min(max(nr - p * part, 0), part);  // rows of this part that hold a token
-      const int ring_tiles = (held + 15) >> 4;
-      const int tiles = ring_tiles + (p + 1 == parts ? TN >> 4 : 0);
-      for (int tl = kw; tl < tiles; tl += kws) {
-        const bool own = tl >= ring_tiles;
-        const int rows = own ? TN : part, row0 = (own ? tl - ring_tiles : tl) * 16;
-        const int lim = own ? T : held;  // rows beyond hold nothing (perhaps not numbers)
-        // this lane's places: key row krow, value rows of keys 2j and 2j + 1 (8 rows on
-        // and 16 columns on keep the swizzle's row and flip one bit of its chunk)
-        const float* kg = (own ? sNK : sK) + (row0 + krow) * 32;
-        const float *k0 = kg + ((j ^ krow) << 2), *k1 = kg + (((4 + j) ^ krow) << 2);
-        const float* vt = own ? sNV : sV;
-        const float* v0 = vt + (row0 + vrow0) * 32 + ((g ^ vrow0) << 2);
-        const float* v1 = vt + (row0 + vrow1) * 32 + ((g ^ vrow1) << 2);
-        // scores of 16 keys: hi hi, and the cross products in sums of their own (the
-        // chain of dependent products is what a warp waits for here)
-        float sc[2][4], sx[2][4];
+      if (!__all_sync(0xffffffffu, clear)) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) sc[i][c] = sx[i][c] = 0.f;
+          for (int i = 0; i < 4; ++i)
+            if (rel[i] > tq[h] || rel[i] <= tq[h] - W) sc[i >> 1][2 * h + (i & 1)] = -INFINITY;
+      }
+      uint32_t ph[4], pl[4];
 #pragma unroll
-        for (int ks = 0; ks < NS; ++ks) {
-          uint32_t qh[4], ql[4];
-          ldsm_x4(qh, aqh + ks * 32);
-          ldsm_x4(ql, aql + ks * 32);
+      for (int h = 0; h < 2; ++h) {
+        float mx = fmaxf(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]),
+                         fmaxf(sc[1][2 * h], sc[1][2 * h + 1]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        mx = fmaxf(mx * scale, m[h]);
+        if (tl != kw || p) {  // not the first keys: rescale
+          const float f = tc::ex2(m[h] - mx);
+          l[h] *= f;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float4 x = *reinterpret_cast<const float4*>((ks & 1 ? k1 : k0) + 256 * i);
-            uint32_t kh[2], kl[2];
-            split2(x.x, x.y, kh[0], kl[0]);
-            split2(x.z, x.w, kh[1], kl[1]);
-            mma16816(sc[i], qh, kh[0], kh[1]);
-            mma16816(sx[i], qh, kl[0], kl[1]);
-            mma16816(sx[i], ql, kh[0], kh[1]);
-          }
-          if (ks & 1) k0 += rows * 32, k1 += rows * 32;
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) sc[i][c] += sx[i][c];
-        // position - base of this thread's keys 8 i + 2 j + c; a ring slot holds the
-        // last position before base that falls on it
-        int rel[4];
-        bool clear = true;  // every row of the tile sees every key
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int k = row0 + (i >> 1) * 8 + (i & 1 ? vrow1 : vrow0);
-          const int back = last - (p * part + k);
-          rel[i] = own ? k : -1 - (back < 0 ? back + W : back);
-          if (k >= lim) rel[i] = 1 << 30;
-          clear = clear && rel[i] < 0 && rel[i] >= T - W;
-        }
-        if (!__all_sync(0xffffffffu, clear)) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (rel[i] > tq[h] || rel[i] <= tq[h] - W) sc[i >> 1][2 * h + (i & 1)] = -INFINITY;
-        }
-        uint32_t ph[4], pl[4];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float mx = fmaxf(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]),
-                           fmaxf(sc[1][2 * h], sc[1][2 * h + 1]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          mx = fmaxf(mx * scale, m[h]);
-          if (tl != kw || p) {  // not the first keys: rescale
-            const float f = tc::ex2(m[h] - mx);
-            l[h] *= f;
-#pragma unroll
-            for (int i = 0; i < 4 * NG; ++i) {
-              acc[i][2 * h] *= f;
-              acc[i][2 * h + 1] *= f;
-            }
-          }
-          m[h] = mx;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float x0 = tc::ex2(fmaf(sc[i][2 * h], scale, -mx));
-            const float x1 = tc::ex2(fmaf(sc[i][2 * h + 1], scale, -mx));
-            l[h] += x0 + x1;
-            split2(x0, x1, ph[2 * i + h], pl[2 * i + h]);
+          for (int i = 0; i < 4 * NG; ++i) {
+            acc[i][2 * h] *= f;
+            acc[i][2 * h + 1] *= f;
           }
         }
-        // values: rows of keys 2j, 2j + 1, 2j + 8, 2j + 9, columns 4 g .. 4 g + 3 of each 32
+        m[h] = mx;
 #pragma unroll
-        for (int q = 0; q < NG; ++q) {
-          float4 x[4];
+        for (int i = 0; i < 2; ++i) {
+          const float x0 = tc::ex2(fmaf(sc[i][2 * h], scale, -mx));
+          const float x1 = tc::ex2(fmaf(sc[i][2 * h + 1], scale, -mx));
+          l[h] += x0 + x1;
+          split2(x0, x1, ph[2 * i + h], pl[2 * i + h]);
+        }
+      }
+      // values: rows of keys 2j, 2j + 1, 2j + 8, 2j + 9, columns 4 g .. 4 g + 3 of each 32
+#pragma unroll
+      for (int q = 0; q < NG; ++q) {
+        float4 x[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          x[u] = *reinterpret_cast<const float4*>((u & 1 ? v1 : v0) + 256 * (u >> 1));
+        v0 += rows * 32, v1 += rows * 32;
+        if (row0 + 16 > lim) {
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            x[u] = *reinterpret_cast<const float4*>((u & 1 ? v1 : v0) + 256 * (u >> 1));
-          v0 += rows * 32, v1 += rows * 32;
-          if (row0 + 16 > lim) {
+            if (row0 + (u & 1 ? vrow1 : vrow0) + (u >> 1) * 8 >= lim)
+              x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-              if (row0 + (u & 1 ? vrow1 : vrow0) + (u >> 1) * 8 >= lim)
-                x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-          }
+        for (int i = 0; i < 4; ++i) {
+          uint32_t vh[2], vl[2];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t vh[2], vl[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-              split2(reinterpret_cast<const float*>(&x[2 * u])[i],
-                     reinterpret_cast<const float*>(&x[2 * u + 1])[i], vh[u], vl[u]);
-            mma16816(acc[4 * q + i], ph, vh[0], vh[1]);
-            mma16816(acc[4 * q + i], ph, vl[0], vl[1]);
-            mma16816(acc[4 * q + i], pl, vh[0], vh[1]);
-          }
+          for (int u = 0; u < 2; ++u)
+            split2(reinterpret_cast<const float*>(&x[2 * u])[i],
+                   reinterpret_cast<const float*>(&x[2 * u + 1])[i], vh[u], vl[u]);
+          mma16816(acc[4 * q + i], ph, vh[0], vh[1]);
+          mma16816(acc[4 * q + i], ph, vl[0], vl[1]);
+          mma16816(acc[4 * q + i], pl, vh[0], vh[1]);
         }
       }
     }
-    // the warps meet: a coefficient for each warp's row, from the common maximum and
-    // sum and the sinks, then the outputs times it, written over the keys and added
+  }
+  // the warps meet: a coefficient for each warp's row, from the common maximum and
+  // sum and the sinks, then the outputs times it, written over the keys and added
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-      if (j == 0) {
-        sMax[warp * 16 + g + 8 * h] = m[h];
-        sSum[warp * 16 + g + 8 * h] = l[h];
-      }
+  for (int h = 0; h < 2; ++h) {
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+    if (j == 0) {
+      sMax[warp * 16 + g + 8 * h] = m[h];
+      sSum[warp * 16 + g + 8 * h] = l[h];
     }
-    __syncthreads();
-    for (int e = tid >> 4; e < RQ; e += nt >> 4) {  // a row a half warp, a lane a warp of its tile
-      const int w = (lane16 * QT + (e >> 4)), at = w * 16 + (e & 15);
-      const bool in = lane16 < kws;
-      const float mw = in ? sMax[at] : -1e30f;
-      float top = fmaxf(mw, fmaxf(sink0, sink1));
+  }
+  __syncthreads();
+  for (int e = tid >> 4; e < RQ; e += nt >> 4) {  // a row a half warp, a lane a warp of its tile
+    const int w = (lane16 * QT + (e >> 4)), at = w * 16 + (e & 15);
+    const bool in = lane16 < kws;
+    const float mw = in ? sMax[at] : -1e30f;
+    float top = fmaxf(mw, fmaxf(sink0, sink1));
 #pragma unroll
-      for (int x = 1; x < 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-      const float f = tc::ex2(mw - top);
-      float sum = (in ? f * sSum[at] : 0.f) + tc::ex2(sink0 - top) + tc::ex2(sink1 - top);
+    for (int x = 1; x < 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    const float f = tc::ex2(mw - top);
+    float sum = (in ? f * sSum[at] : 0.f) + tc::ex2(sink0 - top) + tc::ex2(sink1 - top);
 #pragma unroll
-      for (int x = 1; x < 16; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-      if (in) sCof[at] = f / sum;
+    for (int x = 1; x < 16; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    if (in) sCof[at] = f / sum;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const float f = sCof[warp * 16 + g + 8 * h];
+    float* row = sO + (warp * 16 + g + 8 * h) * LO + 8 * j;
+#pragma unroll
+    for (int q = 0; q < NG; ++q)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)  // columns 8 j + 4 u + (0 .. 3)
+        *reinterpret_cast<float4*>(row + 32 * q + 4 * u) =
+            make_float4(f * acc[4 * q][2 * h + u], f * acc[4 * q + 1][2 * h + u],
+                        f * acc[4 * q + 2][2 * h + u], f * acc[4 * q + 3][2 * h + u]);
+  }
+  __syncthreads();
+  for (int e = tid; e < RQ * (DP / 4); e += nt) {
+    const int r = e / (DP / 4), d = (e - r * (DP / 4)) * 4, row = r0 + r;
+    if (row >= R || d >= D || !live) continue;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = 0; w < kws; ++w) {
+      const float4 v = *reinterpret_cast<const float4*>(
+          sO + ((w * QT + (r >> 4)) * 16 + (r & 15)) * LO + d);
+      x.x += v.x;
+      x.y += v.y;
+      x.z += v.z;
+      x.w += v.w;
     }
-    __syncthreads();
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float f = sCof[warp * 16 + g + 8 * h];
-      float* row = sO + (warp * 16 + g + 8 * h) * LO + 8 * j;
-#pragma unroll
-      for (int q = 0; q < NG; ++q)
-#pragma unroll
-        for (int u = 0; u < 2; ++u)  // columns 8 j + 4 u + (0 .. 3)
-          *reinterpret_cast<float4*>(row + 32 * q + 4 * u) =
-              make_float4(f * acc[4 * q][2 * h + u], f * acc[4 * q + 1][2 * h + u],
-                          f * acc[4 * q + 2][2 * h + u], f * acc[4 * q + 3][2 * h + u]);
-    }
-    __syncthreads();
-    for (int e = tid; e < RQ * (DP / 4); e += nt) {
-      const int r = e / (DP / 4), d = (e - r * (DP / 4)) * 4, row = r0 + r;
-      if (row >= R || d >= D || !live) continue;
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int w = 0; w < kws; ++w) {
-        const float4 v = *reinterpret_cast<const float4*>(
-            sO + ((w * QT + (r >> 4)) * 16 + (r & 15)) * LO + d);
-        x.x += v.x;
-        x.y += v.y;
-        x.z += v.z;
-        x.w += v.w;
-      }
-      const float any = x.x + x.y + x.z + x.w;
-      if (any != any)
-        x = alone(reinterpret_cast<const bf16*>(ws + wo.q + (r0 / RQ) * kQBytes) + r * LQ, RQ * LQ,
-                  kring, vring, nr, last, W, reinterpret_cast<const float*>(ws + wo.k),
-                  reinterpret_cast<const float*>(ws + wo.v), TN, row % T, D, d, a.meta, a.n_meta);
-      bf16* yr = a.y + ((size_t)(b * a.H + hk * rep) * T + row) * D + d;  // D is even
-      *reinterpret_cast<uint32_t*>(yr) = pack_bf16(x.x, x.y);
-      if (d + 2 < D) *reinterpret_cast<uint32_t*>(yr + 2) = pack_bf16(x.z, x.w);
-    }
+    const float any = x.x + x.y + x.z + x.w;
+    if (any != any)
+      x = alone(reinterpret_cast<const bf16*>(ws + wo.q + pass * kQBytes) + r * LQ, RQ * LQ,
+                kring, vring, nr, last, W, reinterpret_cast<const float*>(ws + wo.k),
+                reinterpret_cast<const float*>(ws + wo.v), TN, row % T, D, d, a.meta, a.n_meta);
+    bf16* yr = a.y + ((size_t)(b * a.H + hk * rep) * T + row) * D + d;  // D is even
+    *reinterpret_cast<uint32_t*>(yr) = pack_bf16(x.x, x.y);
+    if (d + 2 < D) *reinterpret_cast<uint32_t*>(yr + 2) = pack_bf16(x.z, x.w);
   }
 }
 
@@ -652,7 +645,7 @@ int launch_attend(SwaBlockArgs& a, int B, cudaStream_t st) {
     done[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(B, a.Hkv);
+  cfg.gridDim = dim3(ceil_div(a.rep * a.T, 16 * QT), B, a.Hkv);
   cfg.blockDim = dim3(32 * warps);
   cfg.dynamicSmemBytes = swa_smem(DP, QT, a.part, a.T, warps).total;
   cfg.stream = st;
