@@ -28,7 +28,6 @@
 //     few warps, and their traffic slows the operands'.
 #include <algorithm>
 #include <atomic>
-#include <type_traits>
 
 #include "common.cuh"
 #include "tc.cuh"
@@ -84,10 +83,28 @@ __device__ __forceinline__ unsigned long long codes_of(const uint4& w, float inv
          (unsigned long long)pack4(code_of(bf16_lo(w.z), inv), code_of(bf16_hi(w.z), inv),
                                    code_of(bf16_lo(w.w), inv), code_of(bf16_hi(w.w), inv)) << 32;
 }
+// Word `at` of the codes of a row that does not start on 16 bytes (`head` values, then the
+// nv vectors rv): the last `head` codes of the vector before and the first ones of w,
+// vector `at`. By a whole warp with consecutive `at`.
 template <typename T>
-__device__ __forceinline__ void store_codes(int8_t* p, const uint4& w, float inv, T) {
-  const auto c = codes_of(w, inv, T());
-  *reinterpret_cast<std::remove_const_t<decltype(c)>*>(p) = c;
+__device__ __forceinline__ auto code_word(const T* row, const uint4* rv, int head, int nv, int at,
+                                          const uint4& w, float inv) {
+  constexpr int N = Vec<T>::N;
+  auto cur = codes_of(w, inv, T()), before = __shfl_up_sync(0xffffffffu, cur, 1);
+  if ((threadIdx.x & 31) == 0 && at < nv) {
+    before = 0;
+    if (at)
+      before = codes_of(__ldg(rv + at - 1), inv, T());
+    else
+      for (int k = 0; k < head; ++k)
+        before |= (decltype(cur))(code_of(Vec<T>::value(row + k), inv) & 0xffu)
+                  << 8 * (N - head + k);
+  }
+  return cur << 8 * head | before >> 8 * (N - head);
+}
+template <typename T>
+__device__ __forceinline__ int head_of(const T* row, int K) {
+  return min(K, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15) & 15) / sizeof(T)));
 }
 
 // ROW threads a row (a warp for short rows, the CTA for long ones): the row is read
@@ -108,9 +125,7 @@ i8_quantize_kernel(const T* __restrict__ x, long long ldx, int8_t* __restrict__ 
   if (m >= M) return;  // whole warps
   const T* row = x + m * ldx;
   int8_t* out = codes + m * ldc;
-  const int head =
-      min(K, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15) & 15) / sizeof(T)));
-  const int nv = (K - head) / V::N;
+  const int head = head_of(row, K), nv = (K - head) / V::N;
   const uint4* rv = reinterpret_cast<const uint4*>(row + head);
   uint4 keep[KEEP];
   uint32_t top = 0;
@@ -141,37 +156,20 @@ i8_quantize_kernel(const T* __restrict__ x, long long ldx, int8_t* __restrict__ 
     for (int k = tid; k < ldc; k += ROW) out[k] = 0;
     return;
   }
+  const auto put = [&](int at, decltype(codes_of(keep[0], inv, T())) c) {
+    if (at < nv) *reinterpret_cast<decltype(c)*>(out + at * V::N) = c;
+  };
   if (head == 0) {
 #pragma unroll
-    for (int i = 0; i < KEEP; ++i) {
-      const int at = tid + i * ROW;
-      if (at < nv) store_codes(out + at * V::N, keep[i], inv, T());
-    }
-    for (int at = tid + KEEP * ROW; at < nv; at += ROW)
-      store_codes(out + at * V::N, rv[at], inv, T());
+    for (int i = 0; i < KEEP; ++i) put(tid + i * ROW, codes_of(keep[i], inv, T()));
+    for (int at = tid + KEEP * ROW; at < nv; at += ROW) put(at, codes_of(rv[at], inv, T()));
   } else {
-    // word `at` holds the last `head` codes of vector at - 1 and the first of vector at
-    const auto word = [&](int at, const uint4& w) {
-      auto cur = codes_of(w, inv, T());
-      auto before = __shfl_up_sync(0xffffffffu, cur, 1);
-      if ((tid & 31) == 0 && at < nv) {
-        before = 0;
-        if (at)
-          before = codes_of(rv[at - 1], inv, T());
-        else
-          for (int k = 0; k < head; ++k)
-            before |= (decltype(cur))(code_of(V::value(row + k), inv) & 0xffu)
-                      << 8 * (V::N - head + k);
-      }
-      if (at < nv)
-        *reinterpret_cast<decltype(cur)*>(out + at * V::N) =
-            cur << 8 * head | before >> 8 * (V::N - head);
-    };
 #pragma unroll
-    for (int i = 0; i < KEEP; ++i) word(tid + i * ROW, keep[i]);
+    for (int i = 0; i < KEEP; ++i)
+      put(tid + i * ROW, code_word(row, rv, head, nv, tid + i * ROW, keep[i], inv));
     for (int at0 = (tid & ~31) + KEEP * ROW; at0 < nv; at0 += ROW) {
       const int at = at0 + (tid & 31);
-      word(at, at < nv ? rv[at] : make_uint4(0, 0, 0, 0));
+      put(at, code_word(row, rv, head, nv, at, at < nv ? rv[at] : make_uint4(0, 0, 0, 0), inv));
     }
   }
   for (int k = nv * V::N + tid; k < K; k += ROW)
@@ -330,17 +328,17 @@ __device__ __forceinline__ void quantize_here(const T* x, long long ldx, int M, 
   };
   for (int m = w; m < M; m += 4) {
     const T* row = x + m * ldx;
-    const int nv = (reinterpret_cast<uintptr_t>(row) & 15) == 0 ? K / V::N : 0;
-    const uint4* rv = reinterpret_cast<const uint4*>(row);
+    const int head = head_of(row, K), nv = (K - head) / V::N;
+    const uint4* rv = reinterpret_cast<const uint4*>(row + head);
     uint4 keep[KEEP];
-    uint32_t top = 0;
+    uint32_t top = lane < head ? __float_as_uint(V::value(row + lane)) & 0x7fffffffu : 0;
 #pragma unroll
     for (int i = 0; i < KEEP; ++i)
       keep[i] = lane + 32 * i < nv ? __ldg(rv + lane + 32 * i) : make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int i = 0; i < KEEP; ++i) top = max(top, V::top(keep[i]));
     for (int i = lane + 32 * KEEP; i < nv; i += 32) top = max(top, V::top(__ldg(rv + i)));
-    for (int k = nv * V::N + lane; k < K; k += 32)
+    for (int k = head + nv * V::N + lane; k < K; k += 32)
       top = max(top, __float_as_uint(V::value(row + k)) & 0x7fffffffu);
     top = __reduce_max_sync(0xffffffffu, top);
     const float t = __uint_as_float(top);
@@ -351,16 +349,19 @@ __device__ __forceinline__ void quantize_here(const T* x, long long ldx, int M, 
       for (int k = k0 + lane; k < k1; k += 32) *at(m, k) = 0;
       continue;
     }
-#pragma unroll
-    for (int i = 0; i < KEEP; ++i) {
-      const int k = (lane + 32 * i) * V::N;
-      if (lane + 32 * i < nv && k >= k0 && k < k1)
-        store_codes(reinterpret_cast<int8_t*>(at(m, k)), keep[i], inv, T());
-    }
-    for (int i = lane + 32 * KEEP; i < nv; i += 32) {
+    const auto put = [&](int i, decltype(codes_of(keep[0], inv, T())) c) {
       const int k = i * V::N;
-      if (k >= k0 && k < k1)
-        store_codes(reinterpret_cast<int8_t*>(at(m, k)), __ldg(rv + i), inv, T());
+      if (i < nv && k >= k0 && k < k1) *reinterpret_cast<decltype(c)*>(at(m, k)) = c;
+    };
+    if (head == 0) {
+#pragma unroll
+      for (int i = 0; i < KEEP; ++i) put(lane + 32 * i, codes_of(keep[i], inv, T()));
+      for (int i = lane + 32 * KEEP; i < nv; i += 32) put(i, codes_of(__ldg(rv + i), inv, T()));
+    } else {  // read again: the kept vectors in registers would weigh on the rows above
+#pragma unroll 2
+      for (int i = lane; i < (nv + 31 & ~31); i += 32)
+        put(i, code_word(row, rv, head, nv, i, i < nv ? __ldg(rv + i) : make_uint4(0, 0, 0, 0),
+                         inv));
     }
     for (int k = nv * V::N + lane; k < K; k += 32)
       if (k >= k0 && k < k1)
