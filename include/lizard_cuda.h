@@ -604,6 +604,20 @@ int lz_int8_linear(const void* x, int x_dtype, long long x_ld, const void* w, lo
                    const float* w_scale, const void* bias, int bias_dtype, void* y, int y_dtype,
                    void* workspace, size_t workspace_bytes, int M, int N, int K, void* stream);
 
+/* The entries above with their arguments as 64-bit words, for bindings in which
+ * converting twenty to thirty arguments costs more than a small launch. words[i] is
+ * argument i: an address, an integer, a float as the bits of a double; strides as
+ * their index in words (0 = null), where they follow the arguments. Same results
+ * and errors as the entry itself. */
+enum {
+  LZ_CALL_GLA_DECODE_BLOCK = 1,
+  LZ_CALL_SWA_DECODE_BLOCK = 2,
+  LZ_CALL_VERIFY_DRAFTS = 3,
+  LZ_CALL_INT8_MATMUL = 4,
+  LZ_CALL_INT8_LINEAR = 5
+};
+int lz_call(int entry, const long long* words, int n_words);
+
 #ifdef __cplusplus
 }
 #endif

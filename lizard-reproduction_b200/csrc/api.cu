@@ -1,6 +1,10 @@
 // extern "C" entry points declared in include/lizard_cuda.h: argument
 // validation, carving of caller-owned buffers, dispatch to the kernels.
 #include <algorithm>
+#include <cstring>
+#include <tuple>
+#include <type_traits>
+#include <utility>
 
 #include "common.cuh"
 #include "gla_layout.h"
@@ -77,6 +81,64 @@ extern "C" int lz_device_timeout_clear(void) {
     if (rc) return rc;
   }
   return LZ_OK;
+}
+
+namespace {
+
+// Argument i of an entry from its 64-bit word.
+struct Words {
+  const long long* w;
+  int n;
+  bool ok;
+};
+template <typename A>
+A word(Words& x, size_t i) {
+  const long long v = x.w[i];
+  if constexpr (std::is_same_v<A, const long long*>) {  // strides: their place in the words
+    x.ok = x.ok && v >= 0 && (v == 0 || v + 8 <= x.n);
+    return v > 0 && x.ok ? x.w + v : nullptr;
+  } else if constexpr (std::is_pointer_v<A>) {
+    return reinterpret_cast<A>(static_cast<uintptr_t>(v));
+  } else if constexpr (std::is_floating_point_v<A>) {
+    double d;
+    std::memcpy(&d, &v, sizeof(d));
+    return static_cast<A>(d);
+  } else {
+    x.ok = x.ok && static_cast<long long>(static_cast<A>(v)) == v;
+    return static_cast<A>(v);
+  }
+}
+template <typename... A, size_t... I>
+int call(int (*entry)(A...), Words x, std::index_sequence<I...>) {
+  LZ_REQUIRE(x.n >= (int)sizeof...(A), LZ_ERR_INVALID_ARGUMENT, "too few words for the entry");
+  const std::tuple<A...> args{word<A>(x, I)...};
+  LZ_REQUIRE(x.ok, LZ_ERR_INVALID_ARGUMENT, "a word does not fit its argument");
+  return std::apply(entry, args);
+}
+template <typename... A>
+int call(int (*entry)(A...), const long long* w, int n) {
+  return call(entry, Words{w, n, true}, std::index_sequence_for<A...>());
+}
+
+}  // namespace
+
+extern "C" int lz_call(int entry, const long long* words, int n_words) {
+  lz::clear_error();
+  LZ_REQUIRE(words, LZ_ERR_INVALID_ARGUMENT, "null pointer");
+  switch (entry) {
+    case LZ_CALL_GLA_DECODE_BLOCK:
+      return call(lz_gla_decode_block, words, n_words);
+    case LZ_CALL_SWA_DECODE_BLOCK:
+      return call(lz_swa_decode_block, words, n_words);
+    case LZ_CALL_VERIFY_DRAFTS:
+      return call(lz_verify_drafts, words, n_words);
+    case LZ_CALL_INT8_MATMUL:
+      return call(lz_int8_matmul, words, n_words);
+    case LZ_CALL_INT8_LINEAR:
+      return call(lz_int8_linear, words, n_words);
+  }
+  lz::set_error("unknown entry");
+  return LZ_ERR_INVALID_ARGUMENT;
 }
 
 extern "C" size_t lz_gla_saved_bytes(int B, int H, int L, int F, int D, int chunk) {

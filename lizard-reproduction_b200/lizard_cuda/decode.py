@@ -193,10 +193,10 @@ def gla_decode_block(fq, fk, v, log_gamma, state, zstate, pending=None):
         return y
     fq, fk = _lib.as_dtype(fq, torch.bfloat16), _lib.as_dtype(fk, torch.bfloat16)
     v, lg = _lib.as_dtype(v, torch.bfloat16), _lib.as_dtype(log_gamma, torch.float32)
-    rc = _lib.call(
-        index, _lib.load().lz_gla_decode_block, fq.data_ptr(), fk.data_ptr(), v.data_ptr(),
-        lg.data_ptr(), per_head, p_fk, p_v, p_lg, p_count, state.data_ptr(), zstate.data_ptr(),
-        y.data_ptr(), B, H, Hkv, Hs, T, Tp, F, D, _lib.raw_stream(index))
+    rc = _lib.call(index, _lib.CALL_GLA_DECODE_BLOCK, _gla_words(
+        fq.data_ptr(), fk.data_ptr(), v.data_ptr(), lg.data_ptr(), per_head, p_fk, p_v, p_lg,
+        p_count, state.data_ptr(), zstate.data_ptr(), y.data_ptr(), B, H, Hkv, Hs, T, Tp, F, D,
+        _lib.raw_stream(index)))
     if rc:
         _lib.check(rc, "gla decode block")
     return y
@@ -220,7 +220,10 @@ def _rows(t, dtype):
     return t if t.stride(3) == 1 else t.contiguous()
 
 
-_strides3, _strides2 = struct.Struct("12q").pack, struct.Struct("8q").pack
+_gla_words, _swa_words = struct.Struct("21q").pack, struct.Struct("52q").pack
+
+
+_NO_STRIDES = (0,) * 8
 
 
 def swa_decode_block(q, k, v, cos, sin, meta, k_ring, v_ring, pos, pending=None):
@@ -256,7 +259,7 @@ def swa_decode_block(q, k, v, cos, sin, meta, k_ring, v_ring, pos, pending=None)
     xdt = q.dtype if q.dtype in _DT else torch.float32
     cdt = cos.dtype if cos.dtype is sin.dtype and cos.dtype in _DT else torch.float32
     Tp = cp_sb = p_k = p_v = p_c = p_s = p_count = 0
-    stp = None
+    strides_p = _NO_STRIDES
     if pending is not None:
         kp, vp, cp, sp, count = pending
         if not (index == kp.get_device() == vp.get_device() == cp.get_device()
@@ -269,7 +272,7 @@ def swa_decode_block(q, k, v, cos, sin, meta, k_ring, v_ring, pos, pending=None)
         if Tp:
             cp, sp, cp_sb = _tables(cp, sp, cdt, B, Tp, D)
             kp, vp = _rows(kp, xdt), _rows(vp, xdt)
-            stp = _strides2(*kp.stride(), *vp.stride())
+            strides_p = kp.stride() + vp.stride()
             p_k, p_v, p_c, p_s = kp.data_ptr(), vp.data_ptr(), cp.data_ptr(), sp.data_ptr()
         if count is not None:
             count = _pending_count(count, B, index)
@@ -282,12 +285,13 @@ def swa_decode_block(q, k, v, cos, sin, meta, k_ring, v_ring, pos, pending=None)
     meta, pos = _lib.as_dtype(meta, torch.float32), pos.contiguous()
     size = _lib.size_query("lz_swa_decode_block_workspace_bytes", B, H, Hkv, T, D)
     ws = pos.new_empty((size + 3) // 4)
-    rc = _lib.call(
-        index, _lib.load().lz_swa_decode_block, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-        _DT[xdt], _strides3(*q.stride(), *k.stride(), *v.stride()), cos.data_ptr(),
-        sin.data_ptr(), _DT[cdt], cs_sb, p_k, p_v, stp, p_c, p_s, cp_sb, p_count,
-        k_ring.data_ptr(), v_ring.data_ptr(), pos.data_ptr(), meta.data_ptr(), meta.numel(),
-        y.data_ptr(), ws.data_ptr(), size, B, H, Hkv, T, Tp, W, D, _lib.raw_stream(index))
+    # the strides follow the 32 arguments
+    rc = _lib.call(index, _lib.CALL_SWA_DECODE_BLOCK, _swa_words(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), _DT[xdt], 32, cos.data_ptr(), sin.data_ptr(),
+        _DT[cdt], cs_sb, p_k, p_v, 44 if Tp else 0, p_c, p_s, cp_sb, p_count, k_ring.data_ptr(),
+        v_ring.data_ptr(), pos.data_ptr(), meta.data_ptr(), meta.numel(), y.data_ptr(),
+        ws.data_ptr(), size, B, H, Hkv, T, Tp, W, D, _lib.raw_stream(index), *q.stride(),
+        *k.stride(), *v.stride(), *strides_p))
     if rc:
         _lib.check(rc, "swa decode block")
     return y

@@ -12,12 +12,15 @@ NaN throughout. int8_quantize lays rows of codes out on 16-byte boundaries, the
 layout the tensor cores read in place; codes in other layouts are repacked on
 every call. There is no backward.
 """
+import struct
+
 import torch
 import torch.nn as nn
 
 from . import _lib
 
 _DT = {torch.float32: _lib.LZ_DTYPE_F32, torch.bfloat16: _lib.LZ_DTYPE_BF16}
+_words = struct.Struct("16q").pack
 
 
 def _rows(t):
@@ -101,11 +104,12 @@ def int8_matmul(a, a_scale, b, b_scale, bias=None, dtype=torch.bfloat16):
         ws = None
         if not (_aligned(ar) and _aligned(br)):
             ws = a.new_empty(_lib.size_query("lz_int8_workspace_bytes", M, N, K))
-        rc = _lib.call(
-            index, _lib.load().lz_int8_matmul, ar.data_ptr(), ar.stride(0),
-            sa.data_ptr(), br.data_ptr(), br.stride(0), sb.data_ptr(), _lib.ptr(bias),
-            0 if bias is None else _DT[bias.dtype], y.data_ptr(), _DT[dtype], _lib.ptr(ws),
-            0 if ws is None else ws.numel(), M, N, K, _lib.raw_stream(index))
+        rc = _lib.call(index, _lib.CALL_INT8_MATMUL, _words(
+            ar.data_ptr(), ar.stride(0), sa.data_ptr(), br.data_ptr(), br.stride(0),
+            sb.data_ptr(), 0 if bias is None else bias.data_ptr(),
+            0 if bias is None else _DT[bias.dtype], y.data_ptr(), _DT[dtype],
+            0 if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), M, N, K,
+            _lib.raw_stream(index)))
         if rc:
             _lib.check(rc, "int8 matmul")
     return y
@@ -137,11 +141,11 @@ def int8_linear(x, weight, weight_scale, bias=None, dtype=None):
         size = (_lib.size_query("lz_int8_linear_workspace_bytes", M, N, K) if _aligned(w)
                 else _lib.size_query("lz_int8_workspace_bytes", M, N, K))
         work = w.new_empty(size) if size else None
-        rc = _lib.call(
-            index, _lib.load().lz_int8_linear, xr.data_ptr(), _DT[xr.dtype],
-            xr.stride(0), w.data_ptr(), w.stride(0), ws.data_ptr(), _lib.ptr(bias),
-            0 if bias is None else _DT[bias.dtype], y.data_ptr(), _DT[dtype], _lib.ptr(work),
-            size, M, N, K, _lib.raw_stream(index))
+        rc = _lib.call(index, _lib.CALL_INT8_LINEAR, _words(
+            xr.data_ptr(), _DT[xr.dtype], xr.stride(0), w.data_ptr(), w.stride(0), ws.data_ptr(),
+            0 if bias is None else bias.data_ptr(), 0 if bias is None else _DT[bias.dtype],
+            y.data_ptr(), _DT[dtype], work.data_ptr() if size else 0, size, M, N, K,
+            _lib.raw_stream(index)))
         if rc:
             _lib.check(rc, "int8 linear")
     return y

@@ -3,11 +3,14 @@ from given random numbers (no counterpart in the reference, which does not
 decode). The tokens that come out follow the target's distribution exactly,
 whatever the draft; see include/lizard_cuda.h (lz_verify_drafts) for the rule.
 """
+import struct
+
 import torch
 
 from . import _lib
 
 _DT = {torch.float32: _lib.LZ_DTYPE_F32, torch.bfloat16: _lib.LZ_DTYPE_BF16}
+_words = struct.Struct("13qd9q").pack
 
 
 def _logits(t, dtype):
@@ -71,11 +74,12 @@ def verify_drafts(target_logits, draft_logits, draft_tokens, uniforms, noise, te
     size = _lib.size_query("lz_verify_drafts_workspace_bytes", B, K, V)
     ws = noise.new_empty(size // 4, dtype=torch.float32)  # whole 16-byte records
     (tb, tr, _), (db, dr, _) = t.stride(), d.stride()
-    rc = _lib.call(
-        index, _lib.load().lz_verify_drafts, t.data_ptr(), tb, tr, d.data_ptr(), db, dr,
-        _DT[xdt], tok.data_ptr(), tok.dtype is torch.int64, u.data_ptr(), e.data_ptr(),
-        e.stride(0), _lib.ptr(temp), temp_all, _lib.ptr(lengths), out.data_ptr(),
-        accepted.data_ptr(), ws.data_ptr(), size, B, K, V, _lib.raw_stream(index))
+    rc = _lib.call(index, _lib.CALL_VERIFY_DRAFTS, _words(
+        t.data_ptr(), tb, tr, d.data_ptr(), db, dr, _DT[xdt], tok.data_ptr(),
+        tok.dtype is torch.int64, u.data_ptr(), e.data_ptr(), e.stride(0),
+        0 if temp is None else temp.data_ptr(), temp_all,
+        0 if lengths is None else lengths.data_ptr(), out.data_ptr(), accepted.data_ptr(),
+        ws.data_ptr(), size, B, K, V, _lib.raw_stream(index)))
     if rc:
         _lib.check(rc, "verify drafts")
     return out, accepted

@@ -149,3 +149,34 @@ def test_a_cache_starts_token_by_token():
     assert cache.draft() is cache and cache.drafting and cache.accepted is None
     cache.settle(None)
     assert not cache.drafting
+
+
+def test_arguments_as_words(lib):
+    """lz_call: the entry's own errors, and those of the words."""
+    import struct
+
+    def call(entry, *words, n=None):
+        w = struct.pack(f"{len(words)}q", *words)
+        return lib.lz_call(entry, w, len(words) if n is None else n)
+
+    assert lib.lz_call(1, None, 21) == 1 and b"null" in _msg(lib)
+    assert call(0, *range(32)) == 1 and b"unknown entry" in _msg(lib)
+    assert call(6, *range(32)) == 1
+    p = 0x1000
+    gla = [p, p, p, p, 0, 0, 0, 0, 0, p, p, p, 2, 8, 2, 2, 4, 0, 64, 64, 0]
+    assert call(1, *gla[:20]) == 1 and b"too few words" in _msg(lib)
+    assert call(1, *gla[:13], 7, *gla[14:]) == 1 and b"divide" in _msg(lib)
+    assert call(1, *gla[:12], 1 << 32, *gla[13:]) == 1 and b"does not fit" in _msg(lib)
+    assert call(1, 0, *gla[1:]) == 1 and b"null" in _msg(lib)
+    swa = [p, p, p, 0, 32, p, p, 0, 0, 0, 0, 0, 0, 0, 0, 0, p, p, p, p, 4, p, p, 1 << 30, 2, 8, 2, 4,
+           0, 64, 64, 0]
+    bad = [0, 0, 0, 1, 0, 0, 0, 2, 0, 0, 0, 1]
+    assert len(swa) == 32
+    assert call(2, *swa, *bad, *[0] * 8) == 1 and b"contiguous" in _msg(lib)
+    assert call(2, *swa[:4], 60, *swa[5:], *bad, *[0] * 8) == 1 and b"does not fit" in _msg(lib)
+    assert call(2, *swa[:4], 0, *swa[5:], *bad, *[0] * 8) == 1 and b"null" in _msg(lib)
+    verify = struct.pack("13qd9q", p, 0, 0, p, 0, 0, 0, p, 1, p, p, 0, 0, 1.0, 0, p, p, p, 0, 2, 65, 9,
+                         0)
+    assert lib.lz_call(3, verify, 23) == 2 and b"at most 64" in _msg(lib)
+    assert call(4, p, 16, p, p, 16, p, 0, 0, p, 0, 0, 0, 4, 4, 1 << 20, 0) == 2
+    assert call(5, p, 0, 16, p, 8, p, 0, 0, p, 0, 0, 0, 4, 4, 16, 0) == 1
