@@ -698,9 +698,12 @@ __device__ __forceinline__ void store_rows(const Out& o, const unsigned char* bu
 }
 
 // Warps: 0 TMA, 1 MMA (and TMEM), 2..9 epilogue (two a lane quadrant, 128 columns each).
+// YTMA: y by TMA; a kernel of its own, since the other's stores cost this one 1.5 % (518
+// against 525 us at 32768 x 8192 x 2048 with the quantisation, back to back) unexecuted.
+template <bool YTMA>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1)
 i8_wide_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw,
-               const __grid_constant__ CUtensorMap ty, const Out o, const int ytma) {
+               const __grid_constant__ CUtensorMap ty, const Out o) {
   extern __shared__ unsigned char raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
@@ -866,7 +869,7 @@ i8_wide_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ C
         }
         if (!ends) continue;
         const int cs = n0 + c0 + 32 - per;  // first column of the staging
-        if (ytma) {
+        if constexpr (YTMA) {
           tc::fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0 && row0 < o.M && cs < o.N) {
@@ -1006,8 +1009,9 @@ int launch_wide(const Operand& x, const Operand& w, const Out& o, bool after_qua
                 o.y, o.N, o.M, (long long)o.N * es, 128 / es, 32);
   if (rc) return rc;
   if (!ytma) ty = tx;
-  static bool done[64] = {false};
-  rc = allow_smem(i8_wide_kernel, kWSmem, done);
+  static bool done[2][64] = {};
+  const auto kernel = ytma ? i8_wide_kernel<true> : i8_wide_kernel<false>;
+  rc = allow_smem(kernel, kWSmem, done[ytma]);
   if (rc) return rc;
   const long long tiles = (long long)ceil_div(o.M, 256) * ceil_div(o.N, 256);
   cudaLaunchConfig_t cfg = {};
@@ -1020,7 +1024,7 @@ int launch_wide(const Operand& x, const Operand& w, const Out& o, bool after_qua
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = after_quantize ? 1 : 0;
-  return launched(cudaLaunchKernelEx(&cfg, i8_wide_kernel, tx, tw, ty, o, ytma), "i8_wide_kernel");
+  return launched(cudaLaunchKernelEx(&cfg, kernel, tx, tw, ty, o), "i8_wide_kernel");
 }
 
 template <typename T>
