@@ -48,6 +48,7 @@ namespace {
 constexpr int kMaxBlock = 64;    // tokens a block
 constexpr int kMaxWindow = 1024;  // as the single-token step
 constexpr int kWarps = 10;        // most warps a CTA
+constexpr int kSmem = 227 * 1024;  // shared memory that a CTA can have
 
 struct Heads {  // [B, heads, T, D] in place: strides in elements, last dimension contiguous
   const void* p;
@@ -239,9 +240,9 @@ __global__ void __launch_bounds__(256) swa_rotate_kernel(const SwaBlockArgs a) {
 
 // Shared memory of the second kernel, in bytes from the 1024-aligned start.
 struct SwaSmem {
-  int k, v, nk, nv, q, stat, bar, total;
+  int k = 0, v = 0, nk = 0, nv = 0, q = 0, stat = 0, bar = 0, total = 0;
 };
-__host__ __device__ inline SwaSmem swa_smem(int DP, int QT, int part, int T, int warps) {
+__host__ __device__ constexpr SwaSmem swa_smem(int DP, int QT, int part, int T, int warps) {
   SwaSmem s;
   const int new_rows = (T + 15) & ~15;
   int n = 0;
@@ -604,28 +605,40 @@ int ring_map(CUtensorMap* m, const float* p, const SwaBlockArgs& a, int heads) {
   return LZ_OK;
 }
 
-// Ring rows in shared memory at a time: 64 KB of keys and values at most.
-int ring_part(int W, int DP) { return std::min((W + 15) & ~15, 64 * 1024 / (DP * 8)); }
+// As many warps as there are 16-key tiles (of a part of the ring and the block) for each
+// row tile, in as few equal turns as fit.
+int block_warps(int QT, int part, int T) {
+  const int tiles = part / 16 + ((T + 15) >> 4), turns = ceil_div(tiles, kWarps / QT);
+  return QT * std::max(ceil_div(tiles, turns), 4 / QT);
+}
 
+// Ring rows in shared memory at a time: 64 KB of keys and values at most, and less where a
+// long block of wide heads (D > 128, T > 48) leaves no room for that.
+int ring_part(int W, int DP, int QT, int T) {
+  int part = std::min((W + 15) & ~15, 64 * 1024 / (DP * 8));
+  while (part > 16 && swa_smem(DP, QT, part, T, block_warps(QT, part, T)).total > kSmem) part -= 16;
+  return part;
+}
+
+// A failed call as this library's error (and no longer the runtime's: a later call would
+// report it as its own).
+int failed(cudaError_t e, const char* what) {
+  set_error(std::string(what) + ": " + cudaGetErrorString(e));
+  cudaGetLastError();
+  return LZ_ERR_CUDA;
+}
 int launched(cudaError_t e, const char* what) {
-  if (e != cudaSuccess) {
-    set_error(std::string(what) + ": " + cudaGetErrorString(e));
-    return LZ_ERR_CUDA;
-  }
+  if (e != cudaSuccess) return failed(e, what);
   count_launches(1);
   return check_launch(what);
 }
 
+// What can be refused of the attention's launch: before the rotation writes the ring.
 template <int DP, int QT>
-int launch_attend(SwaBlockArgs& a, int B, cudaStream_t st) {
-  a.part = ring_part(a.W, DP);
-  const int tiles = a.part / 16 + ((a.T + 15) >> 4);
-  // as many warps as there are 16-key tiles for each row tile, in as few equal turns
-  // as fit
-  const int most_w = kWarps / QT, turns = ceil_div(tiles, most_w);
-  const int warps = QT * std::max(ceil_div(tiles, turns), 4 / QT);
+int prepare_attend(SwaBlockArgs& a, CUtensorMap& tk, CUtensorMap& tv, int B) {
+  static_assert(swa_smem(DP, QT, 16, kMaxBlock, kWarps).total <= kSmem, "every block fits");
+  a.part = ring_part(a.W, DP, QT, a.T);
   a.tma = a.D % 4 == 0 && aligned16(a.kr) && aligned16(a.vr);
-  CUtensorMap tk = {}, tv = {};
   if (a.tma) {
     int rc = ring_map(&tk, a.kr, a, B * a.Hkv);
     if (!rc) rc = ring_map(&tv, a.vr, a, B * a.Hkv);
@@ -637,13 +650,18 @@ int launch_attend(SwaBlockArgs& a, int B, cudaStream_t st) {
   if (dev < 64 && !done[dev]) {
     const int most = swa_smem(DP, QT, 64 * 1024 / (DP * 8), kMaxBlock, kWarps).total;
     cudaError_t e = cudaFuncSetAttribute(swa_block_kernel<DP, QT>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-    if (e != cudaSuccess) {
-      set_error(std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
-      return LZ_ERR_CUDA;
-    }
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         std::min(most, kSmem));
+    if (e != cudaSuccess) return failed(e, "cudaFuncSetAttribute");
     done[dev] = true;
   }
+  return LZ_OK;
+}
+
+template <int DP, int QT>
+int launch_attend(const SwaBlockArgs& a, const CUtensorMap& tk, const CUtensorMap& tv, int B,
+                  cudaStream_t st) {
+  const int warps = block_warps(QT, a.part, a.T);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ceil_div(a.rep * a.T, 16 * QT), B, a.Hkv);
   cfg.blockDim = dim3(32 * warps);
@@ -660,14 +678,17 @@ int launch_attend(SwaBlockArgs& a, int B, cudaStream_t st) {
 
 template <typename XT, int DP, int QT>
 int launch_swa_block(SwaBlockArgs& a, bool pairs, int B, cudaStream_t st) {
+  CUtensorMap tk = {}, tv = {};
+  int rc = a.T ? prepare_attend<DP, QT>(a, tk, tv, B) : LZ_OK;
+  if (rc) return rc;
   const int rows = a.T + a.Tp, per = DP / 2 / (pairs ? 2 : 1);
   const dim3 grid(ceil_div(rows * per, 256), a.Hkv, B);
   if (pairs)
     swa_rotate_kernel<XT, DP, QT, 2><<<grid, 256, 0, st>>>(a);
   else
     swa_rotate_kernel<XT, DP, QT, 1><<<grid, 256, 0, st>>>(a);
-  int rc = launched(cudaSuccess, "swa_rotate_kernel");
-  if (!rc && a.T) rc = launch_attend<DP, QT>(a, B, st);
+  rc = launched(cudaSuccess, "swa_rotate_kernel");
+  if (!rc && a.T) rc = launch_attend<DP, QT>(a, tk, tv, B, st);
   return rc;
 }
 

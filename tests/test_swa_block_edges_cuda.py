@@ -1,0 +1,32 @@
+"""The SWA block step where its sizes, sinks and types leave the usual. Reference and
+tolerances are those of test_decode_block_cuda.py."""
+import pytest
+import torch
+
+from test_decode_block_cuda import _check_swa, _swa_inputs
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _lib(built_lib):
+    import lizard_cuda
+    lizard_cuda.load()
+
+
+@pytest.mark.parametrize("B,H,Hkv,W,D,T,Tp,dtype,pos", [
+    (2, 8, 2, 64, 256, 5, 5, torch.bfloat16, [200, 9]),     # 20 query rows a group
+    (1, 4, 4, 130, 256, 64, 64, torch.float32, [77]),       # the longest block, a ring part cut short
+    (2, 2, 1, 37, 130, 49, 3, torch.float32, [20, 500]),    # the shortest block of that kind
+    (1, 2, 1, 40, 130, 48, 2, torch.bfloat16, [100]),       # and the longest of the other
+    (1, 1, 1, 16, 200, 17, 1, torch.float32, [3]),
+    (1, 4, 1, 1024, 256, 16, 4, torch.bfloat16, [4000]),    # 64 rows, the largest window
+])
+def test_heads_above_128_with_many_query_rows(B, H, Hkv, W, D, T, Tp, dtype, pos):
+    from lizard_cuda.decode import swa_decode_block
+    q, blk, pend, meta, kr, vr, pos = _swa_inputs(B, H, Hkv, W, D, T, Tp, dtype, pos, seed=D + T)
+    kr0, vr0 = kr.clone(), vr.clone()
+    y = swa_decode_block(q, *blk, meta, kr, vr, pos, pending=pend)
+    assert torch.isfinite(y).all()
+    _check_swa(y, q, blk, pend, meta, kr0, vr0, pos, kr, vr)
