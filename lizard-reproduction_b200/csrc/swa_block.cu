@@ -270,7 +270,8 @@ __device__ __noinline__ float4 alone(const bf16* q, int lo, const float* kr, con
   const float scale = rsqrtf((float)D) * kLog2e;
   float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
   for (int i = 0; i < n_meta; ++i) m = fmaxf(m, meta[i] * kLog2e);
-  for (int i = 0; i < n_meta; ++i) l += tc::ex2(meta[i] * kLog2e - m);
+  for (int i = 0; i < n_meta; ++i)  // (sinks of -inf only: m is -inf too, and they weigh nothing)
+    if (meta[i] != -INFINITY) l += tc::ex2(meta[i] * kLog2e - m);
   for (int i = 0; i < nr + t + 1 && l == l; ++i) {
     const bool own = i >= nr;
     const int back = last - i, k = own ? i - nr : i;

@@ -1,5 +1,7 @@
 """The SWA block step where its sizes, sinks and types leave the usual. Reference and
 tolerances are those of test_decode_block_cuda.py."""
+import math
+
 import pytest
 import torch
 
@@ -29,4 +31,19 @@ def test_heads_above_128_with_many_query_rows(B, H, Hkv, W, D, T, Tp, dtype, pos
     kr0, vr0 = kr.clone(), vr.clone()
     y = swa_decode_block(q, *blk, meta, kr, vr, pos, pending=pend)
     assert torch.isfinite(y).all()
+    _check_swa(y, q, blk, pend, meta, kr0, vr0, pos, kr, vr)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_sinks_of_weight_zero_beside_masked_values(bad):
+    """Sinks of -inf weigh nothing, also where an output is computed by itself because a
+    value that its token does not see is not a number."""
+    from lizard_cuda.decode import swa_decode_block
+    q, blk, pend, meta, kr, vr, pos = _swa_inputs(2, 4, 2, 16, 64, 5, 2, torch.bfloat16, [50, 3],
+                                                  seed=21)
+    meta.fill_(-math.inf)
+    blk[1][:, :, 4] = bad  # the last token: the four before do not see it
+    kr0, vr0 = kr.clone(), vr.clone()
+    y = swa_decode_block(q, *blk, meta, kr, vr, pos, pending=pend)
+    assert torch.isfinite(y[:, :, :4]).all()
     _check_swa(y, q, blk, pend, meta, kr0, vr0, pos, kr, vr)
