@@ -213,6 +213,16 @@ def _tables(cos, sin, dtype, B, T, D):
     return _lib.as_dtype(cos, dtype), _lib.as_dtype(sin, dtype), T * D if n > 1 else 0
 
 
+def _common(*tensors):
+    """The tensors' type if they share one that the kernels read, else fp32 (which holds
+    the values of all of them)."""
+    dtype = tensors[0].dtype
+    for t in tensors:
+        if t.dtype is not dtype:
+            return torch.float32
+    return dtype if dtype in _DT else torch.float32
+
+
 def _rows(t, dtype):
     """t in dtype with a contiguous last dimension, in place where it has one."""
     if t.dtype is not dtype:
@@ -236,7 +246,9 @@ def swa_decode_block(q, k, v, cos, sin, meta, k_ring, v_ring, pos, pending=None)
     sin, count) of the next call, which first writes the first count[b] (int32
     [B], None = all) of its tokens to slots (pos[b] + t) % W. pos counts the
     tokens the rings hold before the call, without the pending ones; the caller
-    then advances it by count. T = 0 only advances the rings."""
+    then advances it by count. T = 0 only advances the rings. q, k, v and the
+    pending ones are fp32 or bf16, the tables too; where types differ, or are
+    others, all are read as fp32."""
     index = q.get_device()
     if not (index == k.get_device() == v.get_device() == cos.get_device() == sin.get_device()
             == meta.get_device() == k_ring.get_device() == v_ring.get_device()
@@ -256,8 +268,8 @@ def swa_decode_block(q, k, v, cos, sin, meta, k_ring, v_ring, pos, pending=None)
                          f"{tuple(k_ring.shape)}, {v_ring.dtype} {tuple(v_ring.shape)}")
     if pos.dtype is not torch.int32 or pos.shape != (B,):
         raise ValueError("pos must be int32 [B]")
-    xdt = q.dtype if q.dtype in _DT else torch.float32
-    cdt = cos.dtype if cos.dtype is sin.dtype and cos.dtype in _DT else torch.float32
+    if pending is None:
+        xdt, cdt = _common(q, k, v), _common(cos, sin)
     Tp = cp_sb = p_k = p_v = p_c = p_s = p_count = 0
     strides_p = _NO_STRIDES
     if pending is not None:
@@ -269,6 +281,7 @@ def swa_decode_block(q, k, v, cos, sin, meta, k_ring, v_ring, pos, pending=None)
         if kp.shape != (B, Hkv, Tp, D) or vp.shape != kp.shape:
             raise ValueError(f"pending k and v must be [B, Hkv, T, D], got {tuple(kp.shape)}, "
                              f"{tuple(vp.shape)}")
+        xdt, cdt = _common(q, k, v, kp, vp), _common(cos, sin, cp, sp)
         if Tp:
             cp, sp, cp_sb = _tables(cp, sp, cdt, B, Tp, D)
             kp, vp = _rows(kp, xdt), _rows(vp, xdt)

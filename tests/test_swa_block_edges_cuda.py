@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_decode_block_cuda import _check_swa, _swa_inputs
+from test_decode_block_cuda import _check_swa, _swa_inputs, _tables
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -47,3 +47,24 @@ def test_sinks_of_weight_zero_beside_masked_values(bad):
     y = swa_decode_block(q, *blk, meta, kr, vr, pos, pending=pend)
     assert torch.isfinite(y[:, :, :4]).all()
     _check_swa(y, q, blk, pend, meta, kr0, vr0, pos, kr, vr)
+
+
+@pytest.mark.parametrize("now,before", [(torch.bfloat16, torch.float32),
+                                        (torch.float32, torch.bfloat16)])
+def test_each_block_keeps_its_own_precision(now, before):
+    """The pending block and its tables may be of another type than the block: every value
+    is read as it was given."""
+    from lizard_cuda.decode import swa_decode_block
+    q, blk, _, meta, kr, vr, pos = _swa_inputs(2, 4, 2, 16, 64, 3, 1, now, [40, 5], seed=22,
+                                               tables=now)
+    pend = _swa_inputs(2, 4, 2, 16, 64, 1, 4, before, [40, 5], seed=23, tables=before)[2]
+    blk = blk[:2] + _tables(pos + pend[4], 3, 64, now)
+    kr0, vr0 = kr.clone(), vr.clone()
+    y = swa_decode_block(q, *blk, meta, kr, vr, pos, pending=pend)
+    _check_swa(y, q, blk, pend, meta, kr0, vr0, pos, kr, vr)
+    # and within a block
+    kr, vr = kr0.clone(), vr0.clone()
+    y = swa_decode_block(q, blk[0].to(before), blk[1], blk[2].to(before), blk[3], meta, kr, vr, pos,
+                         pending=pend)
+    _check_swa(y, q, (blk[0].to(before), blk[1], blk[2].to(before), blk[3]), pend, meta, kr0, vr0,
+               pos, kr, vr)
