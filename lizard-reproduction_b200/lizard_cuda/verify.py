@@ -25,7 +25,8 @@ def verify_drafts(target_logits, draft_logits, draft_tokens, uniforms, noise, te
 
     target_logits [B, K + 1, V]: the target's logits at the K drafted positions
     and the one after. draft_logits [B, K, V]: the logits the drafted tokens
-    [B, K] (int64 or int32) were drawn from, at the same temperature. uniforms
+    [B, K] (int64 or int32) were drawn from, at the same temperature. Logits of one
+    type, bf16 or fp32, are read in place, others (and two types) as fp32. uniforms
     fp32 [B, K] in [0, 1) decide the acceptances, noise fp32 [B, V] from Exp(1)
     (torch.Tensor.exponential_) draws the token that follows. temperature: a
     number or fp32 [B]; below 1e-5 a sequence is greedy. lengths int32 [B]:
@@ -67,7 +68,9 @@ def verify_drafts(target_logits, draft_logits, draft_tokens, uniforms, noise, te
     accepted = draft_tokens.new_empty(B, dtype=torch.int32)
     if B == 0:
         return out, accepted
-    xdt = target_logits.dtype if target_logits.dtype in _DT else torch.float32
+    xdt = target_logits.dtype
+    if xdt not in _DT or K and draft_logits.dtype is not xdt:
+        xdt = torch.float32  # holds both: rounded draft logits are not what the draft drew from
     t, d = _logits(target_logits, xdt), _logits(draft_logits, xdt)
     e = _logits(noise, torch.float32)
     tok, u = draft_tokens.contiguous(), _lib.as_dtype(uniforms, torch.float32)
