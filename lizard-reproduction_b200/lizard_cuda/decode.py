@@ -325,7 +325,9 @@ class LayerCache:
     def block(self, fq, fk, v, log_gamma, q, k, cos, sin, meta, accepted):
         """Both branches' outputs for a block of new tokens, after the first
         accepted[b] tokens (int32 [B]) of the block before have been folded in; the
-        block becomes the pending one."""
+        block becomes the pending one. After an error the same call may be repeated:
+        the ring's step comes first (once more, it writes the same slots), the
+        state's, which must not happen twice, last."""
         gla_p = swa_p = None
         if self.pending is not None:
             if accepted is None:
@@ -333,16 +335,17 @@ class LayerCache:
                                  "stands")
             gla_p, swa_p = ((*p, accepted) for p in self.pending)
         v16 = _lib.as_dtype(v, torch.bfloat16)
-        y_gla = gla_decode_block(fq, fk, v16, log_gamma, self.state, self.zstate, gla_p)
         y_swa = swa_decode_block(q, k, v, cos, sin, meta, self.k_ring, self.v_ring, self.pos,
                                  swa_p)
+        y_gla = gla_decode_block(fq, fk, v16, log_gamma, self.state, self.zstate, gla_p)
         if self.pending is not None:
             self.pos += accepted
         self.pending = (fk, v16, log_gamma), (k, v, cos, sin)
         return y_gla, y_swa
 
     def settle(self, accepted):
-        """Fold the first accepted[b] tokens of the pending block in and forget the rest."""
+        """Fold the first accepted[b] tokens of the pending block in and forget the rest.
+        May be repeated after an error, as block."""
         if self.pending is None:
             return
         if accepted is None:
@@ -350,10 +353,10 @@ class LayerCache:
         (fk, v, lg), (k, v_, cos, sin) = self.pending
         H = lg.shape[1] if lg.dim() == 3 else fk.shape[1]
         fq, q = fk.new_empty(fk.shape[0], H, 0, fk.shape[3]), k[:, :, :0]
-        gla_decode_block(fq, fk[:, :, :0], v[:, :, :0], lg[..., :0], self.state, self.zstate,
-                         (fk, v, lg, accepted))
         swa_decode_block(q, q, v_[:, :, :0], cos[:, :0], sin[:, :0], cos.new_empty(0),
                          self.k_ring, self.v_ring, self.pos, (k, v_, cos, sin, accepted))
+        gla_decode_block(fq, fk[:, :, :0], v[:, :, :0], lg[..., :0], self.state, self.zstate,
+                         (fk, v, lg, accepted))
         self.pos += accepted
         self.pending = None
 

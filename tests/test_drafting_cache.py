@@ -1,0 +1,61 @@
+"""The cache of drafted decoding when a call fails, is forgotten or says too much. The two
+kernels' calls are replaced by recorders: no GPU needed."""
+import pytest
+import torch
+
+
+@pytest.fixture
+def cache(monkeypatch):
+    """A LayerCache with a pending block of 3 tokens for 2 rows, whose steps record
+    (name, count) in .calls and raise when their name is in .failing."""
+    from lizard_cuda import decode
+    B, H, T, F, D, W = 2, 2, 3, 4, 8, 16
+    c = decode.LayerCache(torch.zeros(B, H, F, D), torch.zeros(B, H, F), torch.zeros(B, H, W, D),
+                          torch.zeros(B, H, W, D), torch.tensor([20, 30], dtype=torch.int32))
+    c.calls, c.failing = [], set()
+
+    def step(name):
+        def run(*args, **kw):
+            if name in c.failing:
+                raise ValueError(f"{name} refuses")
+            pending = kw.get("pending", args[-1])
+            c.calls.append((name, None if pending is None else pending[-1].tolist()))
+            return torch.zeros(B, H, T, D)
+        return run
+
+    monkeypatch.setattr(decode, "gla_decode_block", step("gla"))
+    monkeypatch.setattr(decode, "swa_decode_block", step("swa"))
+
+    def block(accepted=None):
+        x, f = torch.zeros(B, H, T, D), torch.zeros(B, H, T, F)
+        return c.block(f, f, x, torch.zeros(B, T), x, x, torch.zeros(1, T, D), torch.zeros(1, T, D),
+                       torch.zeros(0), accepted)
+
+    c.next = block
+    block()
+    del c.calls[:]
+    return c
+
+
+def _i32(*x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("settle", [False, True])
+def test_a_refused_step_leaves_nothing_folded_in_twice(cache, settle):
+    """The ring's step (which may be repeated: it writes the same slots) comes before the
+    state's (which may not); where one refuses, pos and the pending block stay."""
+    act = cache.settle if settle else cache.next
+    before = cache.pending
+    cache.failing = {"swa"}
+    with pytest.raises(ValueError, match="swa refuses"):
+        act(_i32(1, 2))
+    assert not [n for n, _ in cache.calls if n == "gla"]
+    cache.failing = {"gla"}
+    with pytest.raises(ValueError, match="gla refuses"):
+        act(_i32(1, 2))
+    assert cache.pending is before and cache.pos.tolist() == [20, 30]
+    cache.failing = set()
+    act(_i32(1, 2))
+    assert [n for n, _ in cache.calls].count("gla") == 1 and cache.pos.tolist() == [21, 32]
+    assert (cache.pending is None) == settle
