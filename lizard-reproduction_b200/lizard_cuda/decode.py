@@ -322,6 +322,13 @@ class LayerCache:
     # GLA branch and (k, v, cos, sin) of the SWA branch
     pending: tuple = None
 
+    def _stand(self, accepted):
+        """How many tokens of the pending block stand: accepted as the kernels clamp it."""
+        if accepted is None:
+            raise ValueError("a block is pending: accepted (int32 [B]) says how much of it "
+                             "stands")
+        return accepted.clamp(0, self.pending[0][0].shape[2])
+
     def block(self, fq, fk, v, log_gamma, q, k, cos, sin, meta, accepted):
         """Both branches' outputs for a block of new tokens, after the first
         accepted[b] tokens (int32 [B]) of the block before have been folded in; the
@@ -330,16 +337,14 @@ class LayerCache:
         state's, which must not happen twice, last."""
         gla_p = swa_p = None
         if self.pending is not None:
-            if accepted is None:
-                raise ValueError("a block is pending: accepted (int32 [B]) says how much of it "
-                                 "stands")
+            stand = self._stand(accepted)
             gla_p, swa_p = ((*p, accepted) for p in self.pending)
         v16 = _lib.as_dtype(v, torch.bfloat16)
         y_swa = swa_decode_block(q, k, v, cos, sin, meta, self.k_ring, self.v_ring, self.pos,
                                  swa_p)
         y_gla = gla_decode_block(fq, fk, v16, log_gamma, self.state, self.zstate, gla_p)
         if self.pending is not None:
-            self.pos += accepted
+            self.pos += stand
         self.pending = (fk, v16, log_gamma), (k, v, cos, sin)
         return y_gla, y_swa
 
@@ -348,8 +353,7 @@ class LayerCache:
         May be repeated after an error, as block."""
         if self.pending is None:
             return
-        if accepted is None:
-            raise ValueError("accepted (int32 [B]) says how much of the pending block stands")
+        stand = self._stand(accepted)
         (fk, v, lg), (k, v_, cos, sin) = self.pending
         H = lg.shape[1] if lg.dim() == 3 else fk.shape[1]
         fq, q = fk.new_empty(fk.shape[0], H, 0, fk.shape[3]), k[:, :, :0]
@@ -357,7 +361,7 @@ class LayerCache:
                          self.k_ring, self.v_ring, self.pos, (k, v_, cos, sin, accepted))
         gla_decode_block(fq, fk[:, :, :0], v[:, :, :0], lg[..., :0], self.state, self.zstate,
                          (fk, v, lg, accepted))
-        self.pos += accepted
+        self.pos += stand
         self.pending = None
 
 

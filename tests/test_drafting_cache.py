@@ -59,3 +59,10 @@ def test_a_refused_step_leaves_nothing_folded_in_twice(cache, settle):
     act(_i32(1, 2))
     assert [n for n, _ in cache.calls].count("gla") == 1 and cache.pos.tolist() == [21, 32]
     assert (cache.pending is None) == settle
+
+
+@pytest.mark.parametrize("settle", [False, True])
+def test_pos_advances_by_what_the_kernels_fold_in(cache, settle):
+    """The kernels take counts as 0 .. the block's length; so does pos."""
+    (cache.settle if settle else cache.next)(_i32(-4, 9))
+    assert cache.pos.tolist() == [20, 33] and cache.pos.dtype == torch.int32

@@ -65,3 +65,14 @@ def test_a_call_that_was_refused_can_be_repeated(what):
     for c in (cache, clean):
         c.settle(n)
     assert _same(cache, clean) and cache.pending is None
+
+
+def test_counts_outside_the_block_are_clamped_throughout():
+    cache, first, second, meta = _cache_and_blocks()
+    clean = _copy(cache)
+    over = torch.tensor([-3, 9], dtype=torch.int32, device=DEV)
+    for c, n in ((cache, over), (clean, over.clamp(0, 4))):
+        c.block(*first, meta, None)
+        c.block(*second, meta, n)
+        c.settle(n)
+    assert _same(cache, clean)
