@@ -115,7 +115,7 @@ class LizardAttention(nn.Module):
             raise ValueError("a sequence-parallel forward does not fill a decode cache")
         if lizard_cache is not None and self.layer_idx in lizard_cache:
             layer_cache = lizard_cache[self.layer_idx]
-            if lizard_cache.drafting:
+            if getattr(lizard_cache, "drafting", False):  # a plain dict serves for tokens
                 return self.decode_block(hidden_states, position_embeddings, layer_cache,
                                          lizard_cache.accepted), None
             return self.decode(hidden_states, position_embeddings, layer_cache), None

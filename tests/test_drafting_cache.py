@@ -1,5 +1,7 @@
 """The cache of drafted decoding when a call fails, is forgotten or says too much. The two
 kernels' calls are replaced by recorders: no GPU needed."""
+import types
+
 import pytest
 import torch
 
@@ -66,3 +68,23 @@ def test_pos_advances_by_what_the_kernels_fold_in(cache, settle):
     """The kernels take counts as 0 .. the block's length; so does pos."""
     (cache.settle if settle else cache.next)(_i32(-4, 9))
     assert cache.pos.tolist() == [20, 33] and cache.pos.dtype == torch.int32
+
+
+def _layer(monkeypatch):
+    """A layer whose forms of decoding record which of them ran."""
+    from lizard_cuda.layer import LizardAttention
+    cfg = types.SimpleNamespace(hidden_size=32, num_attention_heads=4, num_key_value_heads=2)
+    layer = LizardAttention(cfg, 0, window=8, num_meta=2, feature_dim=4)
+    ran = []
+    monkeypatch.setattr(layer, "decode_block",
+                        lambda x, pe, c, accepted: ran.append(accepted) or x)
+    monkeypatch.setattr(layer, "decode", lambda x, pe, c: ran.append("token") or x)
+    return layer, ran
+
+
+def test_a_cache_may_be_a_plain_dict(cache, monkeypatch):
+    layer, ran = _layer(monkeypatch)
+    cache.pending = None
+    x = torch.zeros(2, 1, 32)
+    layer(x, None, lizard_cache={0: cache})
+    assert ran == ["token"]
