@@ -374,19 +374,28 @@ class LizardCache(dict):
 
     Drafted decoding: after draft(accepted) a call takes its tokens (up to 64) as
     one block that can be taken back. It first folds in the first accepted[b]
-    tokens (int32 [B]) of the block before, and leaves its own to the next call;
-    settle(accepted) folds them in and returns to token-by-token decoding."""
+    tokens (int32 [B]) of the block before, and leaves its own to the next call,
+    which needs a draft(accepted) of its own; settle(accepted) folds them in and
+    returns to token-by-token decoding."""
 
     drafting = False
     accepted = None
+    taken = frozenset()  # the layers that have run their block since draft()
 
     def draft(self, accepted=None):
         """The next call's tokens are a block; accepted tokens of the block before (all
         rows 0 when there is none to keep)."""
-        self.drafting, self.accepted = True, accepted
+        self.drafting, self.accepted, self.taken = True, accepted, frozenset()
         return self
+
+    def block_counts(self, layer_idx):
+        """What draft was told, for a layer about to run its block."""
+        if layer_idx in self.taken:
+            raise RuntimeError(f"layer {layer_idx} has run its block since draft(accepted): the "
+                               "next block needs a draft call that says how much of it stands")
+        return self.accepted
 
     def settle(self, accepted):
         for layer in self.values():
             layer.settle(accepted)
-        self.drafting, self.accepted = False, None
+        self.drafting, self.accepted, self.taken = False, None, frozenset()

@@ -116,8 +116,10 @@ class LizardAttention(nn.Module):
         if lizard_cache is not None and self.layer_idx in lizard_cache:
             layer_cache = lizard_cache[self.layer_idx]
             if getattr(lizard_cache, "drafting", False):  # a plain dict serves for tokens
-                return self.decode_block(hidden_states, position_embeddings, layer_cache,
-                                         lizard_cache.accepted), None
+                y = self.decode_block(hidden_states, position_embeddings, layer_cache,
+                                      lizard_cache.block_counts(self.layer_idx))
+                lizard_cache.taken |= {self.layer_idx}
+                return y, None
             return self.decode(hidden_states, position_embeddings, layer_cache), None
         x = hidden_states
         dtype = torch.promote_types(x.dtype, torch.float32)

@@ -88,3 +88,32 @@ def test_a_cache_may_be_a_plain_dict(cache, monkeypatch):
     x = torch.zeros(2, 1, 32)
     layer(x, None, lizard_cache={0: cache})
     assert ran == ["token"]
+
+
+def test_every_block_needs_a_draft_call_of_its_own(cache, monkeypatch):
+    """A second call would fold the newer block in with the older one's counts."""
+    from lizard_cuda.decode import LizardCache
+    layer, ran = _layer(monkeypatch)
+    x, c = torch.zeros(2, 3, 32), LizardCache({0: cache})
+    for n in (_i32(1, 2), _i32(3, 0)):
+        layer(x, None, lizard_cache=c.draft(n))
+        assert ran[-1] is n
+        with pytest.raises(RuntimeError, match="draft"):
+            layer(x, None, lizard_cache=c)
+    assert len(ran) == 2
+
+
+def test_a_block_that_failed_may_be_repeated(cache, monkeypatch):
+    from lizard_cuda.decode import LizardCache
+    layer, ran = _layer(monkeypatch)
+    x, c = torch.zeros(2, 3, 32), LizardCache({0: cache})
+
+    def refuse(*args):
+        raise ValueError("refused")
+
+    with monkeypatch.context() as m:
+        m.setattr(layer, "decode_block", refuse)
+        with pytest.raises(ValueError, match="refused"):
+            layer(x, None, lizard_cache=c.draft(_i32(1, 2)))
+    layer(x, None, lizard_cache=c)
+    assert ran[0].tolist() == [1, 2]
