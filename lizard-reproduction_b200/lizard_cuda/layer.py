@@ -174,7 +174,10 @@ class LizardAttention(nn.Module):
         """Output for new tokens hidden_states [B, T, hidden] that follow the
         tokens in `cache` (advanced in place), one token at a time: the same
         values as the full forward at those positions, within bf16 rounding.
-        position_embeddings are the new tokens' (cos, sin) [B, T, Dh]."""
+        position_embeddings are the new tokens' (cos, sin) [B, T, Dh]. A cache with a
+        block pending has to be settled first."""
+        if cache.pending is not None:
+            raise ValueError("a block is pending: settle(accepted) says how much of it stands")
         x = hidden_states
         dtype = torch.promote_types(x.dtype, torch.float32)
         q = self.heads_view(self.q_proj(x), self.heads)

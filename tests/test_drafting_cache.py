@@ -117,3 +117,18 @@ def test_a_block_that_failed_may_be_repeated(cache, monkeypatch):
             layer(x, None, lizard_cache=c.draft(_i32(1, 2)))
     layer(x, None, lizard_cache=c)
     assert ran[0].tolist() == [1, 2]
+
+
+@pytest.mark.parametrize("whole", [True, False])
+def test_a_pending_block_is_not_passed_over(cache, whole):
+    """Token by token with a block pending: refused, whichever way the layer is called."""
+    from lizard_cuda.decode import LizardCache
+    from lizard_cuda.layer import LizardAttention
+    cfg = types.SimpleNamespace(hidden_size=32, num_attention_heads=4, num_key_value_heads=2)
+    layer = LizardAttention(cfg, 0, window=8, num_meta=2, feature_dim=4)
+    x = torch.zeros(2, 1, 32)
+    with pytest.raises(ValueError, match="settle"):
+        if whole:
+            layer(x, (x, x), lizard_cache=LizardCache({0: cache}))
+        else:
+            layer.decode(x, (x, x), cache)
