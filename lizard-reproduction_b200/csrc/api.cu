@@ -90,12 +90,14 @@ struct Words {
   const long long* w;
   int n;
   bool ok;
+  const int* strides;  // how many each of the entry's arrays of strides holds
 };
 template <typename A>
 A word(Words& x, size_t i) {
   const long long v = x.w[i];
   if constexpr (std::is_same_v<A, const long long*>) {  // strides: their place in the words
-    x.ok = x.ok && v >= 0 && (v == 0 || v + 8 <= x.n);
+    const int need = *x.strides++;
+    x.ok = x.ok && v >= 0 && (v == 0 || v <= x.n - need);
     return v > 0 && x.ok ? x.w + v : nullptr;
   } else if constexpr (std::is_pointer_v<A>) {
     return reinterpret_cast<A>(static_cast<uintptr_t>(v));
@@ -111,14 +113,15 @@ A word(Words& x, size_t i) {
 template <typename... A, size_t... I>
 int call(int (*entry)(A...), Words x, std::index_sequence<I...>) {
   LZ_REQUIRE(x.n >= (int)sizeof...(A), LZ_ERR_INVALID_ARGUMENT, "too few words for the entry");
-  const std::tuple<A...> args{word<A>(x, I)...};
+  const std::tuple<A...> args{word<A>(x, I)...};  // in order
   LZ_REQUIRE(x.ok, LZ_ERR_INVALID_ARGUMENT, "a word does not fit its argument");
   return std::apply(entry, args);
 }
 template <typename... A>
-int call(int (*entry)(A...), const long long* w, int n) {
-  return call(entry, Words{w, n, true}, std::index_sequence_for<A...>());
+int call(int (*entry)(A...), const long long* w, int n, const int* strides = nullptr) {
+  return call(entry, Words{w, n, true, strides}, std::index_sequence_for<A...>());
 }
+constexpr int kSwaBlockStrides[] = {12, 8};  // of q, k, v; of k_prev, v_prev
 
 }  // namespace
 
@@ -129,7 +132,7 @@ extern "C" int lz_call(int entry, const long long* words, int n_words) {
     case LZ_CALL_GLA_DECODE_BLOCK:
       return call(lz_gla_decode_block, words, n_words);
     case LZ_CALL_SWA_DECODE_BLOCK:
-      return call(lz_swa_decode_block, words, n_words);
+      return call(lz_swa_decode_block, words, n_words, kSwaBlockStrides);
     case LZ_CALL_VERIFY_DRAFTS:
       return call(lz_verify_drafts, words, n_words);
     case LZ_CALL_INT8_MATMUL:
