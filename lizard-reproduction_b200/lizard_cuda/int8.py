@@ -118,7 +118,9 @@ def int8_matmul(a, a_scale, b, b_scale, bias=None, dtype=torch.bfloat16):
 def int8_linear(x, weight, weight_scale, bias=None, dtype=None):
     """y [..., N] = x W^T + bias with x [..., K] (fp32 or bf16) quantised row by
     row and the weight given as codes int8 [N, K] with a scale fp32 [N] for each
-    channel (int8_quantize of an nn.Linear weight), in `dtype` (x's by default)."""
+    channel (int8_quantize of an nn.Linear weight), in `dtype` (fp32 or bf16; x's by
+    default). Other float types of x are computed as fp32, whose result is then
+    rounded to x's type."""
     index = x.get_device()
     if not (index == weight.get_device() == weight_scale.get_device()
             == (index if bias is None else bias.get_device()) >= 0):
@@ -126,7 +128,10 @@ def int8_linear(x, weight, weight_scale, bias=None, dtype=None):
     _no_grad(x, weight_scale, bias)
     if x.dim() < 1:
         raise ValueError(f"x must be [..., K], got {tuple(x.shape)}")
+    given = None  # the type of the result where the kernels do not write it
     if x.dtype not in _DT:
+        if dtype is None and x.is_floating_point():
+            given = x.dtype
         x = x.float()
     lead, K, N = x.shape[:-1], x.shape[-1], weight.shape[0]
     if dtype is None:
@@ -148,7 +153,7 @@ def int8_linear(x, weight, weight_scale, bias=None, dtype=None):
             _lib.raw_stream(index)))
         if rc:
             _lib.check(rc, "int8 linear")
-    return y
+    return y if given is None else y.to(given)
 
 
 class Int8Linear(nn.Module):
@@ -165,7 +170,10 @@ class Int8Linear(nn.Module):
         self.register_buffer("codes", codes.as_strided(
             (codes.shape[0], codes.stride(0)), codes.stride()))
         self.register_buffer("scale", scale)
-        self.register_buffer("bias", None if linear.bias is None else linear.bias.detach().clone())
+        bias = linear.bias
+        if bias is not None:  # in a type that the product takes
+            bias = bias.detach().clone() if bias.dtype in _DT else bias.detach().float()
+        self.register_buffer("bias", bias)
 
     def forward(self, x):
         return int8_linear(x, self.codes[:, :self.in_features], self.scale, self.bias)
