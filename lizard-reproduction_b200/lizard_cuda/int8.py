@@ -175,6 +175,17 @@ class Int8Linear(nn.Module):
             bias = bias.detach().clone() if bias.dtype in _DT else bias.detach().float()
         self.register_buffer("bias", bias)
 
+    def _apply(self, fn, recurse=True):
+        """Casts of the module (.half(), .to(dtype)) move the scales and do not round them;
+        the bias is cast, to fp32 where the product does not take the type."""
+        scale = self.scale
+        super()._apply(fn, recurse)
+        if self.scale.dtype is not torch.float32:
+            self.scale = scale.to(self.scale.device)
+        if self.bias is not None and self.bias.dtype not in _DT:
+            self.bias = self.bias.float()
+        return self
+
     def forward(self, x):
         return int8_linear(x, self.codes[:, :self.in_features], self.scale, self.bias)
 

@@ -1,4 +1,6 @@
 """8-bit products for activations and modules of other types than fp32 and bf16."""
+import copy
+
 import pytest
 import torch
 
@@ -41,3 +43,32 @@ def test_a_module_made_of_a_half_layer(bias):
         want = int8_linear(x.float(), codes, scale, lin.bias.float() if bias else None).half()
         y = m(x)
     assert y.dtype == torch.float16 and torch.equal(y, want)
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.to(torch.bfloat16), lambda m: m.half(),
+                                  lambda m: m.double(), lambda m: m.bfloat16().float(),
+                                  lambda m: m.to(DEV, torch.bfloat16), copy.deepcopy])
+def test_the_scale_of_a_module_survives_casts(cast):
+    from lizard_cuda import Int8Linear
+    torch.manual_seed(2)
+    m = Int8Linear(torch.nn.Linear(100, 60, bias=False).to(DEV))
+    scale = m.scale.clone()
+    x = torch.randn(7, 100, device=DEV)
+    want = m(x)
+    m = cast(torch.nn.Sequential(m))[0]
+    assert m.scale.dtype == torch.float32 and torch.equal(m.scale, scale)
+    assert torch.equal(m(x), want)
+    assert m.state_dict()["scale"].data_ptr() == m.scale.data_ptr()
+
+
+def test_the_bias_of_a_module_keeps_a_type_that_the_product_takes():
+    from lizard_cuda import Int8Linear, int8_linear
+    torch.manual_seed(3)
+    lin = torch.nn.Linear(100, 60).to(DEV)
+    x = torch.randn(7, 100, device=DEV)
+    m = Int8Linear(lin).half()
+    bias = lin.bias.detach().half().float()  # the cast rounds it, as it would a linear layer's
+    assert torch.equal(m(x), int8_linear(x, m.codes[:, :100], m.scale, bias))
+    assert m(x.half()).dtype == torch.float16
+    m = Int8Linear(lin).bfloat16()
+    assert m.bias.dtype == torch.bfloat16 and m(x.bfloat16()).dtype == torch.bfloat16
