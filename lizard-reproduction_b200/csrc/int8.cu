@@ -282,6 +282,7 @@ struct Out {  // y and what scales it
   const void* x;  // x itself, rows ldx elements apart, where the product quantises it
   long long ldx;
   int x_bf16;
+  int withhold;  // a test: one load of the first stage is not issued
 };
 __device__ __forceinline__ float bias_at(const Out& o, int n) {
   if (!o.bias) return 0.f;
@@ -294,6 +295,7 @@ __device__ __forceinline__ float scaled(int acc, float sa, float sb, float bias)
 
 // -------------------------------------------------------------------- narrow
 constexpr int kNStaging = 8192;  // bytes of y on their way out: 32 tokens x 128 channels (bf16)
+constexpr int kNoSum = -2147483647 - 1;  // no sum of K <= kMaxK products: a CTA of a split gave up
 constexpr int kFuseK = 4096;  // the largest K whose tokens a CTA quantises by itself
 template <int BN, bool FUSE>
 struct Narrow {
@@ -383,11 +385,22 @@ __device__ __forceinline__ void copy_column(T* y, int N, const T* from, int rows
   }
 }
 
+// By the multiplying thread that leaves its loop after `steps` steps: waits (with a limit
+// again) for its products and for the loads of the ring of S stages, which are that far
+// ahead of it at most, so that none is on its way when the CTA leaves.
+__device__ __noinline__ void in_flight(uint64_t* full, uint64_t* empty, uint32_t S, uint32_t steps) {
+  if (steps) tc::mbar_wait(empty + (steps - 1) % S, ((steps - 1) / S) & 1, 126);
+  for (uint32_t i = steps; i < steps + S; ++i) tc::mbar_wait(full + i % S, (i / S) & 1, 127);
+}
+
 // Warps: 0 TMA, 1 MMA (and TMEM), 2..5 epilogue. split == 1: a CTA walks the (weight
 // tile, token tile) pairs blockIdx.x, + gridDim.x, ..., weight tiles fastest. split
 // > 1: clusters of `split` CTAs, one tile each, K dealt over the cluster. FUSE: x
 // itself comes in o.x, and the epilogue warps quantise it while the weights load: one
 // launch instead of two, for the few tokens of a decode step (M <= 4, K <= kFuseK).
+// A wait that gives up: the loading and the multiplying thread leave their loops, the
+// latter once nothing is in flight, the epilogue goes through all its barriers, and nothing
+// is written from then on.
 template <int BN, bool FUSE>
 __global__ void __launch_bounds__(192)
 i8_narrow_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx,
@@ -414,7 +427,9 @@ i8_narrow_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__
   uint64_t* acc_empty = acc_full + 2;  // [2]
   uint64_t* xready = acc_empty + 2;    // FUSE: the four quantising warps
   uint32_t* tptr = reinterpret_cast<uint32_t*>(xready + 1);
+  volatile int* gave_up = reinterpret_cast<volatile int*>(tptr + 1);  // an epilogue wait did
   if (tid == 0) {
+    *gave_up = 0;
     tc::mbar_init(xready, 4);
     for (int s = 0; s < S; ++s) tc::mbar_init(full + s, 1), tc::mbar_init(empty + s, 1);
     for (int i = 0; i < 2; ++i) tc::mbar_init(acc_full + i, 1), tc::mbar_init(acc_empty + i, 4);
@@ -452,17 +467,19 @@ i8_narrow_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__
     const int pre = min(nk, S), n0 = first % wt * 128;
     for (int i = 0; i < pre; ++i) {
       tc::mbar_expect_tx(full + i, P::kStage);
-      tma_load_2d(sm + (size_t)i * P::kStage, &tw, (kt0 + i) * 128, n0, full + i);
+      if (i || !o.withhold)
+        tma_load_2d(sm + (size_t)i * P::kStage, &tw, (kt0 + i) * 128, n0, full + i);
     }
     grid_dependency_wait();
     uint32_t it = 0;
-    for (int t = first; t < tiles; t += stride) {
+    bool ok = true;
+    for (int t = first; ok && t < tiles; t += stride) {
       const int n = t % wt * 128, m = t / wt * BN;
       for (int k = 0; k < nk; ++k, ++it) {
         const int s = it % S;
         unsigned char* st = sm + (size_t)s * P::kStage;
         if (it >= (uint32_t)pre) {
-          if (it >= S) tc::mbar_wait(empty + s, (it / S - 1) & 1, 120);
+          if (it >= S && !(ok = tc::mbar_wait(empty + s, (it / S - 1) & 1, 120))) break;
           tc::mbar_expect_tx(full + s, P::kStage);
           tma_load_2d(st, &tw, (kt0 + k) * 128, n, full + s);
         }
@@ -472,14 +489,15 @@ i8_narrow_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__
   } else if (warp == 1 && lane == 0) {
     constexpr uint32_t idesc = idesc_i8(128, BN);
     uint32_t it = 0, at = 0;
-    if constexpr (FUSE) tc::mbar_wait(xready, 0, 125);
-    for (int t = first; t < tiles; t += stride, ++at) {
+    bool ok = true;
+    if constexpr (FUSE) ok = tc::mbar_wait(xready, 0, 125);
+    for (int t = first; ok && t < tiles; t += stride, ++at) {
       const int buf = at & 1;
-      if (at >= 2) tc::mbar_wait(acc_empty + buf, (at / 2 - 1) & 1, 123);
+      if (at >= 2 && !(ok = tc::mbar_wait(acc_empty + buf, (at / 2 - 1) & 1, 123))) break;
       tc::tc_fence_after();
       for (int k = 0; k < nk; ++k, ++it) {
         const int s = it % S;
-        tc::mbar_wait(full + s, (it / S) & 1, 121);
+        if (!(ok = tc::mbar_wait(full + s, (it / S) & 1, 121))) break;
         tc::tc_fence_after();
         const uint32_t a0 = smem_u32(sm + (size_t)s * P::kStage);
         const uint64_t ad = tc::sdesc(a0, 0, 1024);
@@ -490,8 +508,9 @@ i8_narrow_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__
           mma_i8(tmem + buf * P::kCols, ad + 2 * q, bd + 2 * q, idesc, (k | q) != 0);
         tc::mma_commit(empty + s);
       }
-      tc::mma_commit(acc_full + buf);
+      if (ok) tc::mma_commit(acc_full + buf);
     }
+    if (!ok) in_flight(full, empty, S, it);
   } else if (warp >= 2 && split == 1) {
     const int quad = warp & 3, ch = quad * 32 + lane;  // lane = weight row n0 + ch
     const int es = o.y_bf16 ? 2 : 4, chunk = min(BN, kNStaging / (128 * es));
@@ -503,7 +522,10 @@ i8_narrow_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__
       float* sa = FUSE ? sSa : sSa + buf * BN;
       if constexpr (!FUSE)
         for (int i = tid - 64; i < BN; i += 128) sa[i] = m0 + i < o.M ? o.sa[m0 + i] : 0.f;
-      tc::mbar_wait(acc_full + buf, (at / 2) & 1, 122);
+      if (!tc::mbar_wait(acc_full + buf, (at / 2) & 1, 122)) {
+        *gave_up = 1;
+        tc::mbar_wait(acc_full + buf, (at / 2) & 1, 122);  // no product is left on its way
+      }
       tc::tc_fence_after();
       const int mt = min(BN, o.M - m0);
       for (int c0 = 0; c0 < mt; c0 += chunk) {
@@ -535,13 +557,13 @@ i8_narrow_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__
         if (ytma) {
           tc::fence_proxy_async_smem();
           tc::named_bar_sync(1, 128);
-          if (tid == 64) {
+          if (tid == 64 && !*gave_up) {
             tma_store_2d(&ty, staging, n0, m0 + c0);
             tc::bulk_commit();
           }
         } else {
           tc::named_bar_sync(1, 128);
-          if (n < o.N) {
+          if (n < o.N && !*gave_up) {
             const int rows = min(chunk, mt - c0);
             const size_t at = (size_t)(m0 + c0) * o.N + n;
             if (o.y_bf16)
@@ -563,7 +585,8 @@ i8_narrow_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__
     if (warp >= 2) {
       const int quad = warp & 3;
       grid_dependency_wait();
-      tc::mbar_wait(acc_full, 0, 124);
+      const bool live = __all_sync(0xffffffffu, tc::mbar_wait(acc_full, 0, 124));
+      if (!live) tc::mbar_wait(acc_full, 0, 124);
       tc::tc_fence_after();
 #pragma unroll 1
       for (int c0 = 0; c0 < BN; c0 += 16) {
@@ -572,7 +595,7 @@ i8_narrow_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__
         tc::tmem_wait_ld();
 #pragma unroll
         for (int c = 0; c < 16; ++c)
-          part[(c0 + c) * 128 + quad * 32 + lane] = __float_as_int(v[c]);
+          part[(c0 + c) * 128 + quad * 32 + lane] = live ? __float_as_int(v[c]) : kNoSum;
       }
     }
     cluster_sync();
@@ -582,6 +605,7 @@ i8_narrow_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__
     for (int e = rank * 192 + tid; e < quads; e += split * 192) {
       const int c = e >> 5, q = (e & 31) * 4;
       int4 sum = make_int4(0, 0, 0, 0);
+      bool lost = false;
 #pragma unroll 4
       for (int r = 0; r < split; ++r) {
         const int4 p = ld_cluster_int4(map_to_rank(base + (c * 128 + q) * 4, r));
@@ -589,6 +613,7 @@ i8_narrow_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__
         sum.y += p.y;
         sum.z += p.z;
         sum.w += p.w;
+        lost = lost || p.x == kNoSum;
       }
       const float sa = FUSE ? sSa[c] : o.sa[m0 + c];
       const int v[4] = {sum.x, sum.y, sum.z, sum.w};
@@ -599,6 +624,7 @@ i8_narrow_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__
         const int nn = min(n0 + q + i, o.N - 1);
         y[i] = scaled(v[i], sa, o.sb[nn], bias_at(o, nn));
       }
+      if (lost) continue;  // (here, so that nothing above waits for it)
       if (n0 + q + 4 <= o.N && (o.N & 3) == 0) {  // y is 16-byte aligned or ytma is off
         if (ytma && o.y_bf16)
           *reinterpret_cast<uint2*>(static_cast<bf16*>(o.y) + at) =
@@ -701,6 +727,7 @@ __device__ __forceinline__ void store_rows(const Out& o, const unsigned char* bu
 // Warps: 0 TMA, 1 MMA (and TMEM), 2..9 epilogue (two a lane quadrant, 128 columns each).
 // YTMA: y by TMA; a kernel of its own, since the other's stores cost this one 1.5 % (518
 // against 525 us at 32768 x 8192 x 2048 with the quantisation, back to back) unexecuted.
+// After a wait that gives up, as the kernel above.
 template <bool YTMA>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(320, 1)
 i8_wide_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw,
@@ -751,17 +778,19 @@ i8_wide_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ C
   if (warp == 0 && lane == 0) {
     grid_dependency_wait();
     uint32_t it = 0;
-    for (int t = cl; t < tiles; t += ncl) {
+    bool ok = true;
+    const uint32_t without = o.withhold ? 0 : ~0u;  // the step whose x is not loaded (a test)
+    for (int t = cl; ok && t < tiles; t += ncl) {
       int mt, nt;
       place(t, mt, nt);
       const int m = mt * 256 + rank * 128, n = nt * 256 + rank * 128;
       for (int k = 0; k < KT; ++k, ++it) {
         const int s = it % kWS;
-        if (it >= kWS) tc::mbar_wait(empty + s, (it / kWS - 1) & 1, 130);
+        if (it >= kWS && !(ok = tc::mbar_wait(empty + s, (it / kWS - 1) & 1, 130))) break;
         const uint32_t bar = map_to_rank(smem_u32(full + s), 0);
         if (rank == 0) tc::mbar_expect_tx(full + s, 2 * kWStage);
         unsigned char* st = sm + (size_t)s * kWStage;
-        tma_load_2d_pair(st, &tx, k * 128, m, bar);
+        if (it != without) tma_load_2d_pair(st, &tx, k * 128, m, bar);
         tma_load_2d_pair(st + kWHalf, &tw, k * 128, n, bar);
       }
     }
@@ -771,13 +800,14 @@ i8_wide_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ C
   } else if (warp == 1 && lane == 0 && rank == 0) {
     constexpr uint32_t idesc = idesc_i8(256, 256);
     uint32_t it = 0, at = 0;
-    for (int t = cl; t < tiles; t += ncl, ++at) {
+    bool ok = true;
+    for (int t = cl; ok && t < tiles; t += ncl, ++at) {
       const int buf = at & 1;
-      if (at >= 2) tc::mbar_wait(acc_empty + buf, (at / 2 - 1) & 1, 131);
+      if (at >= 2 && !(ok = tc::mbar_wait(acc_empty + buf, (at / 2 - 1) & 1, 131))) break;
       tc::tc_fence_after();
       for (int k = 0; k < KT; ++k, ++it) {
         const int s = it % kWS;
-        tc::mbar_wait(full + s, (it / kWS) & 1, 132);
+        if (!(ok = tc::mbar_wait(full + s, (it / kWS) & 1, 132))) break;
         tc::tc_fence_after();
         const uint32_t a0 = smem_u32(sm + (size_t)s * kWStage);
         const uint64_t ad = tc::sdesc(a0, 0, 1024), bd = tc::sdesc(a0 + kWHalf, 0, 1024);
@@ -786,8 +816,9 @@ i8_wide_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ C
           mma_i8_pair(tmem + buf * 256, ad + 2 * q, bd + 2 * q, idesc, (k | q) != 0);
         commit_pair(empty + s);
       }
-      commit_pair(acc_full + buf);
+      if (ok) commit_pair(acc_full + buf);
     }
+    if (!ok) in_flight(full, empty, kWS, it);  // (the loads of both CTAs)
   } else if (warp >= 2) {
     const int quad = warp & 3, col0 = (warp - 2) / 4 * 128, etid = tid - 64;
     unsigned char* buf_y = staging + (warp - 2) * 32 * 128;
@@ -798,6 +829,7 @@ i8_wide_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ C
     uint32_t at = 0;
     // a tile's scales, loaded while the one before is written
     float next_sa = 0.f, next_sb = 0.f, next_bias = 0.f;
+    bool live = true;  // no wait has given up
     const auto fetch = [&](int t) {
       int m, n;
       place(t, m, n);
@@ -818,7 +850,7 @@ i8_wide_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ C
       const float sa = next_sa;
       tc::named_bar_sync(1, 256);  // (every warp is done with the tile before the last)
       if (t + ncl < tiles) fetch(t + ncl);
-      tc::mbar_wait(acc_full + buf, (at / 2) & 1, 133);
+      live = __all_sync(0xffffffffu, tc::mbar_wait(acc_full + buf, (at / 2) & 1, 133)) && live;
       tc::tc_fence_after();
       const uint32_t ta = tmem + buf * 256 + col0 + ((uint32_t)(quad * 32) << 16);
       float v[2][32];
@@ -873,13 +905,13 @@ i8_wide_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ C
         if constexpr (YTMA) {
           tc::fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0 && row0 < o.M && cs < o.N) {
+          if (lane == 0 && row0 < o.M && cs < o.N && live) {
             tma_store_2d(&ty, buf_y, cs, row0);
             tc::bulk_commit();
           }
         } else {
           __syncwarp();
-          store_rows(o, buf_y, row0, cs);
+          if (live) store_rows(o, buf_y, row0, cs);
           __syncwarp();
         }
       }
@@ -1051,6 +1083,7 @@ int quantize(const void* x, int x_dtype, long long ldx, int8_t* codes, long long
 }
 
 std::atomic<int> g_path{0};
+std::atomic<int> g_withhold{0};  // lz_test_withhold_int8_load
 
 // Which kernel, by an estimate of both in hundredths of a us, fitted to measured
 // times (quantisation included) over M = 64 .. 2048, K = 512 .. 8192, N = 512 ..
@@ -1136,6 +1169,10 @@ extern "C" int lz_int8_set_path(int path) {
   return lz::g_path.exchange(path);
 }
 
+extern "C" int lz_test_withhold_int8_load(int on) {
+  return lz::g_withhold.exchange(on ? 1 : 0);
+}
+
 extern "C" int lz_int8_quantize(const void* x, int x_dtype, long long x_ld, void* codes,
                                 long long codes_ld, float* scale, int M, int K, void* stream) {
   using namespace lz;
@@ -1185,7 +1222,7 @@ extern "C" int lz_int8_matmul(const void* a, long long a_ld, const float* a_scal
   if (!rc) rc = as_operand(&w, b, b_ld, N, K, &ws, st);
   if (rc) return rc;
   const Out o = {a_scale, b_scale, bias, y, bias_dtype == LZ_DTYPE_BF16, y_dtype == LZ_DTYPE_BF16,
-                 M, N, K, nullptr, 0, 0};
+                 M, N, K, nullptr, 0, 0, g_withhold.load(std::memory_order_relaxed)};
   return product(x, w, o, false, st);
 }
 
@@ -1211,7 +1248,8 @@ extern "C" int lz_int8_linear(const void* x, int x_dtype, long long x_ld, const 
   if (fits && fuse_quantize(M, N, K)) {
     const Operand wo = {static_cast<const int8_t*>(w), N == 1 ? row16(K) : w_ld, N};
     const Out o = {nullptr, w_scale, bias, y, bias_dtype == LZ_DTYPE_BF16,
-                   y_dtype == LZ_DTYPE_BF16, M, N, K, x, x_ld, x_dtype == LZ_DTYPE_BF16};
+                   y_dtype == LZ_DTYPE_BF16, M, N, K, x, x_ld, x_dtype == LZ_DTYPE_BF16,
+                   g_withhold.load(std::memory_order_relaxed)};
     return launch_narrow<16, true>({nullptr, 0, M}, wo, o, false, st);
   }
   int8_t* codes = reinterpret_cast<int8_t*>(ws);
@@ -1224,6 +1262,6 @@ extern "C" int lz_int8_linear(const void* x, int x_dtype, long long x_ld, const 
   if (rc) return rc;
   const Operand xo = {codes, row16(K), M};
   const Out o = {sa, w_scale, bias, y, bias_dtype == LZ_DTYPE_BF16, y_dtype == LZ_DTYPE_BF16,
-                 M, N, K, nullptr, 0, 0};
+                 M, N, K, nullptr, 0, 0, g_withhold.load(std::memory_order_relaxed)};
   return product(xo, wo, o, true, st);
 }
