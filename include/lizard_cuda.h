@@ -76,9 +76,10 @@ int lz_device_timeout_clear(void);
  * default; leave it off outside tests. */
 int lz_test_withhold_decode_ring_copy(int on);
 
-/* The same for the 8-bit products, process-wide: one load of a CTA's first
- * stage is not issued. Returns the previous setting. */
+/* The same for the 8-bit products and for the block steps, process-wide: one
+ * load of a CTA's first stage is not issued. Return the previous setting. */
 int lz_test_withhold_int8_load(int on);
+int lz_test_withhold_block_load(int on);
 
 /* ------------------------------------------------------------------------ */
 /* GLA                                                                      */

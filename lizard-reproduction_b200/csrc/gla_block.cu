@@ -38,6 +38,7 @@
 // (q K^T) o M has the row sum as its own sum over all columns, and y = (d_t q S + a' V) /
 // sum a' with zero rows of V for z.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -58,6 +59,7 @@ struct GlaBlockArgs {
   bf16* y;
   // rep query heads a state, kvrep state heads a key/value head
   int gph, T, Tp, H, Hkv, Hs, F, D, nsl, rep, kvrep;
+  int withhold;  // a test: the state's first tile is not loaded
 };
 
 __device__ __forceinline__ void cluster_arrive() {
@@ -135,7 +137,7 @@ constexpr int kPend = 8;    // pending tokens folded in at a time
 
 // Shared memory, in bytes from the 1024-aligned start.
 struct BlockSmem {
-  int q, k, v, kw, vw, a, den, m, bar, total;
+  int q, k, v, kw, vw, a, den, m, bar, late, total;
 };
 __host__ __device__ inline BlockSmem block_smem(int KS, int HALVES, int T) {
   const int LD = 64 * KS + 8, DN = 32 * HALVES, TK = (T + 2 + 15) & ~15;
@@ -153,6 +155,7 @@ __host__ __device__ inline BlockSmem block_smem(int KS, int HALVES, int T) {
   s.den = n, n += kQRows * 8;
   s.m = n, n += (T > 0 ? T : 1) * TK * 4;
   s.bar = (n + 7) & ~7, n = s.bar + 8;
+  s.late = n, n += 4;
   s.total = n + 1024;
   return s;
 }
@@ -243,6 +246,8 @@ gla_block_kernel(const __grid_constant__ CUtensorMap ts, const GlaBlockArgs a) {
   float2* sDen = reinterpret_cast<float2*>(sm + o.den);
   float* sM = reinterpret_cast<float*>(sm + o.m);     // [T][TK]
   uint64_t* bar = reinterpret_cast<uint64_t*>(sm + o.bar);
+  // a thread gave up waiting for the state: nothing is written
+  volatile int* late = reinterpret_cast<volatile int*>(sm + o.late);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, j = lane & 3;
   const int b = blockIdx.x, s = blockIdx.y, sl = blockIdx.z, sidx = b * a.Hs + s;
   const int rep = a.rep, R = rep * T;
@@ -252,10 +257,12 @@ gla_block_kernel(const __grid_constant__ CUtensorMap ts, const GlaBlockArgs a) {
 
   if (tid == 0) {
     tc::mbar_init(bar, 1);
+    *late = 0;
     tc::fence_mbar_init();
     tc::mbar_expect_tx(bar, HALVES * tile);  // rows F .. FP and columns beyond D arrive as zeros
 #pragma unroll
-    for (int h = 0; h < HALVES; ++h) tc::tma_load_3d(sm + h * tile, &ts, d0 + 32 * h, 0, sidx, bar);
+    for (int h = 0; h < HALVES; ++h)
+      if (h || !a.withhold) tc::tma_load_3d(sm + h * tile, &ts, d0 + 32 * h, 0, sidx, bar);
   }
   // small loads: they arrive while the rest is staged
   const size_t grow = a.gph ? (size_t)b * a.H + s : (size_t)b;
@@ -350,7 +357,7 @@ gla_block_kernel(const __grid_constant__ CUtensorMap ts, const GlaBlockArgs a) {
   const int cg = warp % (2 * HALVES), fh = warp / (2 * HALVES), half = cg >> 1;
   const int c = (cg & 1) * 16 + g;  // within the 32 of its tile
   cp_async_wait_all();  // here, not at their use: after the stores below it waits for those too
-  const bool live = tc::mbar_wait(bar, 0, 95);  // after a timeout nothing is written
+  if (!tc::mbar_wait(bar, 0, 95)) *late = 1;
   // (f & 7 is 2j or 2j + 1 whatever the step: two swizzled addresses and constants)
   float *even[2], *odd[2];
 #pragma unroll
@@ -410,20 +417,21 @@ gla_block_kernel(const __grid_constant__ CUtensorMap ts, const GlaBlockArgs a) {
           unpack2(st[ks][p][i], even[i][(ks * 16 + 8 * p) * 32], odd[i][(ks * 16 + 8 * p) * 32]);
     tc::fence_proxy_async_smem();
     __syncthreads();
-    if (tid == 0 && live) {
+    if (tid == 0 && !*late) {
 #pragma unroll
       for (int h = 0; h < HALVES; ++h)
         if (d0 + 32 * h < D) tc::tma_store_3d(&ts, sm + h * tile, d0 + 32 * h, 0, sidx);
       tc::bulk_commit();
     }
     if (a.nsl > 1) cluster_wait();
-    if (sl == 0 && live)
+    if (sl == 0 && !*late)
 #pragma unroll
       for (int i = 0; i < ZN; ++i)
         if (tid + i * NT < F) Zs[tid + i * NT] = z[i];
   }
   if (!T) {
     if (tid == 0) tc::bulk_wait_read0();
+    if (tid == 0 && *late) tc::mbar_wait(bar, 0, 95);
     return;
   }
 
@@ -563,6 +571,7 @@ gla_block_kernel(const __grid_constant__ CUtensorMap ts, const GlaBlockArgs a) {
                                                    fh ? x[0][i][2] : x[1][i][2],
                                                    fh ? x[0][i][3] : x[1][i][3]);
     __syncthreads();
+    const bool live = !*late;
     float probe = 0.f;  // NaN once an output is not finite
     const int other = fh ? warp - 2 * HALVES : warp + 2 * HALVES, row = r0 + fh * 16 + g;
 #pragma unroll
@@ -588,6 +597,8 @@ gla_block_kernel(const __grid_constant__ CUtensorMap ts, const GlaBlockArgs a) {
     if (probe != 0.f) redo<KS, HALVES>(a, sm, r0);
   }
   if (tid == 0) tc::bulk_wait_read0();  // the state has left shared memory
+  // once more for a load that may still be on its way
+  if (tid == 0 && *late) tc::mbar_wait(bar, 0, 95);
 }
 
 template <int KS, int HALVES>
@@ -643,9 +654,14 @@ int launch_gla_block(const GlaBlockArgs& a, int B, cudaStream_t stream) {
 }
 
 }  // namespace
+std::atomic<int> g_withhold_block{0};  // lz_test_withhold_block_load
 int gla_block_timeout_flag(unsigned int* out) { return tc::read_timeout_flag_here(out); }
 int gla_block_timeout_clear() { return tc::clear_timeout_flag_here(); }
 }  // namespace lz
+
+extern "C" int lz_test_withhold_block_load(int on) {
+  return lz::g_withhold_block.exchange(on ? 1 : 0);
+}
 
 extern "C" int lz_gla_decode_block(const void* fq, const void* fk, const void* v,
                                    const float* log_gamma, int gate_per_head, const void* fk_prev,
@@ -700,6 +716,7 @@ extern "C" int lz_gla_decode_block(const void* fq, const void* fk, const void* v
   a.nsl = ceil_div(D, 32 * halves);
   a.rep = H / Hs;
   a.kvrep = Hs / Hkv;
+  a.withhold = g_withhold_block.load(std::memory_order_relaxed);
 #define LZ_GB(K_)                                                      \
   case K_:                                                             \
     return halves == 2 ? launch_gla_block<K_, 2>(a, B, st) \

@@ -37,12 +37,14 @@
 // 8-tile sit in rows 0 5 2 7 4 1 6 3: with the swizzle (16-byte chunk ^ row & 7)
 // both reads are then free of bank conflicts.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
 #include "tc.cuh"
 
 namespace lz {
+extern std::atomic<int> g_withhold_block;  // gla_block.cu
 namespace {
 
 constexpr int kMaxBlock = 64;    // tokens a block
@@ -71,6 +73,7 @@ struct SwaBlockArgs {
   int rep;    // query heads a key/value head
   int part;   // ring rows in shared memory at a time, a multiple of 16
   int tma;    // the rings can be read by TMA
+  int withhold;  // a test: the first keys are not loaded
 };
 
 template <typename T>
@@ -330,17 +333,19 @@ swa_block_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__
   const unsigned char* ws = a.ws + (size_t)bk * wo.total;
   constexpr int kQBytes = 2 * RQ * LQ * 2;
   uint32_t phase = 0;
+  bool live = true;  // after a timeout (of any thread) nothing is written
 
   // ring rows [p part, (p + 1) part) into sK / sV; with the first part, the queries and
   // the new keys and values
   const auto load = [&](int p) {
-    if (tid == 0 && (a.tma || !p)) {
+    if (tid == 0 && (a.tma || !p) && live) {  // (a phase that has not ended takes no other load)
       const int nb = TN * DP * 4;
       tc::mbar_expect_tx(bar, (a.tma ? 2 * part * DP * 4 : 0) + (p ? 0 : kQBytes + 2 * nb));
       if (a.tma) {
 #pragma unroll
         for (int i = 0; i < NG; ++i) {  // rows and columns beyond the ring arrive as zeros
-          tc::tma_load_3d(sK + i * part * 32, &tk, 32 * i, p * part, bk, bar);
+          if (i || p || !a.withhold)
+            tc::tma_load_3d(sK + i * part * 32, &tk, 32 * i, p * part, bk, bar);
           tc::tma_load_3d(sV + i * part * 32, &tv, 32 * i, p * part, bk, bar);
         }
       }
@@ -385,7 +390,6 @@ swa_block_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__
   // ldmatrix rows of this lane's queries, hi and lo
   const uint32_t aqh = smem_u32(sQh) + (rt * 16 + (lane & 15)) * (LQ * 2) + (lane >> 4) * 16;
   const uint32_t aql = aqh + RQ * LQ * 2;
-  bool live = true;  // after a timeout nothing is written
 
   float m[2] = {-1e30f, -1e30f}, l[2] = {0.f, 0.f}, acc[4 * NG][4];
 #pragma unroll
@@ -404,8 +408,10 @@ swa_block_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__
       load(p);
     }
     if (a.tma || !p) {
-      live = tc::mbar_wait(bar, phase, 96) && live;
-      phase ^= 1;
+      if (tc::mbar_wait(bar, phase, 96))
+        phase ^= 1;
+      else
+        live = false;
     }
     if (!a.tma) __syncthreads();
     const int held = min(max(nr - p * part, 0), part);  // rows of this part that hold a token
@@ -534,7 +540,7 @@ swa_block_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__
       sSum[warp * 16 + g + 8 * h] = l[h];
     }
   }
-  __syncthreads();
+  live = __syncthreads_and(live);
   for (int e = tid >> 4; e < RQ; e += nt >> 4) {  // a row a half warp, a lane a warp of its tile
     const int w = (lane16 * QT + (e >> 4)), at = w * 16 + (e & 15);
     const bool in = lane16 < kws;
@@ -583,6 +589,7 @@ swa_block_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__
     *reinterpret_cast<uint32_t*>(yr) = pack_bf16(x.x, x.y);
     if (d + 2 < D) *reinterpret_cast<uint32_t*>(yr + 2) = pack_bf16(x.z, x.w);
   }
+  if (tid == 0 && !live) tc::mbar_wait(bar, phase, 96);  // a late load is not left on its way
 }
 
 int ring_map(CUtensorMap* m, const float* p, const SwaBlockArgs& a, int heads) {
@@ -803,6 +810,7 @@ extern "C" int lz_swa_decode_block(const void* q, const void* k, const void* v, 
   a.W = window;
   a.D = D;
   a.rep = H / Hkv;
+  a.withhold = g_withhold_block.load(std::memory_order_relaxed);
   // two columns at a time: even strides and halves, bases on two elements
   const size_t xs = 2 * (x_dtype == LZ_DTYPE_BF16 ? 2 : 4), cs2 = 2 * (cb ? 2 : 4);
   const auto even = [](const Heads& h, size_t to) {

@@ -31,6 +31,7 @@ _SIGNATURES = {
     "lz_device_timeout_clear": (_c_int, []),
     "lz_test_withhold_decode_ring_copy": (_c_int, [_c_int]),
     "lz_test_withhold_int8_load": (_c_int, [_c_int]),
+    "lz_test_withhold_block_load": (_c_int, [_c_int]),
     "lz_gla_saved_bytes": (_c_size, [_c_int] * 6),
     "lz_gla_bwd_workspace_bytes": (_c_size, [_c_int] * 6),
     "lz_gla_fwd_workspace_bytes": (_c_size, [_c_int] * 6),
