@@ -26,10 +26,10 @@
 // output) and contracts the queries with them 32 rows at a time; the two halves of
 // F meet at the end, a row tile each. (8 columns by all of F needs no such meeting
 // but reads every key and query value twice as often from shared memory, which then
-// bounds the kernel.) Measured, 2048 states of 256 x 64, 32 query rows, 8 tokens: 81 us,
+// bounds the kernel.) Measured, 2048 states of 256 x 64, 32 query rows, 8 tokens: 82 us,
 // 4.1 TB/s of state and operands; what is left is the chain of phases of a CTA (load,
-// decays, update, products, meeting) at the two CTAs an SM that registers and shared
-// memory allow. A persistent form that loads the next state under this one's products
+// decays, update, products, meeting) at two CTAs an SM, since this form holds a warp's whole
+// share of the state and then its bf16 parts in registers at once. A persistent form that loads the next state under this one's products
 // was slower (90 us): the rows of a batch accept different numbers of tokens, and
 // CTAs handed out one by one even that out.
 // The scores of the block's keys are shared: a quarter of F a warp, added through

@@ -26,10 +26,11 @@
 // key once instead of twice, but its registers leave 16 warps an SM for 20, and
 // the nine 16-key tiles of a window of 128 and its block do not divide over eight.)
 // Measured, 128 sequences of 8 key / value heads of 64, window 128, 32 query heads, 8
-// tokens: 48 us (85 MB, 1.8 TB/s), 45 of them this kernel: a fifth of its instructions are
-// the conversions, and 1024 CTAs leave the fullest SM 8 for a mean of 6.9. The ring in
-// smaller parts (16, 32, 64 KB) or fewer warps a CTA (4 .. 8), so that more CTAs fit
-// an SM, took 47 to 55 us: a long window is cut at 64 KB.
+// tokens: 47 us (85 MB, 1.8 TB/s). Nothing is full (issue 47 %, DRAM 25 %, tensor cores
+// 16 %): a CTA waits for its ring, computes and merges, two an SM do not hide that, and 1024
+// CTAs leave the fullest SM 8 for a mean of 6.9; a fifth of the instructions are the
+// conversions. The ring in smaller parts (16, 32, 64 KB) or fewer warps a CTA (4 .. 8), so
+// that more CTAs fit an SM, took 47 to 55 us where this took 48: a long window is cut at 64 KB.
 //
 // Fragments. Within a step of 16 columns thread j takes d = 4j .. 4j+3 (the
 // queries are stored in that order), so a key is one 16-byte read; column tile i

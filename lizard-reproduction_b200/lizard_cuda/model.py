@@ -155,7 +155,8 @@ def speculative_generate(model, draft, input_ids, steps, draft_len=4, temperatur
     """Continuation of input_ids [B, L] by `steps` tokens with drafted decoding: the
     draft model proposes draft_len tokens a round, the model checks them in one
     block and adds one of its own. At temperature 0 the tokens are the model's greedy
-    ones; otherwise they follow the model's probabilities at that temperature,
+    ones (up to near ties: the logits of a block and of single steps differ by bf16
+    roundings); otherwise they follow the model's probabilities at that temperature,
     whatever the draft. Both models are Lizard models with the same vocabulary.
     Returns the tokens [B, steps], the model's cache, settled on the tokens before
     the last one it emitted (a row may run a few tokens past `steps`), and how many
