@@ -176,7 +176,7 @@ class LizardAttention(nn.Module):
         values as the full forward at those positions, within bf16 rounding.
         position_embeddings are the new tokens' (cos, sin) [B, T, Dh]. A cache with a
         block pending has to be settled first."""
-        if cache.pending is not None:
+        if getattr(cache, "pending", None) is not None:
             raise ValueError("a block is pending: settle(accepted) says how much of it stands")
         x = hidden_states
         dtype = torch.promote_types(x.dtype, torch.float32)

@@ -132,3 +132,16 @@ def test_a_pending_block_is_not_passed_over(cache, whole):
             layer(x, (x, x), lizard_cache=LizardCache({0: cache}))
         else:
             layer.decode(x, (x, x), cache)
+
+
+def test_a_cache_of_ones_own_needs_no_pending_field(cache):
+    """Token by token, the layer reads the state, the rings and pos; without a GPU it gets
+    as far as the kernels."""
+    from lizard_cuda.layer import LizardAttention
+    cfg = types.SimpleNamespace(hidden_size=32, num_attention_heads=4, num_key_value_heads=2)
+    layer = LizardAttention(cfg, 0, window=8, num_meta=2, feature_dim=4)
+    own = types.SimpleNamespace(state=cache.state, zstate=cache.zstate, k_ring=cache.k_ring,
+                                v_ring=cache.v_ring, pos=cache.pos)
+    x = torch.zeros(2, 1, 32)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        layer(x, (x, x), lizard_cache={0: own})
